@@ -554,6 +554,132 @@ int pf_engine_metrics_get(pf_engine* e, pf_engine_metrics* out);
  * registration), for stats/timing. */
 int pf_engine_executor(pf_engine* e, int32_t device_id, pf_executor** out);
 
+/* ------------------------------------------------------------------------ */
+/* Paged-cache operators: fill, read and attend over the cache that the      */
+/* transfers above move (no reference counterpart: there the inference       */
+/* engine does this)                                                         */
+/* ------------------------------------------------------------------------ */
+/* All three queue sm_100a kernels on `stream` (a cudaStream_t, NULL = legacy
+ * default stream) and return: no allocation, no synchronisation, nothing kept
+ * between calls, so they can be captured into CUDA graphs. Arguments are
+ * checked before anything is queued (PF_ERR_INVALID_ARGUMENT); what only the
+ * device knows (slots, block ids, lengths) is checked by the kernels, which
+ * skip what is out of range and, where `status` is not NULL, OR the bits below
+ * into that int32 on the device. */
+#define PF_KV_BAD_BLOCK 1  /* a block id, or a slot past the cache's end */
+#define PF_KV_BAD_LENGTH 2 /* offsets out of order, or a sequence longer than its block table */
+
+typedef enum pf_dtype {
+  PF_DTYPE_BF16 = 0,
+  PF_DTYPE_FP16 = 1,
+  PF_DTYPE_FP32 = 2,
+  PF_DTYPE_E4M3 = 3, /* OCP fp8 e4m3 codes: largest 448, no infinities */
+  PF_DTYPE_INT8 = 4  /* -127 .. 127 */
+} pf_dtype;
+
+/* K or V of one layer's cache, seen as [num_blocks, block_size, heads,
+ * head_dim] with the last axis contiguous. Strides are in elements and may be
+ * of any order, so KV-first, blocks-first and token-major buffers all fit.
+ * An 8-bit cache has one fp32 scale for each token and head (value = code *
+ * scale); a scale stride of 0 shares it (one for each block, or one in all). */
+typedef struct pf_kv_side {
+  uint64_t data;
+  uint64_t scale; /* 0 for a 16-bit cache */
+  int64_t block_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+  int64_t scale_block_stride;
+  int64_t scale_token_stride;
+  int64_t scale_head_stride;
+} pf_kv_side;
+
+typedef struct pf_kv_cache {
+  pf_kv_side key;
+  pf_kv_side value;
+  uint64_t num_blocks;
+  uint32_t block_size;
+  uint32_t heads;
+  uint32_t head_dim; /* 1 .. 256 */
+  uint32_t dtype;    /* BF16, FP16, E4M3 or INT8 */
+} pf_kv_cache;
+
+/* Dense rows [n, heads, head_dim]: strides in elements, last axis contiguous. */
+typedef struct pf_kv_rows {
+  uint64_t data;
+  int64_t token_stride;
+  int64_t head_stride;
+} pf_kv_rows;
+
+/* Writes n tokens' K and V into the slots of a cache: slot = block *
+ * block_size + offset; a negative slot is skipped (padding). Slots of one call
+ * are distinct: of two equal ones either token may be left, or a mixture. Rows
+ * are bf16, fp16 or fp32; a 16-bit cache takes them rounded to its type. An
+ * 8-bit cache takes, for each token and head,
+ *   scale = max(max|x| / q, 2^-126),  code = round(clamp(x * (1 / scale), -q, q))
+ * in fp32, with q = 448 (E4M3) or 127 (INT8), ties to even. A row that holds a
+ * NaN or an infinity reads back as NaN. With given_scales != 0 the scales are
+ * read, not written, and values beyond them saturate. */
+int pf_kv_write(int32_t device_id, const pf_kv_cache* cache,
+                const pf_kv_rows* key, const pf_kv_rows* value, uint32_t dtype,
+                const int64_t* slots, uint64_t n, int given_scales,
+                int32_t* status, void* stream);
+
+/* Reads the tokens of n_seqs sequences back as dense K and V rows of bf16, fp16
+ * or fp32: token t of sequence s, at block_table[s * table_stride + t /
+ * block_size], goes to row starts[s] + t, for every row of [starts[s],
+ * starts[s + 1]). `starts` has n_seqs + 1 offsets, in order, the last at most
+ * n_rows; rows outside them are left as they are. A token on a bad block reads
+ * as zeros. value = code * scale in fp32, rounded once. */
+int pf_kv_read(int32_t device_id, const pf_kv_cache* cache,
+               const int32_t* block_table, int64_t table_stride,
+               uint32_t max_blocks, uint32_t n_seqs, const int32_t* starts,
+               const pf_kv_rows* key, const pf_kv_rows* value, uint32_t dtype,
+               uint64_t n_rows, int32_t* status, void* stream);
+
+/* Attention of a chunk of new tokens over the cache, which already holds their
+ * K and V: sequence s has the queries q_start[s] .. q_start[s + 1] and kv_len[s]
+ * tokens in the cache, its chunk the last of them. Query i of n stands at
+ * position p = kv_len - n + i and sees the cached tokens j <= p (all of them
+ * with causal = 0) and, with window > 0, j > p - window:
+ *   s_j = scale * q . k_j,  out = sum_j exp(s_j) v_j / sum_j exp(s_j),
+ *   lse = log sum_j exp(s_j).
+ * A query that sees nothing gets zeros and lse = -inf; tokens on a bad block
+ * are not seen. Query heads are a multiple of the cache's: head h reads KV head
+ * h / (q_heads / heads). Query rows outside the sequences are left as they
+ * are. Types: queries and outputs bf16 or fp16, the cache the same type, E4M3
+ * or INT8; head_dim a multiple of 16 up to 128; rows 16-byte aligned. */
+typedef struct pf_kv_attention {
+  pf_kv_rows query;       /* [n_tokens, q_heads, head_dim] */
+  pf_kv_rows out;
+  uint64_t lse;           /* fp32 [n_tokens, q_heads], or 0 */
+  uint64_t block_table;   /* int32 [n_seqs, table_stride] */
+  int64_t table_stride;
+  uint64_t q_start;       /* int32 [n_seqs + 1] */
+  uint64_t kv_len;        /* int32 [n_seqs] */
+  uint64_t status;        /* int32, or 0 */
+  uint64_t workspace;     /* 16-byte aligned scratch of this call */
+  uint64_t workspace_bytes;
+  uint64_t n_tokens;
+  uint32_t n_seqs;
+  uint32_t max_blocks;    /* entries of a block_table row */
+  uint32_t q_heads;
+  uint32_t dtype;         /* of query and out */
+  /* Upper bounds of a sequence's queries and cached tokens, for the choice of
+   * kernel and split; results do not depend on them. 0 = not known. */
+  uint32_t max_q;
+  uint32_t max_kv;
+  float scale;
+  uint32_t causal;
+  uint32_t window;        /* 0 = none */
+  uint32_t reserved;
+} pf_kv_attention;
+
+/* Scratch that pf_kv_attention_run needs for these sizes (pointers are not read). */
+int pf_kv_attention_workspace(int32_t device_id, const pf_kv_cache* cache,
+                              const pf_kv_attention* args, uint64_t* out_bytes);
+int pf_kv_attention_run(int32_t device_id, const pf_kv_cache* cache,
+                        const pf_kv_attention* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

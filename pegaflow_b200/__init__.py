@@ -3,6 +3,8 @@
 Public surface (mirrors the reference's ``pegaflow.pegaflow`` module):
   PegaEngine, PyLoadState        in-process engine + shm load flag
   Executor, Layout, SaveSpec ... transfer executor (C ABI pf_executor_*)
+  KVCache, kv_write, kv_read,    operators on the paged cache that is moved
+  chunk_attention                (C ABI pf_kv_*)
 
 The native library is loaded on first use of any of these names, so
 ``pegaflow_b200.build`` can run before the library exists. A missing or
@@ -28,6 +30,10 @@ _EXPORTS = {
     "refcopy_load": ".transfer",
     "segment_offset": ".transfer",
     "validate": ".transfer",
+    "KVCache": ".kv",
+    "kv_write": ".kv",
+    "kv_read": ".kv",
+    "chunk_attention": ".kv",
 }
 
 __all__ = sorted(_EXPORTS)

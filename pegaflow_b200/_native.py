@@ -14,6 +14,7 @@ from ctypes import (
     Structure,
     c_char_p,
     c_double,
+    c_float,
     c_int,
     c_int32,
     c_int64,
@@ -51,6 +52,15 @@ PF_ALLOCATOR_AUTO_UNIT = 2**64 - 1
 
 PF_POOL_PINNED = 0
 PF_POOL_HOST = 1
+
+PF_DTYPE_BF16 = 0
+PF_DTYPE_FP16 = 1
+PF_DTYPE_FP32 = 2
+PF_DTYPE_E4M3 = 3
+PF_DTYPE_INT8 = 4
+
+PF_KV_BAD_BLOCK = 1
+PF_KV_BAD_LENGTH = 2
 
 
 class LayerDesc(Structure):
@@ -205,6 +215,61 @@ class EngineMetrics(Structure):
     ]
 
 
+class KvSide(Structure):
+    _fields_ = [
+        ("data", c_uint64),
+        ("scale", c_uint64),
+        ("block_stride", c_int64),
+        ("token_stride", c_int64),
+        ("head_stride", c_int64),
+        ("scale_block_stride", c_int64),
+        ("scale_token_stride", c_int64),
+        ("scale_head_stride", c_int64),
+    ]
+
+
+class KvCache(Structure):
+    _fields_ = [
+        ("key", KvSide),
+        ("value", KvSide),
+        ("num_blocks", c_uint64),
+        ("block_size", c_uint32),
+        ("heads", c_uint32),
+        ("head_dim", c_uint32),
+        ("dtype", c_uint32),
+    ]
+
+
+class KvRows(Structure):
+    _fields_ = [("data", c_uint64), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+class KvAttention(Structure):
+    _fields_ = [
+        ("query", KvRows),
+        ("out", KvRows),
+        ("lse", c_uint64),
+        ("block_table", c_uint64),
+        ("table_stride", c_int64),
+        ("q_start", c_uint64),
+        ("kv_len", c_uint64),
+        ("status", c_uint64),
+        ("workspace", c_uint64),
+        ("workspace_bytes", c_uint64),
+        ("n_tokens", c_uint64),
+        ("n_seqs", c_uint32),
+        ("max_blocks", c_uint32),
+        ("q_heads", c_uint32),
+        ("dtype", c_uint32),
+        ("max_q", c_uint32),
+        ("max_kv", c_uint32),
+        ("scale", c_float),
+        ("causal", c_uint32),
+        ("window", c_uint32),
+        ("reserved", c_uint32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "pf_last_error": (c_char_p, []),
@@ -293,6 +358,18 @@ _SIGNATURES = {
     ),
     "pf_engine_metrics_get": (c_int, [c_void_p, POINTER(EngineMetrics)]),
     "pf_engine_executor": (c_int, [c_void_p, c_int32, POINTER(c_void_p)]),
+    "pf_kv_write": (
+        c_int,
+        [c_int32, POINTER(KvCache), POINTER(KvRows), POINTER(KvRows), c_uint32, c_void_p, c_uint64, c_int, c_void_p,
+         c_void_p],
+    ),
+    "pf_kv_read": (
+        c_int,
+        [c_int32, POINTER(KvCache), c_void_p, c_int64, c_uint32, c_uint32, c_void_p, POINTER(KvRows), POINTER(KvRows),
+         c_uint32, c_uint64, c_void_p, c_void_p],
+    ),
+    "pf_kv_attention_workspace": (c_int, [c_int32, POINTER(KvCache), POINTER(KvAttention), POINTER(c_uint64)]),
+    "pf_kv_attention_run": (c_int, [c_int32, POINTER(KvCache), POINTER(KvAttention), c_void_p]),
 }
 
 SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,60 @@
+// Paged-cache operators (pf_kv_* in pegaflow.h): what the host entry points
+// and the kernels share.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "pegaflow.h"
+
+namespace pf {
+
+constexpr uint32_t kKvMaxHeadDim = 256;
+constexpr uint32_t kKvMaxAttentionDim = 128;
+// Smallest scale a quantised row gets: the smallest normal fp32, so that 1 /
+// scale is finite and a row of zeros stores zeros.
+constexpr float kKvSmallestScale = 1.17549435e-38f;
+
+inline bool kv_quantised(uint32_t dtype) { return dtype == PF_DTYPE_E4M3 || dtype == PF_DTYPE_INT8; }
+inline uint32_t kv_dtype_bytes(uint32_t dtype) {
+  return dtype == PF_DTYPE_FP32 ? 4 : kv_quantised(dtype) ? 1 : 2;
+}
+
+struct KvWriteArgs {
+  pf_kv_cache cache;
+  pf_kv_rows key;
+  pf_kv_rows value;
+  const int64_t* slots;
+  uint64_t n;
+  int32_t* status;
+  uint32_t dtype;
+  uint32_t given_scales;
+};
+
+struct KvReadArgs {
+  pf_kv_cache cache;
+  pf_kv_rows key;
+  pf_kv_rows value;
+  const int32_t* block_table;
+  const int32_t* starts;
+  int32_t* status;
+  int64_t table_stride;
+  uint64_t n_rows;
+  uint32_t max_blocks;
+  uint32_t n_seqs;
+  uint32_t dtype;
+};
+
+struct KvAttendArgs {
+  pf_kv_cache cache;
+  pf_kv_attention a;
+};
+
+cudaError_t launch_kv_write(const KvWriteArgs& args, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvReadArgs& args, cudaStream_t stream);
+
+uint64_t kv_attention_workspace(const KvAttendArgs& args, int num_sms);
+cudaError_t launch_kv_attention(const KvAttendArgs& args, int num_sms, cudaStream_t stream);
+
+}  // namespace pf
