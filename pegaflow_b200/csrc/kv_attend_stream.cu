@@ -1,0 +1,650 @@
+// Attention of few query rows over long caches (decoding): the cache is streamed
+// once, so HBM bounds it.
+//
+// For one sequence and one KV head, the rows (its queries times the heads of the
+// group) are at most 8 or 16. A CTA takes a part of the tokens for them; its four
+// warps take batches of 64 tokens in turn, each warp on its own: its running
+// maximum, its sums, its accumulators, joined at the end of the part. Parts of a
+// sequence are joined by a second kernel.
+//
+// The products are transposed, so that a warp's matrix instructions (m16n8k16)
+// have 16 tokens or 16 values on the long side and 8 rows on the short one:
+//   S^T = K Q^T (16 tokens x 8 rows),  O^T += V^T P^T (16 values x 8 rows).
+// Their sums run over the head's values and over the tokens, whose order is free:
+// a lane takes as its share of a row whatever 16 bytes it can load at once, so K
+// and V go from global memory into registers in full sectors and from there into
+// the instructions, with no shared memory in between. A V^T fragment pairs two
+// tokens' values: one byte permutation. P^T is S^T transposed: one movmatrix.
+//
+// 8-bit codes become fp16, which holds all of e4m3 and int8 exactly; the scales
+// stay in fp32: K's multiplies the score, V's the weight. Weights are rounded to
+// 16 bits for the second product, divided by a power of two that follows the
+// largest V scale, so that fp16 has its full precision at any scale. A bf16
+// query is brought into fp16's range by a power of two for each row: values down
+// to 2^-28 of the row's largest stay exact, smaller ones are off by at most 2^-39
+// of it.
+#include <algorithm>
+
+#include "kv_attend.cuh"
+#include "kv_attend_stream.h"
+
+namespace pf {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBatch = 64;  // tokens whose addresses and scales a warp stages at once
+constexpr int kStep = 16;   // tokens of one matrix instruction
+
+struct Staged {
+  int64_t key;    // element offset of the token's K row, -1 if it has none
+  int64_t value;
+  float key_scale;
+  float value_scale;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+
+// Two codes in the low (HIGH: high) 16 bits of x as two fp16 values.
+template <uint32_t STORE, bool HIGH>
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
+  uint32_t r;
+  if constexpr (STORE == PF_DTYPE_E4M3) {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(uint16_t(HIGH ? x >> 16 : x)));
+  } else {
+    // 1024 + (code + 128) as fp16 bits, then minus 1152: all exact.
+    const uint32_t biased = __byte_perm(x ^ 0x80808080u, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __floats2half2_rn(1152.0f, 1152.0f));
+    r = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return r;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_once(uint32_t (&r)[BYTES / 4], const void* p) {
+  if constexpr (BYTES == 16) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "l"(p));
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+  }
+}
+
+// Q, STORE: types. DP: head_dim rounded up to 64 or 128. NT: 8-row tiles.
+template <uint32_t Q, uint32_t STORE, int DP, int NT>
+struct Stream {
+  static constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
+  static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;  // type of the products
+  static constexpr int kElt = kQuant ? 1 : 2;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kChunk = 16 / kElt;           // values of a 16-byte load
+  static constexpr int kKeyLoads = DP * kElt / 64;   // 16-byte loads of a lane for one K row
+  static constexpr int kValueBytes = DP / 8 * kElt;  // of a lane for one V row
+  static constexpr int kValueLoad = kValueBytes < 16 ? kValueBytes : 16;
+  static constexpr int kValueLoads = kValueBytes / kValueLoad;
+  static constexpr int kTiles = DP / 16;
+  using Elem = typename KvElem<STORE>::type;
+
+  struct Shared {
+    Staged staged[kWarps][2][kBatch];
+    float o[kWarps][kRows][DP];
+    float m[kWarps][kRows];
+    float l[kWarps][kRows];
+    int bad[kRows];
+  };
+};
+
+template <uint32_t Q, uint32_t STORE, int DP, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+    kv_attend_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
+  using S = Stream<Q, STORE, DP, NT>;
+  using T = typename KvElem<Q>::type;
+  extern __shared__ __align__(16) unsigned char smem[];
+  typename S::Shared& sh = *reinterpret_cast<typename S::Shared*>(smem);
+  const pf_kv_cache& c = k.cache;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t part = blockIdx.x, head = blockIdx.y;
+  const uint32_t seq = blockIdx.z / plan.tiles;
+  const int32_t group = int32_t(k.a.q_heads / c.heads);
+  let_next_kernel_start();
+
+  const KvSeq s = kv_sequence(k, seq);
+  const int32_t rows = s.n * group;
+  // Tiles beyond the bound that the grid was made for are taken by its CTAs in turn.
+  for (int32_t row0 = int32_t(blockIdx.z % plan.tiles) * S::kRows; row0 < rows; row0 += int32_t(plan.tiles) * S::kRows) {
+    const int32_t row_last = min(rows, row0 + S::kRows) - 1;
+    const int32_t begin = kv_row_begin(k, s, row0 / group);
+    const int32_t end = kv_row_end(k, s, row_last / group);
+    const int32_t per = stream_part_tokens(plan, end - begin);
+    const int32_t lo = begin + int32_t(part) * per;
+    const int32_t hi = min(end, lo + per);
+    if (part && lo >= end) continue;
+
+    // This lane's query rows: g of each tile (as an operand), 2 t and 2 t + 1 (as results).
+    uint32_t q[NT][S::kTiles][2];
+    float f[NT][2];
+    int32_t row_lo[NT][2], row_hi[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int32_t r = row0 + n * 8 + g;
+      const bool on = r < rows;
+      const int32_t i = on ? r / group : 0;
+      const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(s.first + i) * k.a.query.token_stride +
+                   int64_t(int32_t(head) * group + (on ? r - i * group : 0)) * k.a.query.head_stride;
+      uint32_t raw[S::kTiles * 2];
+#pragma unroll
+      for (int j = 0; j < S::kKeyLoads; ++j) {
+        const int d = (t + 4 * j) * S::kChunk;
+#pragma unroll
+        for (int h = 0; h < S::kChunk / 8; ++h) {
+          const uint4 v = on && d < int(c.head_dim) ? *reinterpret_cast<const uint4*>(p + d + h * 8) : make_uint4(0, 0, 0, 0);
+          const int at = j * (S::kChunk / 2) + h * 4;
+          raw[at] = v.x, raw[at + 1] = v.y, raw[at + 2] = v.z, raw[at + 3] = v.w;
+        }
+      }
+      float unit = 1.0f;
+      if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+        // The row's largest exponent, over its four lanes.
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < S::kTiles * 2; ++j) top = max(top, max(raw[j] & 0x7fffu, (raw[j] >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(14 - e) brings it to [2^14, 2^15); both powers are kept within fp32's normal range.
+        const int e = min(max(int(top >> 7) - 127, -100), 127);
+        const float bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+        unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+#pragma unroll
+        for (int j = 0; j < S::kTiles * 2; ++j) {
+          raw[j] = pack2<false>(__uint_as_float(raw[j] << 16) * bring, __uint_as_float(raw[j] & 0xffff0000u) * bring);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < S::kTiles; ++j) q[n][j][0] = raw[2 * j], q[n][j][1] = raw[2 * j + 1];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // Row 2 t + e of the tile has its unit in lane (2 t + e) * 4.
+        f[n][e] = k.a.scale * kLog2e * __shfl_sync(0xffffffffu, unit, (2 * t + e) * 4);
+        const int32_t rr = row0 + n * 8 + 2 * t + e;
+        row_lo[n][e] = rr < rows ? kv_row_begin(k, s, rr / group) : 0;
+        row_hi[n][e] = rr < rows ? kv_row_end(k, s, rr / group) : INT32_MAX;  // a row that is none: nothing is kept of it
+      }
+    }
+    // Tokens that every row of the tile sees.
+    const int32_t all_lo = kv_row_begin(k, s, row_last / group), all_hi = kv_row_end(k, s, row0 / group);
+
+    float o[NT][S::kTiles][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < S::kTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+    }
+    uint32_t v_exp = 1;  // exponent field of the power of two that the weights are divided by
+
+    const char* key_base = reinterpret_cast<const char*>(c.key.data);
+    const char* value_base = reinterpret_cast<const char*>(c.value.data);
+
+    // Staging a batch takes three steps, so that no load is waited for at once:
+    // its tokens' blocks, then addresses and scales, then shared memory.
+    int32_t blocks[2];
+    Staged fresh[2];
+    auto stage_blocks = [&](int32_t batch) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int32_t j = lo + batch * kBatch + u * 32 + lane;
+        blocks[u] = j < hi ? kv_block(k, seq, uint32_t(j) / c.block_size) : -1;
+      }
+    };
+    auto stage_addresses = [&](int32_t batch) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Staged x{-1, -1, 0.0f, 0.0f};
+        if (blocks[u] >= 0) {
+          const int64_t b = blocks[u];
+          const int64_t at = uint32_t(lo + batch * kBatch + u * 32 + lane) % c.block_size;
+          x.key = b * c.key.block_stride + at * c.key.token_stride + int64_t(head) * c.key.head_stride;
+          x.value = b * c.value.block_stride + at * c.value.token_stride + int64_t(head) * c.value.head_stride;
+          if constexpr (S::kQuant) {
+            x.key_scale = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride +
+                                                                      int64_t(head) * c.key.scale_head_stride];
+            x.value_scale = reinterpret_cast<const float*>(
+                c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride +
+                               int64_t(head) * c.value.scale_head_stride];
+          }
+        }
+        fresh[u] = x;
+      }
+    };
+    auto stage_store = [&](int buf) {
+      sh.staged[warp][buf][lane] = fresh[0];
+      sh.staged[warp][buf][32 + lane] = fresh[1];
+      __syncwarp();
+    };
+
+    uint32_t kr[2][S::kKeyLoads][4];
+    uint32_t vr[4][S::kValueLoads][S::kValueLoad / 4];
+    auto load_keys = [&](int buf, int step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t at = sh.staged[warp][buf][step * kStep + g + 8 * h].key;
+#pragma unroll
+        for (int j = 0; j < S::kKeyLoads; ++j) {
+          const int d = (t + 4 * j) * S::kChunk;
+          if (at >= 0 && d < int(c.head_dim)) {
+            load_once<16>(kr[h][j], key_base + (at + d) * S::kElt);
+          } else {
+            kr[h][j][0] = kr[h][j][1] = kr[h][j][2] = kr[h][j][3] = 0;
+          }
+        }
+      }
+    };
+    auto load_values = [&](int buf, int step) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int64_t at = sh.staged[warp][buf][step * kStep + 2 * t + (h & 1) + 8 * (h >> 1)].value;
+#pragma unroll
+        for (int j = 0; j < S::kValueLoads; ++j) {
+          const int d = (8 * j + g) * (S::kValueLoad / S::kElt);
+          if (at >= 0 && d < int(c.head_dim)) {
+            load_once<S::kValueLoad>(vr[h][j], value_base + (at + d) * S::kElt);
+          } else {
+#pragma unroll
+            for (int w = 0; w < S::kValueLoad / 4; ++w) vr[h][j][w] = 0;
+          }
+        }
+      }
+    };
+
+    const int32_t batches = (max(0, hi - lo) + kBatch - 1) / kBatch;
+    int buf = 0;
+    if (warp < batches) {
+      stage_blocks(warp);
+      stage_addresses(warp);
+      stage_store(0);
+      load_keys(0, 0);
+      load_values(0, 0);
+    }
+    for (int32_t batch = warp; batch < batches; batch += kWarps) {
+      const bool more = batch + kWarps < batches;
+      float v_inv = 1.0f;
+      if constexpr (S::kQuant) {
+        const uint32_t mine = max(__float_as_uint(sh.staged[warp][buf][lane].value_scale) & 0x7fffffffu,
+                                  __float_as_uint(sh.staged[warp][buf][32 + lane].value_scale) & 0x7fffffffu);
+        const uint32_t e = min(__reduce_max_sync(0xffffffffu, mine) >> 23, 253u);
+        if (e > v_exp) {
+          const float keep = e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[n][i][x] *= keep;
+            }
+          }
+          v_exp = e;
+        }
+        v_inv = __uint_as_float((254 - v_exp) << 23);
+      }
+#pragma unroll
+      for (int step = 0; step < kBatch / kStep; ++step) {
+        const int32_t j0 = lo + batch * kBatch + step * kStep;
+        // S^T: c0, c1 are token g's scores for the rows 2 t and 2 t + 1, c2, c3 token g + 8's.
+        float x[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (S::kQuant) {
+            const uint32_t w0 = kr[0][i / 4][i % 4], w1 = kr[1][i / 4][i % 4];
+            a0 = codes_to_half2<STORE, false>(w0), a2 = codes_to_half2<STORE, true>(w0);
+            a1 = codes_to_half2<STORE, false>(w1), a3 = codes_to_half2<STORE, true>(w1);
+          } else {
+            a0 = kr[0][i / 2][i % 2 * 2], a2 = kr[0][i / 2][i % 2 * 2 + 1];
+            a1 = kr[1][i / 2][i % 2 * 2], a3 = kr[1][i / 2][i % 2 * 2 + 1];
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<S::kBf16>(x[n], a0, a1, a2, a3, q[n][i][0], q[n][i][1]);
+        }
+        const Staged s0 = sh.staged[warp][buf][step * kStep + g], s1 = sh.staged[warp][buf][step * kStep + g + 8];
+        // The next step's keys are on their way while this one's weights are made.
+        if (step + 1 < kBatch / kStep) {
+          load_keys(buf, step + 1);
+        } else if (more) {
+          stage_store(buf ^ 1);
+          load_keys(buf ^ 1, 0);
+        }
+        if (more && step == 0) stage_blocks(batch + kWarps);
+        if (more && step == 1) stage_addresses(batch + kWarps);
+
+        const bool masked = j0 < all_lo || j0 + kStep > all_hi || __any_sync(0xffffffffu, s0.key < 0 || s1.key < 0);
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = x[n][e] * f[n][e & 1];
+            if constexpr (S::kQuant) y *= e < 2 ? s0.key_scale : s1.key_scale;
+            if (masked) {
+              const int32_t j = j0 + g + (e < 2 ? 0 : 8);
+              if ((e < 2 ? s0.key : s1.key) < 0 || j < row_lo[n][e & 1] || j >= row_hi[n][e & 1]) y = -INFINITY;
+            }
+            x[n][e] = y;
+          }
+          raise = raise || fmaxf(x[n][0], x[n][2]) > m[n][0] + kRaise || fmaxf(x[n][1], x[n][3]) > m[n][1] + kRaise;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float keep[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(x[n][e], x[n][e + 2]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              top = fmaxf(top, m[n][e]);
+              keep[e] = top == -INFINITY ? 0.0f : fast_exp2(m[n][e] - top);
+              m[n][e] = top;
+              l[n][e] *= keep[e];
+            }
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) {
+              o[n][i][0] *= keep[0], o[n][i][1] *= keep[1], o[n][i][2] *= keep[0], o[n][i][3] *= keep[1];
+            }
+          }
+        }
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float base = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+            w[e] = fast_exp2(x[n][e] - base);
+            l[n][e & 1] += w[e];
+            if constexpr (S::kQuant) w[e] *= (e < 2 ? s0.value_scale : s1.value_scale) * v_inv;
+          }
+          p[n][0] = transpose_8x8(pack2<S::kBf16>(w[0], w[1]));
+          p[n][1] = transpose_8x8(pack2<S::kBf16>(w[2], w[3]));
+        }
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (S::kQuant) {
+            const int w = i / 2;
+            const uint32_t sel = i % 2 ? 0x7362 : 0x5140;
+            const uint32_t u = __byte_perm(vr[0][0][w], vr[1][0][w], sel), v = __byte_perm(vr[2][0][w], vr[3][0][w], sel);
+            a0 = codes_to_half2<STORE, false>(u), a1 = codes_to_half2<STORE, true>(u);
+            a2 = codes_to_half2<STORE, false>(v), a3 = codes_to_half2<STORE, true>(v);
+          } else {
+            a0 = __byte_perm(vr[0][i / 4][i % 4], vr[1][i / 4][i % 4], 0x5410);
+            a1 = __byte_perm(vr[0][i / 4][i % 4], vr[1][i / 4][i % 4], 0x7632);
+            a2 = __byte_perm(vr[2][i / 4][i % 4], vr[3][i / 4][i % 4], 0x5410);
+            a3 = __byte_perm(vr[2][i / 4][i % 4], vr[3][i / 4][i % 4], 0x7632);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<S::kBf16>(o[n][i], a0, a1, a2, a3, p[n][0], p[n][1]);
+        }
+        if (step + 1 < kBatch / kStep) {
+          load_values(buf, step + 1);
+        } else if (more) {
+          load_values(buf ^ 1, 0);
+        }
+      }
+      buf ^= 1;
+    }
+
+    // The warps' shares, then the part's: [row][value] in shared memory.
+    const float v_unit = S::kQuant ? __uint_as_float(v_exp << 23) : 1.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) {
+          sh.m[warp][n * 8 + 2 * t + e] = m[n][e];
+          sh.l[warp][n * 8 + 2 * t + e] = sum;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S::kTiles; ++i) {
+        const int d = S::kQuant ? g * (DP / 8) + 2 * i : (i / 4 * 8 + g) * 8 + i % 4 * 2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sh.o[warp][n * 8 + 2 * t + (e & 1)][d + (e >> 1)] = o[n][i][e] * v_unit;
+      }
+    }
+    if (threadIdx.x < S::kRows) sh.bad[threadIdx.x] = 0;
+    __syncthreads();
+
+    const int32_t used = stream_parts(plan, end - begin);
+    // Rows of one tile see different tokens: an infinity behind one row's end may have met its weight of zero.
+    const bool uneven = max(lo, all_lo) > lo || min(hi, all_hi) < hi;
+    auto finish = [&](int32_t r, uint32_t d, float top, float sum, float value) {
+      const int32_t i = r / group, qh = int32_t(head) * group + r - i * group;
+      const int64_t token = int64_t(s.first) + i, id = token * k.a.q_heads + qh;
+      if (used == 1) {
+        const float y = sum == 0.0f ? 0.0f : value / sum;
+        if (d < c.head_dim) {
+          reinterpret_cast<T*>(k.a.out.data)[token * k.a.out.token_stride + int64_t(qh) * k.a.out.head_stride + d] = kv_from_float<Q>(y);
+        }
+        if (d == 0 && k.a.lse) {
+          reinterpret_cast<float*>(k.a.lse)[id] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        }
+      } else {
+        float* ws = reinterpret_cast<float*>(k.a.workspace) + (id * plan.parts + part) * (DP + 4);
+        ws[4 + d] = value;
+        if (d == 0) ws[0] = top, ws[1] = sum;
+      }
+    };
+    for (int32_t e = threadIdx.x; e < S::kRows * DP; e += kThreads) {
+      const int32_t row = e / DP;
+      const uint32_t d = uint32_t(e % DP);
+      if (row0 + row >= rows) break;
+      float top = sh.m[0][row];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.m[w][row]);
+      float sum = 0.0f, value = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float keep = top == -INFINITY ? 1.0f : exp2f(sh.m[w][row] - top);
+        sum += sh.l[w][row] * keep;
+        value += sh.o[w][row][d] * keep;
+      }
+      if (uneven && sum == sum && !isfinite(value)) {
+        sh.bad[row] = 1;
+      } else {
+        finish(row0 + row, d, top, sum, value);
+      }
+    }
+    if (uneven) {
+      __syncthreads();
+      for (int row = warp; row < S::kRows; row += kWarps) {
+        if (!sh.bad[row]) continue;
+        const int32_t r = row0 + row, i = r / group;
+        float top, sum;
+        float4 v;
+        attend_row_exactly<Q, STORE>(k, seq, int64_t(s.first) + i, head * group + uint32_t(r - i * group), head,
+                                     max(lo, kv_row_begin(k, s, i)), min(hi, kv_row_end(k, s, i)), top, sum, v);
+        if (lane * 4 < DP) {
+          finish(r, lane * 4, top, sum, v.x);
+          finish(r, lane * 4 + 1, top, sum, v.y);
+          finish(r, lane * 4 + 2, top, sum, v.z);
+          finish(r, lane * 4 + 3, top, sum, v.w);
+        }
+      }
+    }
+    __syncthreads();  // shared memory is used again by the next tile
+  }
+}
+
+// Joins the parts of the rows that have several, a warp for each row: weights
+// 2^(m_part - max) over the parts' sums. Reads the parts once: HBM or L2.
+template <uint32_t Q, int DP>
+__global__ void __launch_bounds__(128) kv_join_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
+  using T = typename KvElem<Q>::type;
+  const int lane = threadIdx.x & 31;
+  const uint64_t id = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (id >= k.a.n_tokens * k.a.q_heads) return;
+  const uint32_t token = uint32_t(id / k.a.q_heads), qh = uint32_t(id % k.a.q_heads);
+  const uint32_t seq = kv_find_seq(reinterpret_cast<const int32_t*>(k.a.q_start), k.a.n_seqs, token);
+  if (seq == k.a.n_seqs) return;
+  const KvSeq s = kv_sequence(k, seq);
+  const int32_t group = int32_t(k.a.q_heads / k.cache.heads), rows = s.n * group;
+  const int32_t r = (int32_t(token) - s.first) * group + int32_t(qh) % group;
+  if (r >= rows) return;
+  const int32_t tile_rows = 8 * int32_t(plan.row_tiles);
+  const int32_t row0 = r / tile_rows * tile_rows, row_last = min(rows, row0 + tile_rows) - 1;
+  const int32_t used = stream_parts(plan, kv_row_end(k, s, row_last / group) - kv_row_begin(k, s, row0 / group));
+  if (used == 1) return;
+  wait_for_previous_kernel();
+  const float* ws = reinterpret_cast<const float*>(k.a.workspace) + id * plan.parts * (DP + 4);
+  float top = -INFINITY;
+  for (int32_t p = lane; p < used; p += 32) top = fmaxf(top, ws[int64_t(p) * (DP + 4)]);
+  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int32_t p = 0; p < used; ++p) {
+    const float* w = ws + int64_t(p) * (DP + 4);
+    const float keep = exp2f(w[0] - base);
+    sum += w[1] * keep;
+    if (lane * 4 < DP) {
+      const float4 v = *reinterpret_cast<const float4*>(w + 4 + lane * 4);
+      o.x += v.x * keep, o.y += v.y * keep, o.z += v.z * keep, o.w += v.w * keep;
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (lane * 4 < int(k.cache.head_dim)) {
+    KvPack<T, 4> y;
+    y.v[0] = kv_from_float<Q>(o.x * inv);
+    y.v[1] = kv_from_float<Q>(o.y * inv);
+    y.v[2] = kv_from_float<Q>(o.z * inv);
+    y.v[3] = kv_from_float<Q>(o.w * inv);
+    *reinterpret_cast<KvPack<T, 4>*>(reinterpret_cast<T*>(k.a.out.data) + int64_t(token) * k.a.out.token_stride +
+                                     int64_t(qh) * k.a.out.head_stride + lane * 4) = y;
+  }
+  if (lane == 0 && k.a.lse) reinterpret_cast<float*>(k.a.lse)[id] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+uint32_t most_queries(const KvAttendArgs& k) {
+  const uint64_t n = std::max<uint64_t>(1, k.a.n_tokens);
+  return static_cast<uint32_t>(k.a.max_q ? std::min<uint64_t>(k.a.max_q, n) : n);
+}
+
+template <uint32_t Q, uint32_t STORE, int DP, int NT>
+cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
+  using S = Stream<Q, STORE, DP, NT>;
+  const auto kernel = kv_attend_stream_kernel<Q, STORE, DP, NT>;
+  const int shm = int(sizeof(typename S::Shared));
+  if (shm > 48 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shm);
+    if (err != cudaSuccess) return err;
+  }
+  kernel<<<dim3(p.parts, k.cache.heads, k.a.n_seqs * p.tiles), kThreads, shm, stream>>>(k, p);
+  if (p.parts == 1) return cudaGetLastError();
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<uint32_t>((k.a.n_tokens * k.a.q_heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_join_stream_kernel<Q, DP>, k, p);
+}
+
+template <uint32_t Q, uint32_t STORE>
+cudaError_t launch_dims(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
+  if (k.cache.head_dim <= 64) {
+    return p.row_tiles == 1 ? launch_as<Q, STORE, 64, 1>(k, p, stream) : launch_as<Q, STORE, 64, 2>(k, p, stream);
+  }
+  return p.row_tiles == 1 ? launch_as<Q, STORE, 128, 1>(k, p, stream) : launch_as<Q, STORE, 128, 2>(k, p, stream);
+}
+
+template <uint32_t Q>
+cudaError_t launch_store(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
+  switch (k.cache.dtype) {
+    case PF_DTYPE_E4M3: return launch_dims<Q, PF_DTYPE_E4M3>(k, p, stream);
+    case PF_DTYPE_INT8: return launch_dims<Q, PF_DTYPE_INT8>(k, p, stream);
+    default: return launch_dims<Q, Q>(k, p, stream);
+  }
+}
+
+}  // namespace
+
+KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
+  KvStreamPlan p;
+  const uint32_t rows = most_queries(k) * (k.a.q_heads / k.cache.heads);
+  p.row_tiles = rows <= 8 ? 1 : 2;
+  p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
+  uint64_t longest = uint64_t(k.a.max_blocks) * k.cache.block_size;
+  if (k.a.max_kv) longest = std::min<uint64_t>(longest, k.a.max_kv);
+  if (k.a.window) longest = std::min<uint64_t>(longest, uint64_t(k.a.window) + most_queries(k));
+  longest = std::max<uint64_t>(longest, 1);
+  // About twelve CTAs for each SM, four rounds of the three that fit: the last round's idle share is small, and a
+  // part's start (addresses, queries) and end (joining) stay small beside its tokens.
+  const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * p.tiles * k.cache.heads);
+  uint64_t parts = std::max<uint64_t>(1, uint64_t(num_sms) * 12 / items);
+  uint64_t tokens = (longest + parts - 1) / parts;
+  tokens = (tokens + kStreamMinPart - 1) / kStreamMinPart * kStreamMinPart;
+  tokens = std::max<uint64_t>(tokens, 4 * kStreamMinPart);
+  p.part_tokens = static_cast<int32_t>(std::min<uint64_t>(tokens, 1u << 30));
+  p.parts = static_cast<uint32_t>((longest + p.part_tokens - 1) / p.part_tokens);
+  return p;
+}
+
+uint64_t stream_workspace(const KvAttendArgs& k, const KvStreamPlan& p) {
+  if (p.parts == 1) return 0;
+  const uint64_t dp = k.cache.head_dim <= 64 ? 64 : 128;
+  return k.a.n_tokens * k.a.q_heads * p.parts * (dp + 4) * sizeof(float);
+}
+
+cudaError_t launch_attend_stream(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
+  return k.a.dtype == PF_DTYPE_BF16 ? launch_store<PF_DTYPE_BF16>(k, p, stream) : launch_store<PF_DTYPE_FP16>(k, p, stream);
+}
+
+}  // namespace pf

@@ -1,0 +1,37 @@
+// How the streaming attention kernel's grid splits the work (host and device).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kv_ops.h"
+
+namespace pf {
+
+constexpr uint32_t kStreamMaxRows = 16;  // queries times heads of a group that one CTA takes
+constexpr uint32_t kStreamMinPart = 64;  // tokens: a batch of one warp
+
+struct KvStreamPlan {
+  uint32_t row_tiles;   // 8-row tiles of a CTA: 1 or 2
+  uint32_t tiles;       // CTAs side by side for a sequence's rows
+  uint32_t parts;       // CTAs along the tokens
+  int32_t part_tokens;  // tokens of a part, a multiple of kStreamMinPart
+};
+
+// Tokens of each part when `range` tokens are to be covered, and how many parts
+// that takes: the plan's, unless the bound that it was made for was too low.
+__host__ __device__ inline int32_t stream_part_tokens(const KvStreamPlan& p, int32_t range) {
+  const int32_t least = (range + int32_t(p.parts) - 1) / int32_t(p.parts);
+  return p.part_tokens > least ? p.part_tokens : least;
+}
+__host__ __device__ inline int32_t stream_parts(const KvStreamPlan& p, int32_t range) {
+  const int32_t per = stream_part_tokens(p, range);
+  return range <= per ? 1 : (range + per - 1) / per;
+}
+
+KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms);
+uint64_t stream_workspace(const KvAttendArgs& k, const KvStreamPlan& p);
+cudaError_t launch_attend_stream(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream);
+
+}  // namespace pf
