@@ -567,6 +567,7 @@ int pf_engine_executor(pf_engine* e, int32_t device_id, pf_executor** out);
  * skip what is out of range and, where `status` is not NULL, OR the bits below
  * into that int32 on the device. */
 #define PF_KV_BAD_BLOCK 1  /* a block id, or a slot past the cache's end */
+#define PF_KV_TIMED_OUT 4  /* a wait inside the kernel ran out after a second: the outputs are not valid */
 #define PF_KV_BAD_LENGTH 2 /* offsets out of order, or a sequence longer than its block table */
 
 typedef enum pf_dtype {

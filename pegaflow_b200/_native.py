@@ -61,6 +61,7 @@ PF_DTYPE_INT8 = 4
 
 PF_KV_BAD_BLOCK = 1
 PF_KV_BAD_LENGTH = 2
+PF_KV_TIMED_OUT = 4
 
 
 class LayerDesc(Structure):

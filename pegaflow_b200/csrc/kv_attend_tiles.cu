@@ -1,0 +1,952 @@
+// Attention of chunks of new tokens: the products are matrix products, and the
+// tensor cores and the exponentials bound it.
+//
+// An item (kv_attend_tiles.h) is 256 query rows (queries times the heads of a
+// group) of one sequence and KV head: two tiles of 128, so that the tensor cores
+// work for one while the other's softmax runs. For each 128 keys and each tile
+//   S = Q K^T            tcgen05.mma, Q and K in shared memory, S in TMEM
+//   P = 2^(S f - m)      a thread for each row, P in TMEM over S
+//   O += P V             tcgen05.mma, P in TMEM, V in shared memory, O in TMEM
+// and at the end O / sum(P). 128 x 128 x 128 takes the tensor cores 512 clocks, so
+// 256 x 128 keys take 2,048; their 32,768 exponentials take the special-function
+// units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
+// 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
+//
+// Warps 0-3 and 4-7: the softmax of the two tiles. 8-11: load Q, K and V (rows
+// from wherever the block table says, so by 16-byte copies and not by tensor
+// maps; any block size, stride and order). 12: issues the products. mbarriers
+// order them; every wait is bounded, and one that runs out ends the call with a
+// status bit and no hang.
+//
+// 8-bit codes become fp16, which holds all of e4m3 and int8 exactly, on the way
+// into shared memory; the scales stay in fp32 and multiply scores and weights. As
+// in the streaming kernel a bf16 query is brought into fp16's range by a power of
+// two for each row, and weights are divided by one that follows the V scales.
+#include <algorithm>
+
+#include "kv_attend.cuh"
+#include "kv_attend_tiles.h"
+
+namespace pf {
+namespace {
+
+constexpr int kSoftmaxWarps = 8;
+constexpr int kLoadWarps = 4;
+constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kInfos = 4;
+constexpr unsigned long long kWaitNs = 1000000000ull;  // 1 s for each wait
+
+// What the softmax needs to know of a tile of keys.
+struct alignas(16) KeyInfo {
+  float key_scale[kTileKeys];
+  float value_scale[kTileKeys];
+  int64_t key_at[kTileKeys];  // byte offsets of the rows, -1 for a token that is not seen
+  int64_t value_at[kTileKeys];
+  uint32_t seen[kTileKeys / 32];
+  uint32_t v_exp;             // exponent field of the power of two that the weights are divided by
+  uint32_t pad[3];
+};
+
+template <uint32_t Q, uint32_t STORE, int DP>
+struct Tiles {
+  static constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
+  static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;
+  static constexpr int kStages = DP == 128 ? 4 : 6;
+  static constexpr int kTileBytes = 128 * DP * 2;  // 128 rows of Q, K or V: DP / 64 blocks of [128][128 bytes]
+  struct Shared {
+    unsigned char q[2][kTileBytes];
+    unsigned char kv[kStages][kTileBytes];
+    KeyInfo info[kInfos];
+    float q_unit[2][kTileRows];  // by the item's parity
+    uint32_t warp_max[2][kLoadWarps];  // by the tile's parity
+    uint64_t q_full, q_empty;
+    uint64_t kv_full[kStages], kv_empty[kStages];
+    uint64_t info_full[kInfos], info_empty[kInfos];
+    uint64_t s_full[2], p_full[2], o_full[2], o_free[2], done;
+    uint32_t tmem;
+    int failed;  // a wait gave up
+    int stuck;   // the last one did
+  };
+  // TMEM columns.
+  static constexpr uint32_t kS = 0, kO = 256;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+__device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
+// Whether the phase of `parity` completed, within kWaitNs and before another
+// wait of this CTA gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* failed) {
+  if (bar_try(bar, parity)) return true;
+  const unsigned long long t0 = now_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      if (bar_try(bar, parity)) return true;
+    }
+    if (*reinterpret_cast<volatile int*>(failed)) return false;
+    if (now_ns() - t0 > kWaitNs) {
+      *reinterpret_cast<volatile int*>(failed) = 1;
+      return false;
+    }
+  }
+}
+
+// The same for a warp, as one.
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, int* failed) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, failed));
+}
+// Meets the other loading threads; whether all of them say yes.
+__device__ __forceinline__ bool loaders_agree(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(all)
+      : "r"(uint32_t(ok))
+      : "memory");
+  return all;
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+
+// Shared-memory operand in blocks of [rows][128 bytes], 16-byte pieces swizzled by
+// the row's low three bits: groups of 8 rows are 1,024 bytes apart. `across` is
+// the distance of the blocks where the instruction spans several (V: its N side).
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t across) {
+  return uint64_t((address & 0x3ffff) >> 4) | uint64_t(across >> 4) << 16 | uint64_t(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// 128 rows x n columns, fp32 result; b_rows: B is stored with its N side contiguous.
+__host__ __device__ constexpr uint32_t instruction(bool bf16, uint32_t n, bool b_rows) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+#define PF_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define PF_I4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
+__device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : PF_R4(r, 0), PF_R4(r, 4), PF_R4(r, 8), PF_R4(r, 12), PF_R4(r, 16), PF_R4(r, 20), PF_R4(r, 24), PF_R4(r, 28)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::PF_I4(r, 0),
+      PF_I4(r, 4), PF_I4(r, 8), PF_I4(r, 12), PF_I4(r, 16), PF_I4(r, 20), PF_I4(r, 24), PF_I4(r, 28), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PF_I4(r, 0),
+      PF_I4(r, 4), PF_I4(r, 8), PF_I4(r, 12), "r"(at)
+      : "memory");
+}
+// The registers are operands, so that nothing reads them before the wait.
+#define PF_RW4(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3])
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : PF_RW4(r, 0), PF_RW4(r, 4), PF_RW4(r, 8), PF_RW4(r, 12), PF_RW4(r, 16), PF_RW4(r, 20), PF_RW4(r, 24), PF_RW4(r, 28)
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+
+// Four codes as four fp16 values.
+template <uint32_t STORE>
+__device__ __forceinline__ uint2 codes_to_half4(uint32_t x) {
+  uint2 r;
+  if constexpr (STORE == PF_DTYPE_E4M3) {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.x) : "h"(uint16_t(x)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.y) : "h"(uint16_t(x >> 16)));
+  } else {
+    // 1024 + (code + 128) as fp16 bits, then minus 1152: all exact.
+    x ^= 0x80808080u;
+    const uint32_t lo = __byte_perm(x, 0x64646464u, 0x4140), hi = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off), b = __hsub2(*reinterpret_cast<const __half2*>(&hi), off);
+    r.x = *reinterpret_cast<const uint32_t*>(&a), r.y = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return r;
+}
+
+// One CTA's walk along its span: every role does it for itself.
+struct Item {
+  KvSeq s;
+  uint32_t seq;
+  int32_t head;
+  int32_t row0;    // first row of the tile within the sequence's
+  int32_t rows;    // rows of the tile
+  int32_t begin;   // tokens that its rows see
+  int32_t end;
+  int32_t units;   // of the whole item
+  int32_t unit0;   // this CTA's
+  int32_t unit1;
+  int32_t slot;    // where its part goes, -1: the item is whole
+  int32_t group;
+};
+
+struct Walk {
+  const KvAttendArgs& k;
+  int32_t seq, tile, head, unit;
+  int64_t left;
+  int32_t cta;
+  bool first;
+
+  __device__ Walk(const KvAttendArgs& args, const KvTilePlan& p) : k(args), cta(int32_t(blockIdx.x)), first(true) {
+    const char* ws = reinterpret_cast<const char*>(args.a.workspace);
+    const int4 span = *reinterpret_cast<const int4*>(ws + p.spans_at + blockIdx.x * sizeof(KvSpan));
+    seq = span.x, tile = span.y, head = span.z, unit = span.w;
+    left = span_units(reinterpret_cast<const int64_t*>(ws + p.costs_at)[args.a.n_seqs], p.ctas);
+  }
+
+  __device__ bool next(Item& it) {
+    it.group = int32_t(k.a.q_heads / k.cache.heads);
+    for (;;) {
+      if (left <= 0 || seq >= int32_t(k.a.n_seqs)) return false;
+      it.s = kv_sequence(k, uint32_t(seq));
+      it.row0 = tile * kTileRows;
+      it.rows = min(kTileRows, it.s.n * it.group - it.row0);
+      if (it.rows > 0) break;
+      ++seq, tile = 0, head = 0, unit = 0;
+    }
+    it.seq = uint32_t(seq);
+    it.head = head;
+    it.begin = kv_row_begin(k, it.s, it.row0 / it.group);
+    it.end = kv_row_end(k, it.s, (it.row0 + it.rows - 1) / it.group);
+    it.units = tile_units(it.begin, it.end);
+    it.unit0 = unit;
+    it.unit1 = int32_t(min(int64_t(it.units), unit + left));
+    left -= it.unit1 - it.unit0;
+    it.slot = it.unit0 == 0 && it.unit1 == it.units ? -1 : 2 * cta + (first ? 0 : 1);
+    first = false;
+    unit = 0;
+    if (++head == int32_t(k.cache.heads)) {
+      head = 0;
+      ++tile;  // a sequence's end is seen by the next call
+    }
+    return true;
+  }
+};
+
+// Cost of each sequence, then where each CTA's span begins. One block; a warp for
+// a sequence, its lanes over the row tiles, then a warp for each span.
+__global__ void __launch_bounds__(1024) kv_tile_spans_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan p) {
+  let_next_kernel_start();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t n_seqs = int32_t(k.a.n_seqs), heads = int32_t(k.cache.heads);
+  const int32_t group = int32_t(k.a.q_heads) / heads;
+  char* ws = reinterpret_cast<char*>(k.a.workspace);
+  int64_t* costs = reinterpret_cast<int64_t*>(ws + p.costs_at);
+  int4* spans = reinterpret_cast<int4*>(ws + p.spans_at);
+  __shared__ int64_t part[32];
+  __shared__ int64_t front;
+
+  auto units_of = [&](const KvSeq& s, int32_t tile) {
+    const int32_t last = min(s.n * group, (tile + 1) * kTileRows) - 1;
+    return tile_units(kv_row_begin(k, s, tile * kTileRows / group), kv_row_end(k, s, last / group));
+  };
+  if (threadIdx.x == 0) front = 0;
+  __syncthreads();
+  for (int32_t base = 0; base < n_seqs; base += 32) {
+    const int32_t seq = base + warp;
+    int64_t cost = 0;
+    if (seq < n_seqs) {
+      const KvSeq s = kv_sequence(k, uint32_t(seq));
+      const int32_t tiles = (s.n * group + kTileRows - 1) / kTileRows;
+      for (int32_t t = lane; t < tiles; t += 32) cost += units_of(s, t);
+      for (int w = 16; w; w >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, w);
+      cost *= heads;
+    }
+    if (lane == 0) part[warp] = cost;
+    __syncthreads();
+    if (warp == 0) {
+      const int64_t mine = part[lane];
+      int64_t sum = mine;
+      for (int w = 1; w < 32; w <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
+        if (lane >= w) sum += x;
+      }
+      const int64_t before = front;
+      if (base + lane < n_seqs) costs[base + lane] = before + sum - mine;
+      __syncwarp();
+      if (lane == 31) front = before + sum;
+    }
+    __syncthreads();
+  }
+  const int64_t total = front, span = span_units(total, p.ctas);
+  if (threadIdx.x == 0) costs[n_seqs] = total;
+  __syncthreads();
+  for (uint32_t c = uint32_t(warp); c <= p.ctas; c += 32) {
+    const int64_t at = int64_t(c) * span;
+    int4 out = make_int4(n_seqs, 0, 0, 0);
+    if (at < total) {
+      int32_t lo = 0, hi = n_seqs;  // the last sequence with costs[lo] <= at
+      while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (costs[mid] <= at) lo = mid; else hi = mid;
+      }
+      const KvSeq s = kv_sequence(k, uint32_t(lo));
+      const int32_t tiles = (s.n * group + kTileRows - 1) / kTileRows;
+      int64_t rest = at - costs[lo];
+      for (int32_t base = 0; base < tiles; base += 32) {
+        const int32_t t = base + lane;
+        const int32_t units = t < tiles ? units_of(s, t) : 0;
+        int64_t sum = int64_t(units) * heads;
+        for (int w = 1; w < 32; w <<= 1) {
+          const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
+          if (lane >= w) sum += x;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, sum > rest);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          const int32_t u = __shfl_sync(0xffffffffu, units, l);
+          const int64_t in = rest - (__shfl_sync(0xffffffffu, sum, l) - int64_t(u) * heads);
+          out = make_int4(lo, base + l, int32_t(in / u), int32_t(in % u));
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    if (lane == 0) spans[c] = out;
+  }
+}
+
+template <uint32_t Q, uint32_t STORE, int DP>
+__global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan plan) {
+  using S = Tiles<Q, STORE, DP>;
+  using T = typename KvElem<Q>::type;
+  extern __shared__ unsigned char raw_smem[];
+  typename S::Shared& sh =
+      *reinterpret_cast<typename S::Shared*>(raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const pf_kv_cache& c = k.cache;
+  int* failed = &sh.failed;
+
+  if (threadIdx.x == 0) {
+    bar_init(&sh.q_full, kLoadThreads);
+    bar_init(&sh.q_empty, 1);
+    for (int i = 0; i < S::kStages; ++i) bar_init(&sh.kv_full[i], kLoadThreads), bar_init(&sh.kv_empty[i], 1);
+    for (int i = 0; i < kInfos; ++i) bar_init(&sh.info_full[i], kLoadThreads), bar_init(&sh.info_empty[i], kSoftmaxWarps * 32);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.s_full[i], 1), bar_init(&sh.p_full[i], 128);
+      bar_init(&sh.o_full[i], 1), bar_init(&sh.o_free[i], 128);
+    }
+    bar_init(&sh.done, 1);
+    sh.failed = sh.stuck = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tmem = sh.tmem;
+  wait_for_previous_kernel();  // the spans
+  let_next_kernel_start();
+
+  Walk walk(k, plan);
+  Item it;
+
+  if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+    // ------------------------------------------------------------- loading
+    const int tid = threadIdx.x - kSoftmaxWarps * 32, lw = warp - kSoftmaxWarps;
+    uint32_t tile_no = 0, stage_no = 0, item_no = 0;
+    uint32_t pending = 0;  // filled stages (cp.async) that are not yet handed over
+    auto hand_over = [&](uint32_t stage) {
+      fence_async_shared();
+      bar_arrive(&sh.kv_full[stage % S::kStages]);
+    };
+    // Copies rows of 16-bit values; the stage is handed over when later ones are on their way.
+    auto copy_rows = [&](const int64_t* at, uint64_t data) {
+      constexpr int kPieces = DP / 8;
+      if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
+      const uint32_t base = smem_u32(sh.kv[stage_no % S::kStages]);
+      const int piece = tid % kPieces;
+      const bool there = piece * 8 < int(c.head_dim);
+#pragma unroll 4
+      for (int r = tid / kPieces; r < kTileKeys; r += kLoadThreads / kPieces) {
+        const int64_t off = at[r];
+        const bool on = there && off >= 0;
+        const uint32_t to = base + (piece >> 3) * 16384 + r * 128 + ((piece & 7) ^ (r & 7)) * 16;
+        const char* from = reinterpret_cast<const char*>(data) + (on ? off + piece * 16 : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++stage_no;
+      if (++pending == 3) {
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        hand_over(stage_no - 3);
+        --pending;
+      }
+      return true;
+    };
+    auto flush = [&] {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      for (; pending; --pending) hand_over(stage_no - pending);
+    };
+    // Rows of codes: loaded ahead into registers, written as fp16.
+    constexpr int kCodePieces = DP / 16;  // 16-byte loads of a row
+    constexpr int kCodeRows = kLoadThreads / kCodePieces;
+    constexpr int kCodeLoads = kTileKeys / kCodeRows;
+    uint4 codes[S::kQuant ? kCodeLoads : 1];
+    auto load_codes = [&](const int64_t* at, uint64_t data) {
+      const int piece = tid % kCodePieces;
+      const bool there = piece * 16 < int(c.head_dim);
+#pragma unroll
+      for (int i = 0; i < kCodeLoads; ++i) {
+        const int64_t off = at[tid / kCodePieces + i * kCodeRows];
+        codes[i] = there && off >= 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(data) + off + piece * 16)
+                                     : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store_codes = [&]() -> bool {
+      if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
+      unsigned char* base = sh.kv[stage_no % S::kStages];
+      const int piece = tid % kCodePieces * 2;  // of 16 bytes of fp16
+#pragma unroll
+      for (int i = 0; i < kCodeLoads; ++i) {
+        const int r = tid / kCodePieces + i * kCodeRows;
+        const uint2 a = codes_to_half4<STORE>(codes[i].x), b = codes_to_half4<STORE>(codes[i].y);
+        const uint2 e = codes_to_half4<STORE>(codes[i].z), d = codes_to_half4<STORE>(codes[i].w);
+        unsigned char* row = base + (piece >> 3) * 16384 + r * 128;
+        *reinterpret_cast<uint4*>(row + ((piece & 7) ^ (r & 7)) * 16) = make_uint4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<uint4*>(row + (((piece & 7) + 1) ^ (r & 7)) * 16) = make_uint4(e.x, e.y, d.x, d.y);
+      }
+      hand_over(stage_no++);
+      return true;
+    };
+
+    // A thread whose wait gave up goes on without copying to the next place where all loading threads meet.
+    bool ok = true;
+    while (loaders_agree(ok) && walk.next(it)) {
+      // Q: a thread for each row of both tiles. All that is filled is handed over before waiting for the
+      // products that read the last item's.
+      if constexpr (!S::kQuant) flush();
+      ok = loaders_agree(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
+      if (!ok) break;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int r = h * 128 + tid;
+        const bool on = r < it.rows;
+        if (h * 128 >= it.rows) break;
+        const int32_t row = it.row0 + (on ? r : 0), i = row / it.group;
+        const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(it.s.first + i) * k.a.query.token_stride +
+                     int64_t(it.head * it.group + row - i * it.group) * k.a.query.head_stride;
+        const uint32_t flip = k.a.scale < 0.0f ? 0x80008000u : 0u;
+        float bring = 1.0f, unit = 1.0f;
+        if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+          uint32_t top = 0;
+          for (int d = 0; d < int(c.head_dim); d += 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + d);
+            for (uint32_t x : {v.x, v.y, v.z, v.w}) top = max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu));
+          }
+          const int e = min(max(int(top >> 7) - 127, -100), 127);
+          bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+          unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+        }
+        sh.q_unit[item_no & 1][r] = unit;
+#pragma unroll 4
+        for (int piece = 0; piece < DP / 8; ++piece) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (on && piece * 8 < int(c.head_dim)) {
+            v = *reinterpret_cast<const uint4*>(p + piece * 8);
+            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+            if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+              auto to_half = [&](uint32_t x) {
+                return pack_pair<false>(__uint_as_float(x << 16) * bring, __uint_as_float(x & 0xffff0000u) * bring);
+              };
+              v = make_uint4(to_half(v.x), to_half(v.y), to_half(v.z), to_half(v.w));
+            }
+          }
+          *reinterpret_cast<uint4*>(sh.q[h] + (piece >> 3) * 16384 + tid * 128 + ((piece & 7) ^ (tid & 7)) * 16) = v;
+        }
+      }
+      fence_async_shared();
+      bar_arrive(&sh.q_full);
+
+      uint32_t v_exp = 1;
+      auto block_of = [&](int32_t unit) {
+        const int32_t j = it.begin + unit * kTileKeys + tid;
+        return unit < it.unit1 && j < it.end ? kv_block(k, it.seq, uint32_t(j) / c.block_size) : -1;
+      };
+      int32_t block = block_of(it.unit0);
+      for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
+        KeyInfo& info = sh.info[tile_no % kInfos];
+        ok = ok && bar_wait(&sh.info_empty[tile_no % kInfos], (tile_no / kInfos & 1) ^ 1, failed);
+        const int64_t b = block, at = uint32_t(it.begin + unit * kTileKeys + tid) % c.block_size;
+        info.key_at[tid] = b < 0 ? -1 : (b * c.key.block_stride + at * c.key.token_stride + it.head * c.key.head_stride) * (S::kQuant ? 1 : 2);
+        info.value_at[tid] = b < 0 ? -1 : (b * c.value.block_stride + at * c.value.token_stride + it.head * c.value.head_stride) * (S::kQuant ? 1 : 2);
+        float vs = 0.0f;
+        if constexpr (S::kQuant) {
+          float ks = 0.0f;
+          if (b >= 0) {
+            ks = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride + it.head * c.key.scale_head_stride];
+            vs = reinterpret_cast<const float*>(c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride + it.head * c.value.scale_head_stride];
+          }
+          info.key_scale[tid] = ks;
+          info.value_scale[tid] = vs;
+          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs) & 0x7fffffffu);
+          if (lane == 0) sh.warp_max[tile_no & 1][lw] = top;
+        }
+        const uint32_t seen = __ballot_sync(0xffffffffu, b >= 0);
+        if (lane == 0) info.seen[lw] = seen;
+        // Meeting here also keeps the slots apart: who writes a slot again (kInfos tiles on; warp_max: two) has
+        // met those who read it last.
+        if (!(ok = loaders_agree(ok))) break;
+        if constexpr (S::kQuant) {
+          const uint32_t* w = sh.warp_max[tile_no & 1];
+          const uint32_t top = max(max(w[0], w[1]), max(w[2], w[3]));
+          v_exp = max(v_exp, min(top >> 23, 253u));
+          if (tid == 0) info.v_exp = v_exp;
+        }
+        bar_arrive(&sh.info_full[tile_no % kInfos]);
+        block = block_of(unit + 1);  // on its way while this tile is copied
+        if constexpr (S::kQuant) {
+          load_codes(info.key_at, c.key.data);
+          ok = store_codes();
+          load_codes(info.value_at, c.value.data);
+          ok = ok && store_codes();
+        } else {
+          ok = copy_rows(info.key_at, c.key.data) && copy_rows(info.value_at, c.value.data);
+        }
+      }
+      ++item_no;
+    }
+    if constexpr (!S::kQuant) flush();
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ products
+    if (lane == 0) {
+      constexpr uint32_t kScores = instruction(S::kBf16, kTileKeys, false), kSums = instruction(S::kBf16, DP, true);
+      uint32_t stage_no = 0, item_no = 0, tile_no[2] = {0, 0}, o_no[2] = {0, 0};
+      auto scores = [&](int h, uint32_t stage) {
+        const uint32_t a = smem_u32(sh.q[h]), b = smem_u32(sh.kv[stage % S::kStages]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t off = (i >> 2) * 16384 + (i & 3) * 32;
+          mma_ss(tmem + S::kS + h * 128, operand(a + off, 16), operand(b + off, 16), kScores, i > 0);
+        }
+        mma_commit(&sh.s_full[h]);
+      };
+      auto sums = [&](int h, uint32_t stage, bool add) {
+        const uint32_t b = smem_u32(sh.kv[stage % S::kStages]);
+#pragma unroll
+        for (int i = 0; i < kTileKeys / 16; ++i) {
+          mma_ts(tmem + S::kO + h * 128, tmem + S::kS + h * 128 + i * 8, operand(b + i * 2048, 16384), kSums, add || i > 0);
+        }
+      };
+      bool ok = true;
+      while (ok && walk.next(it)) {
+        const int halves = it.rows > 128 ? 2 : 1;
+        const int32_t n = it.unit1 - it.unit0;
+        ok = bar_wait(&sh.q_full, item_no & 1, failed) &&
+             bar_wait(&sh.kv_full[stage_no % S::kStages], stage_no / S::kStages & 1, failed);
+        if (!ok) break;
+        tmem_after_sync();
+        for (int h = 0; h < halves; ++h) scores(h, stage_no);
+        mma_commit(&sh.kv_empty[stage_no % S::kStages]);
+        if (n == 1) mma_commit(&sh.q_empty);
+        for (int32_t j = 0; j < n && ok; ++j) {
+          const uint32_t v = stage_no + 1, next_key = stage_no + 2;
+          ok = bar_wait(&sh.kv_full[v % S::kStages], v / S::kStages & 1, failed);
+          for (int h = 0; h < halves && ok; ++h) {
+            ok = bar_wait(&sh.p_full[h], tile_no[h] & 1, failed);
+            ++tile_no[h];
+            if (ok && j == 0) ok = bar_wait(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed);
+            if (!ok) break;
+            tmem_after_sync();
+            sums(h, v, j > 0);
+            if (j + 1 < n) {
+              if (h == 0) ok = bar_wait(&sh.kv_full[next_key % S::kStages], next_key / S::kStages & 1, failed);
+              if (!ok) break;
+              scores(h, next_key);
+            } else {
+              mma_commit(&sh.o_full[h]);
+            }
+          }
+          if (!ok) break;
+          mma_commit(&sh.kv_empty[v % S::kStages]);
+          if (j + 1 < n) mma_commit(&sh.kv_empty[next_key % S::kStages]);
+          if (j + 2 == n) mma_commit(&sh.q_empty);
+          stage_no += 2;
+        }
+        ++item_no;
+      }
+      // Whatever was issued is done before the memory that it uses is given back.
+      mma_commit(&sh.done);
+      bar_wait(&sh.done, 0, &sh.stuck);
+    }
+  } else {
+    // ------------------------------------------------------------- softmax
+    const int h = warp >> 2, r = threadIdx.x;  // r: the row of the item
+    const uint32_t lanes = uint32_t(warp & 3) << 21;  // lane 32 * (warp % 4) in the address' upper half
+    const uint32_t s_at = tmem + S::kS + h * 128 + lanes, o_at = tmem + S::kO + h * 128 + lanes;
+    uint32_t tile_no = 0, s_no = 0, o_no = 0, item_no = 0;
+    const float factor = fmaxf(fabsf(k.a.scale) * kLog2e, 1e-30f);  // never 0, which would turn -inf into NaN
+    bool ok = true;
+    while (ok && walk.next(it)) {
+      const bool active = h * 128 < it.rows;
+      const bool mine = r < it.rows;
+      const int32_t row = it.row0 + (mine ? r : 0), i = row / it.group;
+      const int32_t row_lo = mine ? kv_row_begin(k, it.s, i) : 0, row_hi = mine ? kv_row_end(k, it.s, i) : INT32_MAX;
+      float m = -INFINITY, l = 0.0f, f = factor;
+      uint32_t v_exp = 1;
+      for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
+        KeyInfo& info = sh.info[tile_no % kInfos];
+        if (!(ok = bar_wait_warp(&sh.info_full[tile_no % kInfos], tile_no / kInfos & 1, failed))) break;
+        if (!active) {
+          bar_arrive(&sh.info_empty[tile_no % kInfos]);
+          continue;
+        }
+        if (unit == it.unit0) f = fmaxf(factor * sh.q_unit[item_no & 1][r], 1.2e-38f);
+        if (!(ok = bar_wait_warp(&sh.s_full[h], s_no & 1, failed))) break;
+        ++s_no;
+        tmem_after_sync();
+        const int32_t j0 = it.begin + unit * kTileKeys;
+        const bool whole = (info.seen[0] & info.seen[1] & info.seen[2] & info.seen[3]) == 0xffffffffu;
+        const bool masked = !whole || __any_sync(0xffffffffu, row_lo > j0 || row_hi < j0 + kTileKeys);
+        uint32_t s[32] = {};
+        // A score's place in the softmax, masked or not.
+        auto score = [&](int piece, int x) {
+          float y = __uint_as_float(s[x]);
+          if constexpr (S::kQuant) y *= info.key_scale[piece * 32 + x];
+          return y;
+        };
+        auto hide = [&](int piece, int x, float y) {
+          const int32_t j = j0 + piece * 32 + x;
+          return j >= row_lo && j < row_hi && (info.seen[piece] >> x & 1) ? y : -INFINITY;
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int piece = 0; piece < 4; ++piece) {
+          tmem_load32(s, s_at + piece * 32);
+          tmem_wait_load(s);
+          if (masked) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) top = fmaxf(top, hide(piece, x, score(piece, x)));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) top = fmaxf(top, score(piece, x));
+          }
+        }
+        top *= f;
+        float keep = 1.0f;
+        if (top > m + kRaise) {
+          keep = fast_exp2(m - top);  // 0 at first
+          m = top;
+          l *= keep;
+        }
+        float v_inv = 1.0f;
+        if constexpr (S::kQuant) {
+          const uint32_t e = info.v_exp;
+          if (e > v_exp) {
+            keep *= e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
+            v_exp = e;
+          }
+          v_inv = __uint_as_float((254 - v_exp) << 23);
+        }
+        if (unit > it.unit0 && __any_sync(0xffffffffu, keep != 1.0f)) {
+#pragma unroll 1
+          for (int piece = 0; piece < DP / 32; ++piece) {
+            tmem_load32(s, o_at + piece * 32);
+            tmem_wait_load(s);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) s[x] = __float_as_uint(__uint_as_float(s[x]) * keep);
+            tmem_store32(o_at + piece * 32, s);
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int piece = 0; piece < 4; ++piece) {
+          tmem_load32(s, s_at + piece * 32);
+          tmem_wait_load(s);
+          uint32_t p[16];
+          float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            float y[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float z = score(piece, x + u);
+              if (masked) z = hide(piece, x + u, z);
+              y[u] = fast_exp2(fmaf(z, f, -base));
+              sum[u] += y[u];
+              if constexpr (S::kQuant) y[u] *= info.value_scale[piece * 32 + x + u] * v_inv;
+            }
+            p[x / 2] = pack_pair<S::kBf16>(y[0], y[1]);
+          }
+          l += sum[0] + sum[1];
+          tmem_store16(s_at + piece * 16, p);
+        }
+        tmem_wait_store();
+        tmem_before_sync();
+        bar_arrive(&sh.p_full[h]);
+        bar_arrive(&sh.info_empty[tile_no % kInfos]);
+      }
+      ++item_no;
+      if (!ok) break;
+      if (!active) continue;
+      if (!(ok = bar_wait_warp(&sh.o_full[h], o_no & 1, failed))) break;
+      ++o_no;
+      tmem_after_sync();
+      // The result, or this CTA's part of it. An infinity or a NaN in a value that this row does not see may
+      // have met its weight of zero: such rows are made again, token by token.
+      const float v_unit = S::kQuant ? __uint_as_float(v_exp << 23) : 1.0f;
+      const int64_t token = int64_t(it.s.first) + i;
+      const int32_t qh = it.head * it.group + row - i * it.group;
+      T* out = reinterpret_cast<T*>(k.a.out.data) + token * k.a.out.token_stride + int64_t(qh) * k.a.out.head_stride;
+      float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
+                    (int64_t(max(it.slot, 0)) * kTileRows + r) * (DP + 4);
+      const float times = it.slot >= 0 ? v_unit : l == 0.0f ? 0.0f : v_unit / l;
+      bool bad = false;
+#pragma unroll 1
+      for (int piece = 0; piece < DP / 32; ++piece) {
+        uint32_t s[32];
+        tmem_load32(s, o_at + piece * 32);
+        tmem_wait_load(s);
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          bad = bad || !isfinite(__uint_as_float(s[x]));
+          s[x] = __float_as_uint(__uint_as_float(s[x]) * times);
+        }
+        if (mine && it.slot >= 0) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + 4 + piece * 32 + x) = make_uint4(s[x], s[x + 1], s[x + 2], s[x + 3]);
+        } else if (mine) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            if (piece * 32 + x < int(c.head_dim)) {
+              uint4 y;
+              constexpr bool kOutBf16 = Q == PF_DTYPE_BF16;
+              y.x = pack_pair<kOutBf16>(__uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+              y.y = pack_pair<kOutBf16>(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
+              y.z = pack_pair<kOutBf16>(__uint_as_float(s[x + 4]), __uint_as_float(s[x + 5]));
+              y.w = pack_pair<kOutBf16>(__uint_as_float(s[x + 6]), __uint_as_float(s[x + 7]));
+              *reinterpret_cast<uint4*>(out + piece * 32 + x) = y;
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tmem_before_sync();
+      bar_arrive(&sh.o_free[h]);
+      if (mine) {
+        if (it.slot >= 0) {
+          part[0] = m, part[1] = l;
+        } else if (k.a.lse) {
+          reinterpret_cast<float*>(k.a.lse)[token * k.a.q_heads + qh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
+      }
+      uint32_t again = __ballot_sync(0xffffffffu, mine && bad && l == l);
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        const int32_t row_r = it.row0 + (r & ~31) + src, i_r = row_r / it.group, qh_r = it.head * it.group + row_r - i_r * it.group;
+        const int64_t token_r = int64_t(it.s.first) + i_r;
+        float m_r, l_r;
+        float4 v;
+        attend_row_exactly<Q, STORE>(k, it.seq, token_r, uint32_t(qh_r), uint32_t(it.head),
+                                     max(it.begin + it.unit0 * kTileKeys, kv_row_begin(k, it.s, i_r)),
+                                     min(it.begin + it.unit1 * kTileKeys, kv_row_end(k, it.s, i_r)), m_r, l_r, v);
+        if (it.slot >= 0) {
+          float* to = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
+                      (int64_t(it.slot) * kTileRows + (r & ~31) + src) * (DP + 4);
+          if (lane == 0) to[0] = m_r, to[1] = l_r;
+          if (lane * 4 < DP) *reinterpret_cast<float4*>(to + 4 + lane * 4) = v;
+        } else {
+          const float inv = l_r == 0.0f ? 0.0f : 1.0f / l_r;
+          if (lane * 4 < int(c.head_dim)) {
+            KvPack<T, 4> y;
+            y.v[0] = kv_from_float<Q>(v.x * inv), y.v[1] = kv_from_float<Q>(v.y * inv);
+            y.v[2] = kv_from_float<Q>(v.z * inv), y.v[3] = kv_from_float<Q>(v.w * inv);
+            *reinterpret_cast<KvPack<T, 4>*>(reinterpret_cast<T*>(k.a.out.data) + token_r * k.a.out.token_stride +
+                                             int64_t(qh_r) * k.a.out.head_stride + lane * 4) = y;
+          }
+          if (lane == 0 && k.a.lse) {
+            reinterpret_cast<float*>(k.a.lse)[token_r * k.a.q_heads + qh_r] = l_r == 0.0f ? -INFINITY : (m_r + log2f(l_r)) * kLn2;
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    if (sh.failed) kv_flag(reinterpret_cast<int32_t*>(k.a.status), PF_KV_TIMED_OUT);
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the parts of an item that lies in several spans: the block of the CTA in
+// whose span it begins, a warp for a row, weights 2^(m - max).
+template <uint32_t Q, int DP>
+__global__ void __launch_bounds__(256) kv_join_tiles_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan plan) {
+  using T = typename KvElem<Q>::type;
+  wait_for_previous_kernel();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const char* ws = reinterpret_cast<const char*>(k.a.workspace);
+  const int64_t span = span_units(reinterpret_cast<const int64_t*>(ws + plan.costs_at)[k.a.n_seqs], plan.ctas);
+  const int64_t cta = blockIdx.x;
+  const int4 next = *reinterpret_cast<const int4*>(ws + plan.spans_at + (cta + 1) * sizeof(KvSpan));
+  if (next.x >= int32_t(k.a.n_seqs) || next.w == 0) return;
+  const int64_t at = (cta + 1) * span - next.w;  // where the item begins
+  if (at / span != cta) return;
+  const KvSeq s = kv_sequence(k, uint32_t(next.x));
+  const int32_t group = int32_t(k.a.q_heads / k.cache.heads);
+  const int32_t row0 = next.y * kTileRows, rows = min(kTileRows, s.n * group - row0);
+  const KvSplit split =
+      item_split(at, tile_units(kv_row_begin(k, s, row0 / group), kv_row_end(k, s, (row0 + rows - 1) / group)), span);
+  const float* parts = reinterpret_cast<const float*>(ws + plan.parts_at);
+  for (int32_t r = int32_t(blockIdx.y) * 8 + warp; r < rows; r += int32_t(gridDim.y) * 8) {
+    float top = -INFINITY;
+    for (int64_t p = split.first; p <= split.last; ++p) {
+      top = fmaxf(top, parts[(part_slot(at, p, span) * kTileRows + r) * (DP + 4)]);
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+    for (int64_t p = split.first; p <= split.last; ++p) {
+      const float* w = parts + (part_slot(at, p, span) * kTileRows + r) * (DP + 4);
+      const float keep = exp2f(w[0] - base);
+      sum += w[1] * keep;
+      if (lane * 4 < DP) {
+        const float4 v = *reinterpret_cast<const float4*>(w + 4 + lane * 4);
+        o.x += v.x * keep, o.y += v.y * keep, o.z += v.z * keep, o.w += v.w * keep;
+      }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int32_t i = (row0 + r) / group, qh = next.z * group + row0 + r - i * group;
+    const int64_t token = int64_t(s.first) + i;
+    if (lane * 4 < int(k.cache.head_dim)) {
+      KvPack<T, 4> y;
+      y.v[0] = kv_from_float<Q>(o.x * inv), y.v[1] = kv_from_float<Q>(o.y * inv);
+      y.v[2] = kv_from_float<Q>(o.z * inv), y.v[3] = kv_from_float<Q>(o.w * inv);
+      *reinterpret_cast<KvPack<T, 4>*>(reinterpret_cast<T*>(k.a.out.data) + token * k.a.out.token_stride +
+                                       int64_t(qh) * k.a.out.head_stride + lane * 4) = y;
+    }
+    if (lane == 0 && k.a.lse) {
+      reinterpret_cast<float*>(k.a.lse)[token * k.a.q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+  }
+}
+
+template <typename... A>
+cudaError_t launch_early(void (*kernel)(A...), dim3 grid, int threads, size_t shm, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shm;
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <uint32_t Q, uint32_t STORE, int DP>
+cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t stream) {
+  const auto kernel = kv_attend_tiles_kernel<Q, STORE, DP>;
+  const size_t shm = sizeof(typename Tiles<Q, STORE, DP>::Shared) + 1024;
+  static_assert(sizeof(typename Tiles<Q, STORE, DP>::Shared) + 1024 <= 227 * 1024, "tile kernel shared memory");
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shm));
+  if (err != cudaSuccess) return err;
+  kv_tile_spans_kernel<<<1, 1024, 0, stream>>>(k, p);
+  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  if ((err = launch_early(kernel, dim3(p.ctas), kThreads, shm, stream, k, p)) != cudaSuccess) return err;
+  return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 4), 256, 0, stream, k, p);
+}
+
+template <uint32_t Q, uint32_t STORE>
+cudaError_t launch_dims(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t stream) {
+  return k.cache.head_dim <= 64 ? launch_as<Q, STORE, 64>(k, p, stream) : launch_as<Q, STORE, 128>(k, p, stream);
+}
+
+template <uint32_t Q>
+cudaError_t launch_store(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t stream) {
+  switch (k.cache.dtype) {
+    case PF_DTYPE_E4M3: return launch_dims<Q, PF_DTYPE_E4M3>(k, p, stream);
+    case PF_DTYPE_INT8: return launch_dims<Q, PF_DTYPE_INT8>(k, p, stream);
+    default: return launch_dims<Q, Q>(k, p, stream);
+  }
+}
+
+}  // namespace
+
+KvTilePlan tile_plan(const KvAttendArgs& k, int num_sms) {
+  KvTilePlan p{};
+  p.ctas = uint32_t(num_sms);
+  auto take = [&p](uint64_t bytes) {
+    const uint64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.spans_at = take((uint64_t(p.ctas) + 1) * sizeof(KvSpan));
+  p.costs_at = take((uint64_t(k.a.n_seqs) + 1) * sizeof(int64_t));
+  const uint64_t dp = k.cache.head_dim <= 64 ? 64 : 128;
+  p.parts_at = take(2 * uint64_t(p.ctas) * kTileRows * (dp + 4) * sizeof(float));
+  return p;
+}
+
+cudaError_t launch_attend_tiles(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t stream) {
+  return k.a.dtype == PF_DTYPE_BF16 ? launch_store<PF_DTYPE_BF16>(k, p, stream) : launch_store<PF_DTYPE_FP16>(k, p, stream);
+}
+
+}  // namespace pf

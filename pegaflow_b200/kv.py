@@ -13,7 +13,8 @@ synchronised or kept between calls, so they can be captured into CUDA graphs.
 Sizes, types and strides are checked before anything is queued (ValueError, or
 PegaError from the library); what only the device knows (slots, block ids,
 lengths) is skipped where it is out of range, and reported through ``status``,
-an int32 tensor that gets the bits BAD_BLOCK and BAD_LENGTH ORed into it.
+an int32 tensor that gets the bits BAD_BLOCK, BAD_LENGTH and TIMED_OUT (a wait
+within a kernel ran out: the outputs are not valid) ORed into it.
 
 A cache that a transfer loads, or that ``kv_write`` fills, is read by the others
 as soon as their stream is behind it; the same tensors are registered with
@@ -32,6 +33,7 @@ from . import _native as N
 
 BAD_BLOCK = N.PF_KV_BAD_BLOCK
 BAD_LENGTH = N.PF_KV_BAD_LENGTH
+TIMED_OUT = N.PF_KV_TIMED_OUT
 
 _ROWS = {torch.bfloat16: N.PF_DTYPE_BF16, torch.float16: N.PF_DTYPE_FP16, torch.float32: N.PF_DTYPE_FP32}
 _CACHE = {torch.bfloat16: N.PF_DTYPE_BF16, torch.float16: N.PF_DTYPE_FP16, torch.float8_e4m3fn: N.PF_DTYPE_E4M3,

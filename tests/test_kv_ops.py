@@ -221,3 +221,15 @@ def test_empty_calls_need_nothing(native):
     assert N.lib.pf_kv_read(0, byref(c), None, 0, 0, 0, None, byref(r), byref(r), 0, 5, 0, 0) == N.PF_OK
     a = attention(N, c, n_tokens=0)
     assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_OK
+
+
+def test_tile_spans():
+    """The tile kernel's work shared among CTAs, replayed on the host (tests/kv_tiles_test.cpp)."""
+    build = ROOT / "tests" / "_build"
+    build.mkdir(exist_ok=True)
+    exe = build / "kv_tiles_test"
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{ROOT / 'include'}", f"-I{ROOT / 'pegaflow_b200' / 'csrc'}",
+                    "-I/usr/local/cuda/include", str(ROOT / "tests" / "kv_tiles_test.cpp"), "-o", str(exe)], check=True,
+                   capture_output=True, text=True)
+    out = subprocess.run([str(exe), "3000"], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout
