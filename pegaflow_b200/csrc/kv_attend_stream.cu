@@ -361,12 +361,22 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
           for (int e = 0; e < 4; ++e) {
             float y = x[n][e] * f[n][e & 1];
             if constexpr (S::kQuant) y *= e < 2 ? s0.key_scale : s1.key_scale;
-            if (masked) {
-              const int32_t j = j0 + g + (e < 2 ? 0 : 8);
-              if ((e < 2 ? s0.key : s1.key) < 0 || j < row_lo[n][e & 1] || j >= row_hi[n][e & 1]) y = -INFINITY;
-            }
             x[n][e] = y;
           }
+        }
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int32_t j = j0 + g + (e < 2 ? 0 : 8);
+              const bool on = (e < 2 ? s0.key : s1.key) >= 0 && j >= row_lo[n][e & 1] && j < row_hi[n][e & 1];
+              x[n][e] = on ? x[n][e] : -INFINITY;
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
           raise = raise || fmaxf(x[n][0], x[n][2]) > m[n][0] + kRaise || fmaxf(x[n][1], x[n][3]) > m[n][1] + kRaise;
         }
         if (__any_sync(0xffffffffu, raise)) {

@@ -366,6 +366,92 @@ __global__ void __launch_bounds__(1024) kv_tile_spans_kernel(const __grid_consta
   }
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+
+// 32 scores of the thread's row, before the factor that the row has in common:
+// -inf where the row does not see the token (lo <= place < hi, and it is there).
+template <bool QUANT, bool MASKED>
+__device__ __forceinline__ void row_scores(float2 (&y)[16], const KeyInfo& info, uint32_t s_at, int piece, int32_t lo, int32_t hi) {
+  uint32_t s[32];
+  tmem_load32(s, s_at + piece * 32);
+  tmem_wait_load(s);
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    y[x] = make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1]));
+    if constexpr (QUANT) y[x] = mul2(y[x], *reinterpret_cast<const float2*>(&info.key_scale[piece * 32 + 2 * x]));
+  }
+  if constexpr (MASKED) {
+    // Bit x: token 32 * piece + x.
+    const int32_t from = min(max(lo - piece * 32, 0), 32), to = min(max(hi - piece * 32, 0), 32);
+    const uint32_t below_to = to == 32 ? 0xffffffffu : (1u << to) - 1, below_from = from == 32 ? 0xffffffffu : (1u << from) - 1;
+    const uint32_t seen = info.seen[piece] & below_to & ~below_from;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      y[x].x = seen >> (2 * x) & 1 ? y[x].x : -INFINITY;
+      y[x].y = seen >> (2 * x + 1) & 1 ? y[x].y : -INFINITY;
+    }
+  }
+}
+
+template <bool QUANT, bool MASKED>
+__device__ __forceinline__ float row_top(const KeyInfo& info, uint32_t s_at, int32_t lo, int32_t hi) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int piece = 0; piece < 4; ++piece) {
+    float2 y[16];
+    row_scores<QUANT, MASKED>(y, info, s_at, piece, lo, hi);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) top[x & 3] = fmaxf(top[x & 3], fmaxf(y[x].x, y[x].y));
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// The row's weights 2^(score f - base), as 16-bit values over the scores in TMEM
+// (for the second product: times the V scale and v_inv); their sum in fp32.
+template <bool QUANT, bool BF16, bool MASKED>
+__device__ __forceinline__ float row_weights(const KeyInfo& info, uint32_t s_at, int32_t lo, int32_t hi, float f, float base, float v_inv) {
+  float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+  const float2 ff = make_float2(f, f), minus = make_float2(-base, -base), vv = make_float2(v_inv, v_inv);
+#pragma unroll
+  for (int piece = 0; piece < 4; ++piece) {
+    float2 y[16];
+    row_scores<QUANT, MASKED>(y, info, s_at, piece, lo, hi);
+    uint32_t p[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      y[x] = fma2(y[x], ff, minus);
+      y[x].x = fast_exp2(y[x].x);
+      y[x].y = fast_exp2(y[x].y);
+      sum[x & 1] = add2(sum[x & 1], y[x]);
+      if constexpr (QUANT) y[x] = mul2(y[x], mul2(*reinterpret_cast<const float2*>(&info.value_scale[piece * 32 + 2 * x]), vv));
+      p[x] = pack_pair<BF16>(y[x].x, y[x].y);
+    }
+    tmem_store16(s_at + piece * 16, p);
+  }
+  const float2 all = add2(sum[0], sum[1]);
+  return all.x + all.y;
+}
+
 template <uint32_t Q, uint32_t STORE, int DP>
 __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan plan) {
   using S = Tiles<Q, STORE, DP>;
@@ -661,29 +747,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
         const int32_t j0 = it.begin + unit * kTileKeys;
         const bool whole = (info.seen[0] & info.seen[1] & info.seen[2] & info.seen[3]) == 0xffffffffu;
         const bool masked = !whole || __any_sync(0xffffffffu, row_lo > j0 || row_hi < j0 + kTileKeys);
-        uint32_t s[32] = {};
-        // A score's place in the softmax, masked or not.
-        auto score = [&](int piece, int x) {
-          float y = __uint_as_float(s[x]);
-          if constexpr (S::kQuant) y *= info.key_scale[piece * 32 + x];
-          return y;
-        };
-        auto hide = [&](int piece, int x, float y) {
-          const int32_t j = j0 + piece * 32 + x;
-          return j >= row_lo && j < row_hi && (info.seen[piece] >> x & 1) ? y : -INFINITY;
-        };
-        float top = -INFINITY;
-#pragma unroll
-        for (int piece = 0; piece < 4; ++piece) {
-          tmem_load32(s, s_at + piece * 32);
-          tmem_wait_load(s);
-          if (masked) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) top = fmaxf(top, hide(piece, x, score(piece, x)));
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) top = fmaxf(top, score(piece, x));
-          }
+        uint32_t s[32];
+        float top;
+        if (masked) {
+          top = row_top<S::kQuant, true>(info, s_at, row_lo - j0, row_hi - j0);
+        } else {
+          top = row_top<S::kQuant, false>(info, s_at, 0, 0);
         }
         top *= f;
         float keep = 1.0f;
@@ -712,27 +781,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int piece = 0; piece < 4; ++piece) {
-          tmem_load32(s, s_at + piece * 32);
-          tmem_wait_load(s);
-          uint32_t p[16];
-          float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            float y[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float z = score(piece, x + u);
-              if (masked) z = hide(piece, x + u, z);
-              y[u] = fast_exp2(fmaf(z, f, -base));
-              sum[u] += y[u];
-              if constexpr (S::kQuant) y[u] *= info.value_scale[piece * 32 + x + u] * v_inv;
-            }
-            p[x / 2] = pack_pair<S::kBf16>(y[0], y[1]);
-          }
-          l += sum[0] + sum[1];
-          tmem_store16(s_at + piece * 16, p);
+        if (masked) {
+          l += row_weights<S::kQuant, S::kBf16, true>(info, s_at, row_lo - j0, row_hi - j0, f, base, v_inv);
+        } else {
+          l += row_weights<S::kQuant, S::kBf16, false>(info, s_at, 0, 0, f, base, v_inv);
         }
         tmem_wait_store();
         tmem_before_sync();
