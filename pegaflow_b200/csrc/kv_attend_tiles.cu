@@ -34,7 +34,11 @@ constexpr int kSoftmaxWarps = 8;
 constexpr int kLoadWarps = 4;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+// Four warpgroups; the last has one warp at work. Registers are shared out anew
+// once they run (setmaxnreg): 256 x 168 + 128 x 96 + 128 x 72 <= 512 x 128.
+constexpr int kThreads = 512;
+constexpr int kSoftmaxRegs = 168, kLoadRegs = 96, kMmaRegs = 72;
+static_assert(kSoftmaxWarps * kSoftmaxRegs + kLoadWarps * kLoadRegs + 4 * kMmaRegs <= kThreads / 32 * 128, "registers");
 constexpr int kInfos = 4;
 constexpr unsigned long long kWaitNs = 1000000000ull;  // 1 s for each wait
 
@@ -491,15 +495,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
   Item it;
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ------------------------------------------------------------- loading
     const int tid = threadIdx.x - kSoftmaxWarps * 32, lw = warp - kSoftmaxWarps;
     uint32_t tile_no = 0, stage_no = 0, item_no = 0;
-    uint32_t pending = 0;  // filled stages (cp.async) that are not yet handed over
-    auto hand_over = [&](uint32_t stage) {
-      fence_async_shared();
-      bar_arrive(&sh.kv_full[stage % S::kStages]);
-    };
-    // Copies rows of 16-bit values; the stage is handed over when later ones are on their way.
+    // Copies rows of 16-bit values; their arrival counts for the stage's barrier by itself (the products' thread
+    // orders them before its instructions' reads).
     auto copy_rows = [&](const int64_t* at, uint64_t data) {
       constexpr int kPieces = DP / 8;
       if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
@@ -514,18 +515,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
         const char* from = reinterpret_cast<const char*>(data) + (on ? off + piece * 16 : 0);
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sh.kv_full[stage_no % S::kStages])) : "memory");
       ++stage_no;
-      if (++pending == 3) {
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-        hand_over(stage_no - 3);
-        --pending;
-      }
       return true;
-    };
-    auto flush = [&] {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      for (; pending; --pending) hand_over(stage_no - pending);
     };
     // Rows of codes: loaded ahead into registers, written as fp16.
     constexpr int kCodePieces = DP / 16;  // 16-byte loads of a row
@@ -555,16 +547,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
         *reinterpret_cast<uint4*>(row + ((piece & 7) ^ (r & 7)) * 16) = make_uint4(a.x, a.y, b.x, b.y);
         *reinterpret_cast<uint4*>(row + (((piece & 7) + 1) ^ (r & 7)) * 16) = make_uint4(e.x, e.y, d.x, d.y);
       }
-      hand_over(stage_no++);
+      fence_async_shared();
+      bar_arrive(&sh.kv_full[stage_no++ % S::kStages]);
       return true;
     };
 
     // A thread whose wait gave up goes on without copying to the next place where all loading threads meet.
     bool ok = true;
     while (loaders_agree(ok) && walk.next(it)) {
-      // Q: a thread for each row of both tiles. All that is filled is handed over before waiting for the
-      // products that read the last item's.
-      if constexpr (!S::kQuant) flush();
+      // Q: a thread for each row of both tiles.
       ok = loaders_agree(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
       if (!ok) break;
 #pragma unroll 1
@@ -655,10 +646,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       }
       ++item_no;
     }
-    if constexpr (!S::kQuant) flush();
-  } else if (warp == kMmaWarp) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kMmaWarp && lane == 0) {
+      // A stage is there: what copies and stores wrote comes before what the products read.
+      auto filled = [&](uint32_t stage) {
+        const bool ok = bar_wait(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, failed);
+        if constexpr (!S::kQuant) fence_async_shared();
+        return ok;
+      };
       constexpr uint32_t kScores = instruction(S::kBf16, kTileKeys, false), kSums = instruction(S::kBf16, DP, true);
       uint32_t stage_no = 0, item_no = 0, tile_no[2] = {0, 0}, o_no[2] = {0, 0};
       auto scores = [&](int h, uint32_t stage) {
@@ -681,8 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       while (ok && walk.next(it)) {
         const int halves = it.rows > 128 ? 2 : 1;
         const int32_t n = it.unit1 - it.unit0;
-        ok = bar_wait(&sh.q_full, item_no & 1, failed) &&
-             bar_wait(&sh.kv_full[stage_no % S::kStages], stage_no / S::kStages & 1, failed);
+        ok = bar_wait(&sh.q_full, item_no & 1, failed) && filled(stage_no);
         if (!ok) break;
         tmem_after_sync();
         for (int h = 0; h < halves; ++h) scores(h, stage_no);
@@ -690,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
         if (n == 1) mma_commit(&sh.q_empty);
         for (int32_t j = 0; j < n && ok; ++j) {
           const uint32_t v = stage_no + 1, next_key = stage_no + 2;
-          ok = bar_wait(&sh.kv_full[v % S::kStages], v / S::kStages & 1, failed);
+          ok = filled(v);
           for (int h = 0; h < halves && ok; ++h) {
             ok = bar_wait(&sh.p_full[h], tile_no[h] & 1, failed);
             ++tile_no[h];
@@ -699,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
             tmem_after_sync();
             sums(h, v, j > 0);
             if (j + 1 < n) {
-              if (h == 0) ok = bar_wait(&sh.kv_full[next_key % S::kStages], next_key / S::kStages & 1, failed);
+              if (h == 0) ok = filled(next_key);
               if (!ok) break;
               scores(h, next_key);
             } else {
@@ -720,6 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
     }
   } else {
     // ------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int h = warp >> 2, r = threadIdx.x;  // r: the row of the item
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // lane 32 * (warp % 4) in the address' upper half
     const uint32_t s_at = tmem + S::kS + h * 128 + lanes, o_at = tmem + S::kO + h * 128 + lanes;
