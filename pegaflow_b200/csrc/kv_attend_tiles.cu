@@ -12,16 +12,23 @@
 // units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
 // 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
 //
-// Warps 0-3 and 4-7: the softmax of the two tiles. 8-11: load Q, K and V (rows
-// from wherever the block table says, so by 16-byte copies and not by tensor
-// maps; any block size, stride and order). 12: issues the products. mbarriers
-// order them; every wait is bounded, and one that runs out ends the call with a
-// status bit and no hang.
+// Warps 0-3 and 4-7: the softmax of the two tiles. 8-10: load Q, K and V. 11:
+// issues the products. mbarriers order them; every wait is bounded, and one that
+// runs out ends the call with a status bit and no hang.
+//
+// A tile of 128 16-bit keys comes by TMA, a box of each block, where all 128 are
+// seen and the block size allows it (8 to 128 tokens, or whole tiles); else a row
+// at a time by 16-byte copies, with zeros for tokens that are not there: any
+// block size works, and nothing behind a sequence's end is ever multiplied.
 //
 // 8-bit codes become fp16, which holds all of e4m3 and int8 exactly, on the way
-// into shared memory; the scales stay in fp32 and multiply scores and weights. As
-// in the streaming kernel a bf16 query is brought into fp16's range by a power of
-// two for each row, and weights are divided by one that follows the V scales.
+// into shared memory. K's scales stay in fp32 and multiply the scores; V's are
+// multiplied into the values there, which rounds them to fp16 (2^-11, the weights'
+// own rounding) after division by a power of two that follows the largest scale.
+// As in the streaming kernel a bf16 query is brought into fp16's range by a power
+// of two for each row.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "kv_attend.cuh"
@@ -31,16 +38,12 @@ namespace pf {
 namespace {
 
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 4;
+constexpr int kLoadWarps = 3;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
-// Four warpgroups; the last has one warp at work. Registers are shared out anew
-// once they run (setmaxnreg): 256 x 168 + 128 x 96 + 128 x 72 <= 512 x 128.
-constexpr int kThreads = 512;
-constexpr int kSoftmaxRegs = 168, kLoadRegs = 96, kMmaRegs = 72;
-static_assert(kSoftmaxWarps * kSoftmaxRegs + kLoadWarps * kLoadRegs + 4 * kMmaRegs <= kThreads / 32 * 128, "registers");
+constexpr int kThreads = (kMmaWarp + 1) * 32;  // 12 warps: 168 registers each
 constexpr int kInfos = 4;
-constexpr unsigned long long kWaitNs = 1000000000ull;  // 1 s for each wait
+constexpr long long kWaitClocks = 2000000000ll;  // of the SM, for each wait: a second or a little more
 
 // What the softmax needs to know of a tile of keys.
 struct alignas(16) KeyInfo {
@@ -49,8 +52,13 @@ struct alignas(16) KeyInfo {
   int64_t key_at[kTileKeys];  // byte offsets of the rows, -1 for a token that is not seen
   int64_t value_at[kTileKeys];
   uint32_t seen[kTileKeys / 32];
-  uint32_t v_exp;             // exponent field of the power of two that the weights are divided by
+  uint32_t v_exp;             // exponent field of the power of two that V is divided by; it never falls within an item
   uint32_t pad[3];
+};
+
+struct KvBoxMaps {
+  CUtensorMap key;
+  CUtensorMap value;
 };
 
 template <uint32_t Q, uint32_t STORE, int DP>
@@ -64,26 +72,20 @@ struct Tiles {
     unsigned char kv[kStages][kTileBytes];
     KeyInfo info[kInfos];
     float q_unit[2][kTileRows];  // by the item's parity
-    uint32_t warp_max[2][kLoadWarps];  // by the tile's parity
+    uint32_t warp_max[2][kTileKeys / 32];  // by the tile's parity
     uint64_t q_full, q_empty;
     uint64_t kv_full[kStages], kv_empty[kStages];
     uint64_t info_full[kInfos], info_empty[kInfos];
     uint64_t s_full[2], p_full[2], o_full[2], o_free[2], done;
     uint32_t tmem;
     int failed;  // a wait gave up
-    int stuck;   // the last one did
+    int stuck[2];  // those for copies and products in flight did as well
   };
   // TMEM columns.
   static constexpr uint32_t kS = 0, kO = 256;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 
 __device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -100,18 +102,18 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done;
 }
-// Whether the phase of `parity` completed, within kWaitNs and before another
+// Whether the phase of `parity` completed, within kWaitClocks and before another
 // wait of this CTA gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* failed) {
   if (bar_try(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
+  const long long t0 = clock64();
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i) {
       if (bar_try(bar, parity)) return true;
     }
     if (*reinterpret_cast<volatile int*>(failed)) return false;
-    if (now_ns() - t0 > kWaitNs) {
+    if (clock64() - t0 > kWaitClocks) {
       *reinterpret_cast<volatile int*>(failed) = 1;
       return false;
     }
@@ -126,11 +128,22 @@ __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, in
 __device__ __forceinline__ bool loaders_agree(bool ok) {
   uint32_t all;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
       : "=r"(all)
-      : "r"(uint32_t(ok))
+      : "r"(uint32_t(ok)), "n"(kLoadThreads)
       : "memory");
   return all;
+}
+
+__device__ __forceinline__ void bar_arrive_expecting(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// A box of one block's rows for one head: 64 values wide (zeros past head_dim).
+__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, int d, int token, int head, int block, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+      "l"(map), "r"(d), "r"(token), "r"(head), "r"(block), "r"(smem_u32(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -228,6 +241,12 @@ __device__ __forceinline__ uint2 codes_to_half4(uint32_t x) {
   return r;
 }
 
+// Four codes times a scale: the product in fp32, rounded once to fp16.
+__device__ __forceinline__ uint2 times_half4(uint2 x, float by) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
+  return make_uint2(pack_pair<false>(a.x * by, a.y * by), pack_pair<false>(b.x * by, b.y * by));
+}
+
 // One CTA's walk along its span: every role does it for itself.
 struct Item {
   KvSeq s;
@@ -235,8 +254,9 @@ struct Item {
   int32_t head;
   int32_t row0;    // first row of the tile within the sequence's
   int32_t rows;    // rows of the tile
-  int32_t begin;   // tokens that its rows see
+  int32_t first;   // tokens that its rows see
   int32_t end;
+  int32_t begin;   // where its first tile of keys begins
   int32_t units;   // of the whole item
   int32_t unit0;   // this CTA's
   int32_t unit1;
@@ -270,7 +290,8 @@ struct Walk {
     }
     it.seq = uint32_t(seq);
     it.head = head;
-    it.begin = kv_row_begin(k, it.s, it.row0 / it.group);
+    it.first = kv_row_begin(k, it.s, it.row0 / it.group);
+    it.begin = it.first & -kTileKeys;
     it.end = kv_row_end(k, it.s, (it.row0 + it.rows - 1) / it.group);
     it.units = tile_units(it.begin, it.end);
     it.unit0 = unit;
@@ -302,7 +323,7 @@ __global__ void __launch_bounds__(1024) kv_tile_spans_kernel(const __grid_consta
 
   auto units_of = [&](const KvSeq& s, int32_t tile) {
     const int32_t last = min(s.n * group, (tile + 1) * kTileRows) - 1;
-    return tile_units(kv_row_begin(k, s, tile * kTileRows / group), kv_row_end(k, s, last / group));
+    return tile_units(kv_row_begin(k, s, tile * kTileRows / group) & -kTileKeys, kv_row_end(k, s, last / group));
   };
   if (threadIdx.x == 0) front = 0;
   __syncthreads();
@@ -392,72 +413,132 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// 32 scores of the thread's row, before the factor that the row has in common:
-// -inf where the row does not see the token (lo <= place < hi, and it is there).
-template <bool QUANT, bool MASKED>
-__device__ __forceinline__ void row_scores(float2 (&y)[16], const KeyInfo& info, uint32_t s_at, int piece, int32_t lo, int32_t hi) {
-  uint32_t s[32];
-  tmem_load32(s, s_at + piece * 32);
-  tmem_wait_load(s);
+// The larger of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Which of 32 tokens the row sees: lo <= place < hi, and they are there.
+__device__ __forceinline__ uint32_t seen_bits(const KeyInfo& info, int piece, int32_t lo, int32_t hi) {
+  const int32_t from = min(max(lo - piece * 32, 0), 32), to = min(max(hi - piece * 32, 0), 32);
+  const uint32_t below_to = to == 32 ? 0xffffffffu : (1u << to) - 1, below_from = from == 32 ? 0xffffffffu : (1u << from) - 1;
+  return info.seen[piece] & below_to & ~below_from;
+}
+
+// Multiplies a row's fp32 values, or pairs of 16-bit ones, in TMEM: rarely done,
+// so out of the way.
+__device__ __noinline__ void rescale_sums(uint32_t at, int columns, float by) {
+#pragma unroll 1
+  for (int x = 0; x < columns; x += 32) {
+    uint32_t s[32];
+    tmem_load32(s, at + x);
+    tmem_wait_load(s);
 #pragma unroll
-  for (int x = 0; x < 16; ++x) {
-    y[x] = make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1]));
-    if constexpr (QUANT) y[x] = mul2(y[x], *reinterpret_cast<const float2*>(&info.key_scale[piece * 32 + 2 * x]));
+    for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * by);
+    tmem_store32(at + x, s);
   }
-  if constexpr (MASKED) {
-    // Bit x: token 32 * piece + x.
-    const int32_t from = min(max(lo - piece * 32, 0), 32), to = min(max(hi - piece * 32, 0), 32);
-    const uint32_t below_to = to == 32 ? 0xffffffffu : (1u << to) - 1, below_from = from == 32 ? 0xffffffffu : (1u << from) - 1;
-    const uint32_t seen = info.seen[piece] & below_to & ~below_from;
+}
+template <bool BF16>
+__device__ __noinline__ void rescale_weights(uint32_t at, float by) {
+  uint32_t p[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : PF_R4(p, 0), PF_R4(p, 4), PF_R4(p, 8), PF_R4(p, 12)
+               : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : PF_RW4(p, 0), PF_RW4(p, 4), PF_RW4(p, 8), PF_RW4(p, 12) : : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float2 w;
+    if constexpr (BF16) {
+      w = make_float2(__uint_as_float(p[i] << 16), __uint_as_float(p[i] & 0xffff0000u));
+    } else {
+      w = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+    }
+    p[i] = pack_pair<BF16>(w.x * by, w.y * by);
+  }
+  tmem_store16(at, p);
+}
+
+// What a row's softmax carries from tile to tile.
+struct RowState {
+  float m;  // the maximum that the weights go by
+  float l;  // their sum
+};
+
+// One tile's scores of a row into weights 2^(score f - m), 16-bit pairs over the
+// scores in TMEM, 32 scores at a time. m stays as long as no score passes it by
+// kRaise. Where one does (or the row had none yet), m becomes the largest score so
+// far, and the sum, O (o_columns of it) and the weights already made follow.
+template <bool QUANT, bool BF16, bool MASKED>
+__device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, uint32_t s_at, uint32_t o_at, int o_columns,
+                                            int32_t lo, int32_t hi, float f) {
+  float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+  const float2 ff = make_float2(f, f);
+  uint32_t s[32];
+  tmem_load32(s, s_at);
+#pragma unroll 1
+  for (int piece = 0; piece < 4; ++piece) {
+    float2 y[16];
+    float4 ks[QUANT ? 8 : 1];
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) ks[x] = *reinterpret_cast<const float4*>(&info.key_scale[piece * 32 + 4 * x]);
+    }
+    const uint32_t seen = MASKED ? seen_bits(info, piece, lo, hi) : 0;
+    const float base = row.m == -INFINITY ? 0.0f : row.m;
+    const float2 minus = make_float2(-base, -base);
+    float tops[2] = {-INFINITY, -INFINITY};
+    tmem_wait_load(s);
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      y[x].x = seen >> (2 * x) & 1 ? y[x].x : -INFINITY;
-      y[x].y = seen >> (2 * x + 1) & 1 ? y[x].y : -INFINITY;
+      y[x] = make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1]));
+      if constexpr (QUANT) y[x] = mul2(y[x], x % 2 ? make_float2(ks[x / 2].z, ks[x / 2].w) : make_float2(ks[x / 2].x, ks[x / 2].y));
+      if constexpr (MASKED) {
+        y[x].x = seen >> (2 * x) & 1 ? y[x].x : -INFINITY;
+        y[x].y = seen >> (2 * x + 1) & 1 ? y[x].y : -INFINITY;
+      }
+      y[x] = fma2(y[x], ff, minus);
+      tops[x & 1] = max3_nan(tops[x & 1], y[x].x, y[x].y);
     }
-  }
-}
-
-template <bool QUANT, bool MASKED>
-__device__ __forceinline__ float row_top(const KeyInfo& info, uint32_t s_at, int32_t lo, int32_t hi) {
-  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (piece < 3) tmem_load32(s, s_at + (piece + 1) * 32);  // on its way meanwhile
+    const float top = max3_nan(tops[0], tops[1], tops[1]);
+    const bool raise = top > (row.m == -INFINITY ? -INFINITY : kRaise);  // a NaN raises nothing: it reaches the sum
+    if (__any_sync(0xffffffffu, raise)) {
+      float keep = 1.0f;
+      if (raise) {
+        const float m = base + top;
+        keep = fast_exp2(row.m - m);  // 0 at first
+        const float2 shift = make_float2(-top, -top);
 #pragma unroll
-  for (int piece = 0; piece < 4; ++piece) {
-    float2 y[16];
-    row_scores<QUANT, MASKED>(y, info, s_at, piece, lo, hi);
-#pragma unroll
-    for (int x = 0; x < 16; ++x) top[x & 3] = fmaxf(top[x & 3], fmaxf(y[x].x, y[x].y));
-  }
-  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-}
-
-// The row's weights 2^(score f - base), as 16-bit values over the scores in TMEM
-// (for the second product: times the V scale and v_inv); their sum in fp32.
-template <bool QUANT, bool BF16, bool MASKED>
-__device__ __forceinline__ float row_weights(const KeyInfo& info, uint32_t s_at, int32_t lo, int32_t hi, float f, float base, float v_inv) {
-  float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-  const float2 ff = make_float2(f, f), minus = make_float2(-base, -base), vv = make_float2(v_inv, v_inv);
-#pragma unroll
-  for (int piece = 0; piece < 4; ++piece) {
-    float2 y[16];
-    row_scores<QUANT, MASKED>(y, info, s_at, piece, lo, hi);
+        for (int x = 0; x < 16; ++x) y[x] = add2(y[x], shift);
+        row.m = m;
+        row.l *= keep;
+        sum[0] = mul2(sum[0], make_float2(keep, keep));
+        sum[1] = mul2(sum[1], make_float2(keep, keep));
+      }
+      __syncwarp();
+      rescale_sums(o_at, o_columns, keep);
+      for (int before = 0; before < piece; ++before) rescale_weights<BF16>(s_at + before * 16, keep);
+    }
     uint32_t p[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      y[x] = fma2(y[x], ff, minus);
       y[x].x = fast_exp2(y[x].x);
       y[x].y = fast_exp2(y[x].y);
       sum[x & 1] = add2(sum[x & 1], y[x]);
-      if constexpr (QUANT) y[x] = mul2(y[x], mul2(*reinterpret_cast<const float2*>(&info.value_scale[piece * 32 + 2 * x]), vv));
       p[x] = pack_pair<BF16>(y[x].x, y[x].y);
     }
     tmem_store16(s_at + piece * 16, p);
   }
   const float2 all = add2(sum[0], sum[1]);
-  return all.x + all.y;
+  row.l += all.x + all.y;
 }
 
 template <uint32_t Q, uint32_t STORE, int DP>
-__global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan plan) {
+__global__ void __launch_bounds__(kThreads, 1)
+    kv_attend_tiles_kernel(const __grid_constant__ KvAttendArgs k, const __grid_constant__ KvTilePlan plan,
+                           const __grid_constant__ KvBoxMaps maps) {
   using S = Tiles<Q, STORE, DP>;
   using T = typename KvElem<Q>::type;
   extern __shared__ unsigned char raw_smem[];
@@ -477,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       bar_init(&sh.o_full[i], 1), bar_init(&sh.o_free[i], 128);
     }
     bar_init(&sh.done, 1);
-    sh.failed = sh.stuck = 0;
+    sh.failed = sh.stuck[0] = sh.stuck[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -495,25 +576,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
   Item it;
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ------------------------------------------------------------- loading
-    const int tid = threadIdx.x - kSoftmaxWarps * 32, lw = warp - kSoftmaxWarps;
+    const int tid = threadIdx.x - kSoftmaxWarps * 32;
     uint32_t tile_no = 0, stage_no = 0, item_no = 0;
     // Copies rows of 16-bit values; their arrival counts for the stage's barrier by itself (the products' thread
     // orders them before its instructions' reads).
-    auto copy_rows = [&](const int64_t* at, uint64_t data) {
+    auto copy_rows = [&](const int64_t* at, uint64_t data) -> bool {
       constexpr int kPieces = DP / 8;
       if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
-      const uint32_t base = smem_u32(sh.kv[stage_no % S::kStages]);
       const int piece = tid % kPieces;
       const bool there = piece * 8 < int(c.head_dim);
-#pragma unroll 4
-      for (int r = tid / kPieces; r < kTileKeys; r += kLoadThreads / kPieces) {
-        const int64_t off = at[r];
-        const bool on = there && off >= 0;
-        const uint32_t to = base + (piece >> 3) * 16384 + r * 128 + ((piece & 7) ^ (r & 7)) * 16;
-        const char* from = reinterpret_cast<const char*>(data) + (on ? off + piece * 16 : 0);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+      const uint32_t base = smem_u32(sh.kv[stage_no % S::kStages]) + (piece >> 3) * 16384;
+      const char* from = reinterpret_cast<const char*>(data) + piece * 16;
+      // Eight rows' offsets are read, then the eight copies are issued: the reads' latency is met once.
+      constexpr int kRows = kLoadThreads / kPieces, kAhead = 8;
+#pragma unroll 1
+      for (int r0 = tid / kPieces; r0 < kTileKeys; r0 += kRows * kAhead) {
+        int64_t off[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) off[i] = r0 + i * kRows < kTileKeys ? at[r0 + i * kRows] : -1;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int r = r0 + i * kRows;
+          const bool on = there && off[i] >= 0;
+          if (r < kTileKeys) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + r * 128 + ((piece & 7) ^ (r & 7)) * 16),
+                         "l"(on ? from + off[i] : reinterpret_cast<const char*>(data)), "r"(on ? 16 : 0)
+                         : "memory");
+          }
+        }
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sh.kv_full[stage_no % S::kStages])) : "memory");
       ++stage_no;
@@ -522,30 +613,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
     // Rows of codes: loaded ahead into registers, written as fp16.
     constexpr int kCodePieces = DP / 16;  // 16-byte loads of a row
     constexpr int kCodeRows = kLoadThreads / kCodePieces;
-    constexpr int kCodeLoads = kTileKeys / kCodeRows;
-    uint4 codes[S::kQuant ? kCodeLoads : 1];
-    auto load_codes = [&](const int64_t* at, uint64_t data) {
+    constexpr int kCodeLoads = (kTileKeys + kCodeRows - 1) / kCodeRows;
+    using Codes = uint4[S::kQuant ? kCodeLoads : 1];
+    auto load_codes = [&](Codes& codes, const int64_t* at, uint64_t data) {
       const int piece = tid % kCodePieces;
       const bool there = piece * 16 < int(c.head_dim);
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
-        const int64_t off = at[tid / kCodePieces + i * kCodeRows];
-        codes[i] = there && off >= 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(data) + off + piece * 16)
-                                     : make_uint4(0, 0, 0, 0);
+        const int r = tid / kCodePieces + i * kCodeRows;
+        const int64_t off = r < kTileKeys ? at[r] : -1;
+        codes[i] = make_uint4(0, 0, 0, 0);
+        if (there && off >= 0) codes[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(data) + off + piece * 16);
       }
     };
-    auto store_codes = [&]() -> bool {
+    auto store_codes = [&](const Codes& codes, const float* scales, float inv) -> bool {
       if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
-      unsigned char* base = sh.kv[stage_no % S::kStages];
       const int piece = tid % kCodePieces * 2;  // of 16 bytes of fp16
+      unsigned char* base = sh.kv[stage_no % S::kStages] + (piece >> 3) * 16384;
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
         const int r = tid / kCodePieces + i * kCodeRows;
-        const uint2 a = codes_to_half4<STORE>(codes[i].x), b = codes_to_half4<STORE>(codes[i].y);
-        const uint2 e = codes_to_half4<STORE>(codes[i].z), d = codes_to_half4<STORE>(codes[i].w);
-        unsigned char* row = base + (piece >> 3) * 16384 + r * 128;
-        *reinterpret_cast<uint4*>(row + ((piece & 7) ^ (r & 7)) * 16) = make_uint4(a.x, a.y, b.x, b.y);
-        *reinterpret_cast<uint4*>(row + (((piece & 7) + 1) ^ (r & 7)) * 16) = make_uint4(e.x, e.y, d.x, d.y);
+        if (r >= kTileKeys) break;
+        uint2 x = codes_to_half4<STORE>(codes[i].x), y = codes_to_half4<STORE>(codes[i].y);
+        uint2 z = codes_to_half4<STORE>(codes[i].z), w = codes_to_half4<STORE>(codes[i].w);
+        if (scales) {
+          const float by = scales[r] * inv;  // below 2
+          x = times_half4(x, by), y = times_half4(y, by), z = times_half4(z, by), w = times_half4(w, by);
+        }
+        *reinterpret_cast<uint4*>(base + r * 128 + ((piece & 7) ^ (r & 7)) * 16) = make_uint4(x.x, x.y, y.x, y.y);
+        *reinterpret_cast<uint4*>(base + r * 128 + (((piece & 7) + 1) ^ (r & 7)) * 16) = make_uint4(z.x, z.y, w.x, w.y);
       }
       fence_async_shared();
       bar_arrive(&sh.kv_full[stage_no++ % S::kStages]);
@@ -555,102 +651,187 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
     // A thread whose wait gave up goes on without copying to the next place where all loading threads meet.
     bool ok = true;
     while (loaders_agree(ok) && walk.next(it)) {
-      // Q: a thread for each row of both tiles.
+      auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
+      // Each thread's tokens of a tile: tid and, for the first warp, tid + 96.
+      auto token_of = [&](int32_t unit, int u) { return it.begin + unit * kTileKeys + tid + u * kLoadThreads; };
+      int32_t block[2];
+      auto look_up = [&](int32_t unit) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int32_t j = token_of(unit, u);
+          const bool on = unit < it.unit1 && tid + u * kLoadThreads < kTileKeys && j >= it.first && j < it.end;
+          block[u] = on ? kv_block(k, it.seq, page_of(j)) : -1;
+        }
+      };
+      look_up(it.unit0);
+
+      // Q: a thread for a row at a time, of both tiles.
       ok = loaders_agree(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
       if (!ok) break;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        const int r = h * 128 + tid;
+      for (int r = tid; r < kTileRows; r += kLoadThreads) {
+        if (r >= 128 && it.rows <= 128) break;
         const bool on = r < it.rows;
-        if (h * 128 >= it.rows) break;
         const int32_t row = it.row0 + (on ? r : 0), i = row / it.group;
         const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(it.s.first + i) * k.a.query.token_stride +
                      int64_t(it.head * it.group + row - i * it.group) * k.a.query.head_stride;
+        uint4 v[DP / 8];
+#pragma unroll
+        for (int piece = 0; piece < DP / 8; ++piece) {
+          v[piece] = make_uint4(0, 0, 0, 0);
+          if (on && piece * 8 < int(c.head_dim)) v[piece] = *reinterpret_cast<const uint4*>(p + piece * 8);
+        }
         const uint32_t flip = k.a.scale < 0.0f ? 0x80008000u : 0u;
         float bring = 1.0f, unit = 1.0f;
         if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
           uint32_t top = 0;
-          for (int d = 0; d < int(c.head_dim); d += 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p + d);
-            for (uint32_t x : {v.x, v.y, v.z, v.w}) top = max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu));
+#pragma unroll
+          for (int piece = 0; piece < DP / 8; ++piece) {
+            for (uint32_t x : {v[piece].x, v[piece].y, v[piece].z, v[piece].w}) top = max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu));
           }
           const int e = min(max(int(top >> 7) - 127, -100), 127);
           bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
           unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
         }
         sh.q_unit[item_no & 1][r] = unit;
-#pragma unroll 4
-        for (int piece = 0; piece < DP / 8; ++piece) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (on && piece * 8 < int(c.head_dim)) {
-            v = *reinterpret_cast<const uint4*>(p + piece * 8);
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-            if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
-              auto to_half = [&](uint32_t x) {
-                return pack_pair<false>(__uint_as_float(x << 16) * bring, __uint_as_float(x & 0xffff0000u) * bring);
-              };
-              v = make_uint4(to_half(v.x), to_half(v.y), to_half(v.z), to_half(v.w));
-            }
+        auto convert = [&](uint32_t x) {
+          x ^= flip;
+          if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+            x = pack_pair<false>(__uint_as_float(x << 16) * bring, __uint_as_float(x & 0xffff0000u) * bring);
           }
-          *reinterpret_cast<uint4*>(sh.q[h] + (piece >> 3) * 16384 + tid * 128 + ((piece & 7) ^ (tid & 7)) * 16) = v;
+          return x;
+        };
+        unsigned char* to = sh.q[r >> 7] + (r & 127) * 128;
+#pragma unroll
+        for (int piece = 0; piece < DP / 8; ++piece) {
+          *reinterpret_cast<uint4*>(to + (piece >> 3) * 16384 + ((piece & 7) ^ (r & 7)) * 16) =
+              make_uint4(convert(v[piece].x), convert(v[piece].y), convert(v[piece].z), convert(v[piece].w));
         }
       }
       fence_async_shared();
       bar_arrive(&sh.q_full);
 
+      // What the softmax needs of a tile, and where its rows are.
       uint32_t v_exp = 1;
-      auto block_of = [&](int32_t unit) {
-        const int32_t j = it.begin + unit * kTileKeys + tid;
-        return unit < it.unit1 && j < it.end ? kv_block(k, it.seq, uint32_t(j) / c.block_size) : -1;
+      float v_inv = 0.0f;
+      auto offsets = [&](int32_t unit, KeyInfo& info) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int x = tid + u * kLoadThreads;
+          if (x >= kTileKeys) break;  // whole warps
+          const int32_t j = token_of(unit, u);
+          const int64_t b = block[u], at = uint32_t(j) - page_of(j) * c.block_size;
+          constexpr int kElt = S::kQuant ? 1 : 2;
+          info.key_at[x] = b < 0 ? -1 : (b * c.key.block_stride + at * c.key.token_stride + it.head * c.key.head_stride) * kElt;
+          info.value_at[x] = b < 0 ? -1 : (b * c.value.block_stride + at * c.value.token_stride + it.head * c.value.head_stride) * kElt;
+          if constexpr (S::kQuant) {
+            float ks = 0.0f, vs = 0.0f;
+            if (b >= 0) {
+              ks = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride + it.head * c.key.scale_head_stride];
+              vs = reinterpret_cast<const float*>(c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride + it.head * c.value.scale_head_stride];
+            }
+            info.key_scale[x] = ks;
+            info.value_scale[x] = vs;
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs) & 0x7fffffffu);
+            if (lane == 0) sh.warp_max[tile_no & 1][x >> 5] = top;
+          }
+        }
       };
-      int32_t block = block_of(it.unit0);
-      for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
+      auto prepare = [&](int32_t unit) -> bool {
         KeyInfo& info = sh.info[tile_no % kInfos];
         ok = ok && bar_wait(&sh.info_empty[tile_no % kInfos], (tile_no / kInfos & 1) ^ 1, failed);
-        const int64_t b = block, at = uint32_t(it.begin + unit * kTileKeys + tid) % c.block_size;
-        info.key_at[tid] = b < 0 ? -1 : (b * c.key.block_stride + at * c.key.token_stride + it.head * c.key.head_stride) * (S::kQuant ? 1 : 2);
-        info.value_at[tid] = b < 0 ? -1 : (b * c.value.block_stride + at * c.value.token_stride + it.head * c.value.head_stride) * (S::kQuant ? 1 : 2);
-        float vs = 0.0f;
-        if constexpr (S::kQuant) {
-          float ks = 0.0f;
-          if (b >= 0) {
-            ks = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride + it.head * c.key.scale_head_stride];
-            vs = reinterpret_cast<const float*>(c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride + it.head * c.value.scale_head_stride];
-          }
-          info.key_scale[tid] = ks;
-          info.value_scale[tid] = vs;
-          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs) & 0x7fffffffu);
-          if (lane == 0) sh.warp_max[tile_no & 1][lw] = top;
+        const uint32_t seen = __ballot_sync(0xffffffffu, block[0] >= 0);
+        if (lane == 0) info.seen[tid >> 5] = seen;
+        if (tid < kTileKeys - kLoadThreads) {
+          const uint32_t last = __ballot_sync(0xffffffffu, block[1] >= 0);
+          if (lane == 0) info.seen[kLoadThreads / 32] = last;
         }
-        const uint32_t seen = __ballot_sync(0xffffffffu, b >= 0);
-        if (lane == 0) info.seen[lw] = seen;
+        if constexpr (S::kQuant) offsets(unit, info);
         // Meeting here also keeps the slots apart: who writes a slot again (kInfos tiles on; warp_max: two) has
         // met those who read it last.
-        if (!(ok = loaders_agree(ok))) break;
+        ok = loaders_agree(ok);
+        if (!ok) return false;
         if constexpr (S::kQuant) {
           const uint32_t* w = sh.warp_max[tile_no & 1];
-          const uint32_t top = max(max(w[0], w[1]), max(w[2], w[3]));
-          v_exp = max(v_exp, min(top >> 23, 253u));
+          v_exp = max(v_exp, min(max(max(w[0], w[1]), max(w[2], w[3])) >> 23, 253u));
+          v_inv = __uint_as_float((254 - v_exp) << 23);
           if (tid == 0) info.v_exp = v_exp;
         }
         bar_arrive(&sh.info_full[tile_no % kInfos]);
-        block = block_of(unit + 1);  // on its way while this tile is copied
-        if constexpr (S::kQuant) {
-          load_codes(info.key_at, c.key.data);
-          ok = store_codes();
-          load_codes(info.value_at, c.value.data);
-          ok = ok && store_codes();
+        return true;
+      };
+      // A whole tile of one side by TMA: the thread that has a box's first token issues it.
+      auto load_boxes = [&](int32_t unit, const CUtensorMap& map) -> bool {
+        const uint32_t stage = stage_no++ % S::kStages;
+        if (!bar_wait(&sh.kv_empty[stage], ((stage_no - 1) / S::kStages & 1) ^ 1, failed)) return false;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int x = tid + u * kLoadThreads;
+          if (x < kTileKeys && x % plan.box_rows == 0) mine += plan.box_rows * DP * 2;
+        }
+        if (mine) {
+          bar_arrive_expecting(&sh.kv_full[stage], mine);
         } else {
-          ok = copy_rows(info.key_at, c.key.data) && copy_rows(info.value_at, c.value.data);
+          bar_arrive(&sh.kv_full[stage]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int x = tid + u * kLoadThreads;
+          if (x < kTileKeys && x % plan.box_rows == 0) {
+            const int32_t j = token_of(unit, u);
+#pragma unroll
+            for (int d = 0; d < DP; d += 64) {
+              load_box(smem_u32(sh.kv[stage]) + d / 64 * 16384 + x * 128, &map, d, int(uint32_t(j) - page_of(j) * c.block_size), it.head, block[u], &sh.kv_full[stage]);
+            }
+          }
+        }
+        return true;
+      };
+      if constexpr (S::kQuant) {
+        // A tile's V is on its way while its K is converted, the next tile's K while this one's V is.
+        Codes key, value;
+        if (!prepare(it.unit0)) break;
+        load_codes(key, sh.info[tile_no % kInfos].key_at, c.key.data);
+        for (int32_t unit = it.unit0; unit < it.unit1; ++unit) {
+          const KeyInfo& info = sh.info[tile_no % kInfos];
+          const float inv = v_inv;
+          look_up(unit + 1);
+          load_codes(value, info.value_at, c.value.data);
+          ok = ok && store_codes(key, nullptr, 0.0f);
+          ++tile_no;
+          if (unit + 1 < it.unit1) {
+            if (!prepare(unit + 1)) break;
+            load_codes(key, sh.info[tile_no % kInfos].key_at, c.key.data);
+          }
+          ok = ok && store_codes(value, info.value_scale, inv);
+        }
+      } else {
+        for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
+          if (!prepare(unit)) break;
+          KeyInfo& info = sh.info[tile_no % kInfos];
+          const bool whole = (info.seen[0] & info.seen[1] & info.seen[2] & info.seen[3]) == 0xffffffffu;
+          if (whole && plan.box_rows) {
+            ok = load_boxes(unit, maps.key) && load_boxes(unit, maps.value);
+          } else {
+            offsets(unit, info);
+            if (!loaders_agree(true)) break;  // the offsets are written
+            ok = copy_rows(info.key_at, c.key.data) && copy_rows(info.value_at, c.value.data);
+          }
+          look_up(unit + 1);
         }
       }
       ++item_no;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp >= kMmaWarp) {
+    if (*reinterpret_cast<volatile int*>(failed)) {  // boxes that nobody waits for any more
+      for (uint32_t n = stage_no > S::kStages ? stage_no - S::kStages : 0; n < stage_no; ++n) {
+        bar_wait(&sh.kv_full[n % S::kStages], n / S::kStages & 1, &sh.stuck[1]);
+      }
+    }
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == kMmaWarp && lane == 0) {
+    if (lane == 0) {
       // A stage is there: what copies and stores wrote comes before what the products read.
       auto filled = [&](uint32_t stage) {
         const bool ok = bar_wait(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, failed);
@@ -713,11 +894,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       }
       // Whatever was issued is done before the memory that it uses is given back.
       mma_commit(&sh.done);
-      bar_wait(&sh.done, 0, &sh.stuck);
+      bar_wait(&sh.done, 0, &sh.stuck[0]);
     }
   } else {
     // ------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int h = warp >> 2, r = threadIdx.x;  // r: the row of the item
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // lane 32 * (warp % 4) in the address' upper half
     const uint32_t s_at = tmem + S::kS + h * 128 + lanes, o_at = tmem + S::kO + h * 128 + lanes;
@@ -729,7 +909,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       const bool mine = r < it.rows;
       const int32_t row = it.row0 + (mine ? r : 0), i = row / it.group;
       const int32_t row_lo = mine ? kv_row_begin(k, it.s, i) : 0, row_hi = mine ? kv_row_end(k, it.s, i) : INT32_MAX;
-      float m = -INFINITY, l = 0.0f, f = factor;
+      RowState sm{-INFINITY, 0.0f};
+      float f = factor;
       uint32_t v_exp = 1;
       for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
         KeyInfo& info = sh.info[tile_no % kInfos];
@@ -745,44 +926,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
         const int32_t j0 = it.begin + unit * kTileKeys;
         const bool whole = (info.seen[0] & info.seen[1] & info.seen[2] & info.seen[3]) == 0xffffffffu;
         const bool masked = !whole || __any_sync(0xffffffffu, row_lo > j0 || row_hi < j0 + kTileKeys);
-        uint32_t s[32];
-        float top;
-        if (masked) {
-          top = row_top<S::kQuant, true>(info, s_at, row_lo - j0, row_hi - j0);
-        } else {
-          top = row_top<S::kQuant, false>(info, s_at, 0, 0);
-        }
-        top *= f;
-        float keep = 1.0f;
-        if (top > m + kRaise) {
-          keep = fast_exp2(m - top);  // 0 at first
-          m = top;
-          l *= keep;
-        }
-        float v_inv = 1.0f;
+        const int o_columns = unit > it.unit0 ? DP : 0;  // O holds nothing yet in front of an item's first tile
         if constexpr (S::kQuant) {
           const uint32_t e = info.v_exp;
           if (e > v_exp) {
-            keep *= e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
+            rescale_sums(o_at, o_columns, e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23));
             v_exp = e;
           }
-          v_inv = __uint_as_float((254 - v_exp) << 23);
         }
-        if (unit > it.unit0 && __any_sync(0xffffffffu, keep != 1.0f)) {
-#pragma unroll 1
-          for (int piece = 0; piece < DP / 32; ++piece) {
-            tmem_load32(s, o_at + piece * 32);
-            tmem_wait_load(s);
-#pragma unroll
-            for (int x = 0; x < 32; ++x) s[x] = __float_as_uint(__uint_as_float(s[x]) * keep);
-            tmem_store32(o_at + piece * 32, s);
-          }
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
         if (masked) {
-          l += row_weights<S::kQuant, S::kBf16, true>(info, s_at, row_lo - j0, row_hi - j0, f, base, v_inv);
+          row_weights<S::kQuant, S::kBf16, true>(sm, info, s_at, o_at, o_columns, row_lo - j0, row_hi - j0, f);
         } else {
-          l += row_weights<S::kQuant, S::kBf16, false>(info, s_at, 0, 0, f, base, v_inv);
+          row_weights<S::kQuant, S::kBf16, false>(sm, info, s_at, o_at, o_columns, 0, 0, f);
         }
         tmem_wait_store();
         tmem_before_sync();
@@ -795,6 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_tiles_kernel(const __gr
       if (!(ok = bar_wait_warp(&sh.o_full[h], o_no & 1, failed))) break;
       ++o_no;
       tmem_after_sync();
+      const float m = sm.m, l = sm.l;
       // The result, or this CTA's part of it. An infinity or a NaN in a value that this row does not see may
       // have met its weight of zero: such rows are made again, token by token.
       const float v_unit = S::kQuant ? __uint_as_float(v_exp << 23) : 1.0f;
@@ -900,7 +1056,7 @@ __global__ void __launch_bounds__(256) kv_join_tiles_kernel(const __grid_constan
   const int32_t group = int32_t(k.a.q_heads / k.cache.heads);
   const int32_t row0 = next.y * kTileRows, rows = min(kTileRows, s.n * group - row0);
   const KvSplit split =
-      item_split(at, tile_units(kv_row_begin(k, s, row0 / group), kv_row_end(k, s, (row0 + rows - 1) / group)), span);
+      item_split(at, tile_units(kv_row_begin(k, s, row0 / group) & -kTileKeys, kv_row_end(k, s, (row0 + rows - 1) / group)), span);
   const float* parts = reinterpret_cast<const float*>(ws + plan.parts_at);
   for (int32_t r = int32_t(blockIdx.y) * 8 + warp; r < rows; r += int32_t(gridDim.y) * 8) {
     float top = -INFINITY;
@@ -951,6 +1107,38 @@ cudaError_t launch_early(void (*kernel)(A...), dim3 grid, int threads, size_t sh
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// The rows of a block as TMA sees them: [blocks][heads][tokens][values], boxes of
+// up to 128 tokens x 64 values in the operands' swizzle. False: copied instead.
+bool box_map(const pf_kv_cache& c, const pf_kv_side& s, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (!encode) return false;
+  const uint32_t rows = std::min<uint32_t>(c.block_size, kTileKeys);
+  const cuuint64_t dims[4] = {c.head_dim, c.block_size, c.heads, c.num_blocks};
+  // An axis of one element may have any stride; the map wants a real one.
+  auto stride = [](int64_t elements, uint64_t n) { return n > 1 ? cuuint64_t(elements) * 2 : cuuint64_t(16); };
+  const cuuint64_t strides[3] = {stride(s.token_stride, c.block_size), stride(s.head_stride, c.heads),
+                                 stride(s.block_stride, c.num_blocks)};
+  for (cuuint64_t x : strides) {
+    if (x == 0 || x >= (1ull << 40)) return false;
+  }
+  const cuuint32_t box[4] = {64, rows, 1, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, c.dtype == PF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                reinterpret_cast<void*>(s.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <uint32_t Q, uint32_t STORE, int DP>
 cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t stream) {
   const auto kernel = kv_attend_tiles_kernel<Q, STORE, DP>;
@@ -958,9 +1146,14 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t s
   static_assert(sizeof(typename Tiles<Q, STORE, DP>::Shared) + 1024 <= 227 * 1024, "tile kernel shared memory");
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shm));
   if (err != cudaSuccess) return err;
+  KvBoxMaps maps{};
+  KvTilePlan plan = p;
+  if (Tiles<Q, STORE, DP>::kQuant || !box_map(k.cache, k.cache.key, &maps.key) || !box_map(k.cache, k.cache.value, &maps.value)) {
+    plan.box_rows = 0;
+  }
   kv_tile_spans_kernel<<<1, 1024, 0, stream>>>(k, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  if ((err = launch_early(kernel, dim3(p.ctas), kThreads, shm, stream, k, p)) != cudaSuccess) return err;
+  if ((err = launch_early(kernel, dim3(p.ctas), kThreads, shm, stream, k, plan, maps)) != cudaSuccess) return err;
   return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 4), 256, 0, stream, k, p);
 }
 
@@ -983,6 +1176,13 @@ cudaError_t launch_store(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_
 KvTilePlan tile_plan(const KvAttendArgs& k, int num_sms) {
   KvTilePlan p{};
   p.ctas = uint32_t(num_sms);
+  const uint32_t page = k.cache.block_size;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i) {
+    if (page == 1u << i) p.page_shift = i;
+  }
+  // Boxes of whole swizzle groups (8 rows) that tile 128 rows.
+  p.box_rows = page % kTileKeys == 0 ? kTileKeys : page >= 8 && kTileKeys % page == 0 ? page : 0;
   auto take = [&p](uint64_t bytes) {
     const uint64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;

@@ -21,6 +21,8 @@ constexpr int kTileKeys = 128;  // tokens of a unit
 
 struct KvTilePlan {
   uint32_t ctas;
+  int32_t page_shift;    // log2 of the block size, -1 if it is no power of two
+  uint32_t box_rows;     // tokens of a TMA box, 0: none
   uint32_t reserved;
   uint64_t spans_at;     // byte offsets in the workspace: KvSpan[ctas + 1]
   uint64_t costs_at;     // int64[n_seqs + 1], units in front of each sequence
