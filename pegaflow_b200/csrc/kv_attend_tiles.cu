@@ -53,7 +53,8 @@ struct alignas(16) KeyInfo {
   int64_t value_at[kTileKeys];
   uint32_t seen[kTileKeys / 32];
   uint32_t v_exp;             // exponent field of the power of two that V is divided by; it never falls within an item
-  uint32_t pad[3];
+  uint32_t boxed;             // came by TMA
+  uint32_t pad[2];
 };
 
 struct KvBoxMaps {
@@ -150,6 +151,15 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// One thread of a converged warp, always the same. Products are issued under it:
+// their operands live in uniform registers, and only here does the compiler know
+// that one thread's values are the warp's (issued by `lane == 0` each of them
+// took 100 clocks).
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes;
+}
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -811,7 +821,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!prepare(unit)) break;
           KeyInfo& info = sh.info[tile_no % kInfos];
           const bool whole = (info.seen[0] & info.seen[1] & info.seen[2] & info.seen[3]) == 0xffffffffu;
-          if (whole && plan.box_rows) {
+          const bool boxed = whole && plan.box_rows;
+          info.boxed = boxed;  // all threads write the same
+          if (boxed) {
             ok = load_boxes(unit, maps.key) && load_boxes(unit, maps.value);
           } else {
             offsets(unit, info);
@@ -831,71 +843,85 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
-      // A stage is there: what copies and stores wrote comes before what the products read.
-      auto filled = [&](uint32_t stage) {
-        const bool ok = bar_wait(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, failed);
-        if constexpr (!S::kQuant) fence_async_shared();
-        return ok;
-      };
-      constexpr uint32_t kScores = instruction(S::kBf16, kTileKeys, false), kSums = instruction(S::kBf16, DP, true);
-      uint32_t stage_no = 0, item_no = 0, tile_no[2] = {0, 0}, o_no[2] = {0, 0};
-      auto scores = [&](int h, uint32_t stage) {
-        const uint32_t a = smem_u32(sh.q[h]), b = smem_u32(sh.kv[stage % S::kStages]);
+    constexpr uint32_t kScores = instruction(S::kBf16, kTileKeys, false), kSums = instruction(S::kBf16, DP, true);
+    uint32_t stage_no = 0, info_no = 0, item_no = 0, tile_no[2] = {0, 0}, o_no[2] = {0, 0};
+    const uint32_t q_at = smem_u32(sh.q), kv_at = smem_u32(sh.kv);
+    // A stage is there. What copies wrote (no box, no store with a fence of its own) is ordered before what the
+    // products read.
+    auto filled = [&](uint32_t stage, uint32_t info) {
+      const bool ok = bar_wait_warp(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, failed);
+      if constexpr (!S::kQuant) {
+        if (!sh.info[info % kInfos].boxed) fence_async_shared();
+      }
+      return ok;
+    };
+    auto scores = [&](int h, uint32_t stage) {
+      const uint64_t a = operand(q_at + h * S::kTileBytes, 16), b = operand(kv_at + stage % S::kStages * S::kTileBytes, 16);
+      if (elected()) {
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t off = (i >> 2) * 16384 + (i & 3) * 32;
-          mma_ss(tmem + S::kS + h * 128, operand(a + off, 16), operand(b + off, 16), kScores, i > 0);
+          constexpr uint32_t kBlock = 16384 >> 4, kStep = 32 >> 4;
+          const uint32_t off = (i >> 2) * kBlock + (i & 3) * kStep;
+          mma_ss(tmem + S::kS + h * 128, a + off, b + off, kScores, i > 0);
         }
         mma_commit(&sh.s_full[h]);
-      };
-      auto sums = [&](int h, uint32_t stage, bool add) {
-        const uint32_t b = smem_u32(sh.kv[stage % S::kStages]);
+      }
+      __syncwarp();
+    };
+    auto sums = [&](int h, uint32_t stage, bool add) {
+      const uint64_t b = operand(kv_at + stage % S::kStages * S::kTileBytes, 16384);
+      if (elected()) {
 #pragma unroll
         for (int i = 0; i < kTileKeys / 16; ++i) {
-          mma_ts(tmem + S::kO + h * 128, tmem + S::kS + h * 128 + i * 8, operand(b + i * 2048, 16384), kSums, add || i > 0);
+          mma_ts(tmem + S::kO + h * 128, tmem + S::kS + h * 128 + i * 8, b + i * (2048 >> 4), kSums, add || i > 0);
         }
-      };
-      bool ok = true;
-      while (ok && walk.next(it)) {
-        const int halves = it.rows > 128 ? 2 : 1;
-        const int32_t n = it.unit1 - it.unit0;
-        ok = bar_wait(&sh.q_full, item_no & 1, failed) && filled(stage_no);
-        if (!ok) break;
-        tmem_after_sync();
-        for (int h = 0; h < halves; ++h) scores(h, stage_no);
-        mma_commit(&sh.kv_empty[stage_no % S::kStages]);
-        if (n == 1) mma_commit(&sh.q_empty);
-        for (int32_t j = 0; j < n && ok; ++j) {
-          const uint32_t v = stage_no + 1, next_key = stage_no + 2;
-          ok = filled(v);
-          for (int h = 0; h < halves && ok; ++h) {
-            ok = bar_wait(&sh.p_full[h], tile_no[h] & 1, failed);
-            ++tile_no[h];
-            if (ok && j == 0) ok = bar_wait(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed);
-            if (!ok) break;
-            tmem_after_sync();
-            sums(h, v, j > 0);
-            if (j + 1 < n) {
-              if (h == 0) ok = filled(next_key);
-              if (!ok) break;
-              scores(h, next_key);
-            } else {
-              mma_commit(&sh.o_full[h]);
-            }
-          }
-          if (!ok) break;
-          mma_commit(&sh.kv_empty[v % S::kStages]);
-          if (j + 1 < n) mma_commit(&sh.kv_empty[next_key % S::kStages]);
-          if (j + 2 == n) mma_commit(&sh.q_empty);
-          stage_no += 2;
-        }
-        ++item_no;
       }
-      // Whatever was issued is done before the memory that it uses is given back.
-      mma_commit(&sh.done);
-      bar_wait(&sh.done, 0, &sh.stuck[0]);
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elected()) mma_commit(bar);
+      __syncwarp();
+    };
+    bool ok = true;
+    while (ok && walk.next(it)) {
+      const int halves = it.rows > 128 ? 2 : 1;
+      const int32_t n = it.unit1 - it.unit0;
+      ok = bar_wait_warp(&sh.q_full, item_no & 1, failed) && filled(stage_no, info_no);
+      if (!ok) break;
+      tmem_after_sync();
+      for (int h = 0; h < halves; ++h) scores(h, stage_no);
+      commit(&sh.kv_empty[stage_no % S::kStages]);
+      if (n == 1) commit(&sh.q_empty);
+      for (int32_t j = 0; j < n && ok; ++j) {
+        const uint32_t v = stage_no + 1, next_key = stage_no + 2;
+        ok = filled(v, info_no);
+        for (int h = 0; h < halves && ok; ++h) {
+          ok = bar_wait_warp(&sh.p_full[h], tile_no[h] & 1, failed);
+          ++tile_no[h];
+          if (ok && j == 0) ok = bar_wait_warp(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed);
+          if (!ok) break;
+          tmem_after_sync();
+          sums(h, v, j > 0);
+          if (j + 1 < n) {
+            if (h == 0) ok = filled(next_key, info_no + 1);
+            if (!ok) break;
+            scores(h, next_key);
+          } else {
+            commit(&sh.o_full[h]);
+          }
+        }
+        if (!ok) break;
+        commit(&sh.kv_empty[v % S::kStages]);
+        if (j + 1 < n) commit(&sh.kv_empty[next_key % S::kStages]);
+        if (j + 2 == n) commit(&sh.q_empty);
+        stage_no += 2;
+        ++info_no;
+      }
+      ++item_no;
     }
+    // Whatever was issued is done before the memory that it uses is given back.
+    commit(&sh.done);
+    bar_wait(&sh.done, 0, &sh.stuck[0]);
   } else {
     // ------------------------------------------------------------- softmax
     const int h = warp >> 2, r = threadIdx.x;  // r: the row of the item
