@@ -470,6 +470,19 @@ __device__ __noinline__ void rescale_weights(uint32_t at, float by) {
   tmem_store16(at, p);
 }
 
+// 32 weights 2^y as 16-bit pairs, and their sum before that rounding.
+template <bool BF16>
+__device__ __forceinline__ float2 weights32(uint32_t (&p)[16], const float2 (&y)[16]) {
+  float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const float2 w = make_float2(fast_exp2(y[x].x), fast_exp2(y[x].y));
+    sum[x & 1] = add2(sum[x & 1], w);
+    p[x] = pack_pair<BF16>(w.x, w.y);
+  }
+  return add2(sum[0], sum[1]);
+}
+
 // What a row's softmax carries from tile to tile.
 struct RowState {
   float m;  // the maximum that the weights go by
@@ -483,7 +496,7 @@ struct RowState {
 template <bool QUANT, bool BF16, bool MASKED>
 __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, uint32_t s_at, uint32_t o_at, int o_columns,
                                             int32_t lo, int32_t hi, float f) {
-  float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+  float2 all = make_float2(row.l, 0.0f);
   const float2 ff = make_float2(f, f);
   uint32_t s[32];
   tmem_load32(s, s_at);
@@ -498,7 +511,6 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
     const uint32_t seen = MASKED ? seen_bits(info, piece, lo, hi) : 0;
     const float base = row.m == -INFINITY ? 0.0f : row.m;
     const float2 minus = make_float2(-base, -base);
-    float tops[2] = {-INFINITY, -INFINITY};
     tmem_wait_load(s);
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
@@ -509,10 +521,15 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
         y[x].y = seen >> (2 * x + 1) & 1 ? y[x].y : -INFINITY;
       }
       y[x] = fma2(y[x], ff, minus);
-      tops[x & 1] = max3_nan(tops[x & 1], y[x].x, y[x].y);
     }
     if (piece < 3) tmem_load32(s, s_at + (piece + 1) * 32);  // on its way meanwhile
-    const float top = max3_nan(tops[0], tops[1], tops[1]);
+    // The exponentials do not wait for the maximum: they are made again where it is passed.
+    uint32_t p[16];
+    float2 sum = weights32<BF16>(p, y);
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int x = 0; x < 16; ++x) tops[x & 3] = max3_nan(tops[x & 3], y[x].x, y[x].y);
+    const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
     const bool raise = top > (row.m == -INFINITY ? -INFINITY : kRaise);  // a NaN raises nothing: it reaches the sum
     if (__any_sync(0xffffffffu, raise)) {
       float keep = 1.0f;
@@ -523,26 +540,17 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
 #pragma unroll
         for (int x = 0; x < 16; ++x) y[x] = add2(y[x], shift);
         row.m = m;
-        row.l *= keep;
-        sum[0] = mul2(sum[0], make_float2(keep, keep));
-        sum[1] = mul2(sum[1], make_float2(keep, keep));
+        all = mul2(all, make_float2(keep, keep));
+        sum = weights32<BF16>(p, y);
       }
       __syncwarp();
       rescale_sums(o_at, o_columns, keep);
       for (int before = 0; before < piece; ++before) rescale_weights<BF16>(s_at + before * 16, keep);
     }
-    uint32_t p[16];
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      y[x].x = fast_exp2(y[x].x);
-      y[x].y = fast_exp2(y[x].y);
-      sum[x & 1] = add2(sum[x & 1], y[x]);
-      p[x] = pack_pair<BF16>(y[x].x, y[x].y);
-    }
+    all = add2(all, sum);
     tmem_store16(s_at + piece * 16, p);
   }
-  const float2 all = add2(sum[0], sum[1]);
-  row.l += all.x + all.y;
+  row.l = all.x + all.y;
 }
 
 template <uint32_t Q, uint32_t STORE, int DP>
