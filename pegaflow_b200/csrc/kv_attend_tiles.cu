@@ -30,6 +30,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attend.cuh"
 #include "kv_attend_tiles.h"
@@ -66,7 +67,7 @@ template <uint32_t Q, uint32_t STORE, int DP>
 struct Tiles {
   static constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
   static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;
-  static constexpr int kStages = DP == 128 ? 4 : 6;
+  static constexpr int kStages = 4;  // two tiles' K and V
   static constexpr int kTileBytes = 128 * DP * 2;  // 128 rows of Q, K or V: DP / 64 blocks of [128][128 bytes]
   struct Shared {
     unsigned char q[2][kTileBytes];
@@ -82,7 +83,7 @@ struct Tiles {
     int failed;  // a wait gave up
     int stuck[2];  // those for copies and products in flight did as well
   };
-  // TMEM columns.
+  // TMEM columns (all 512 are allocated, so they begin at 0).
   static constexpr uint32_t kS = 0, kO = 256;
 };
 
@@ -586,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = 0;
+  if (sh.tmem != 0) sh.failed = 1;  // cannot be: the waits would end the call
   wait_for_previous_kernel();  // the spans
   let_next_kernel_start();
 
@@ -863,26 +865,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return ok;
     };
-    auto scores = [&](int h, uint32_t stage) {
-      const uint64_t a = operand(q_at + h * S::kTileBytes, 16), b = operand(kv_at + stage % S::kStages * S::kTileBytes, 16);
+    // The stage and the half are constants here: addresses and descriptors are then uniform from the start, and an
+    // instruction is issued in its own time, not in that of six moves to uniform registers.
+    auto scores = [&](auto half, auto stage) {
+      constexpr int h = decltype(half)::value, st = decltype(stage)::value;
+      const uint64_t a = operand(q_at + h * S::kTileBytes, 16), b = operand(kv_at + st * S::kTileBytes, 16);
       if (elected()) {
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          constexpr uint32_t kBlock = 16384 >> 4, kStep = 32 >> 4;
-          const uint32_t off = (i >> 2) * kBlock + (i & 3) * kStep;
-          mma_ss(tmem + S::kS + h * 128, a + off, b + off, kScores, i > 0);
+        for (int x = 0; x < DP / 16; ++x) {
+          constexpr uint32_t kBlock = 16384 >> 4, kPiece = 32 >> 4;
+          const uint32_t off = (x >> 2) * kBlock + (x & 3) * kPiece;
+          mma_ss(S::kS + h * 128, a + off, b + off, kScores, x > 0);
         }
         mma_commit(&sh.s_full[h]);
       }
       __syncwarp();
     };
-    auto sums = [&](int h, uint32_t stage, bool add) {
-      const uint64_t b = operand(kv_at + stage % S::kStages * S::kTileBytes, 16384);
+    auto sums = [&](auto half, auto stage, bool add) {
+      constexpr int h = decltype(half)::value, st = decltype(stage)::value;
+      const uint64_t b = operand(kv_at + st * S::kTileBytes, 16384);
       if (elected()) {
+        mma_ts(S::kO + h * 128, S::kS + h * 128, b, kSums, add);
 #pragma unroll
-        for (int i = 0; i < kTileKeys / 16; ++i) {
-          mma_ts(tmem + S::kO + h * 128, tmem + S::kS + h * 128 + i * 8, b + i * (2048 >> 4), kSums, add || i > 0);
-        }
+        for (int x = 1; x < kTileKeys / 16; ++x) mma_ts(S::kO + h * 128, S::kS + h * 128 + x * 8, b + x * (2048 >> 4), kSums, true);
       }
       __syncwarp();
     };
@@ -890,40 +895,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elected()) mma_commit(bar);
       __syncwarp();
     };
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
     bool ok = true;
-    while (ok && walk.next(it)) {
-      const int halves = it.rows > 128 ? 2 : 1;
-      const int32_t n = it.unit1 - it.unit0;
-      ok = bar_wait_warp(&sh.q_full, item_no & 1, failed) && filled(stage_no, info_no);
-      if (!ok) break;
-      tmem_after_sync();
-      for (int h = 0; h < halves; ++h) scores(h, stage_no);
-      commit(&sh.kv_empty[stage_no % S::kStages]);
-      if (n == 1) commit(&sh.q_empty);
-      for (int32_t j = 0; j < n && ok; ++j) {
-        const uint32_t v = stage_no + 1, next_key = stage_no + 2;
-        ok = filled(v, info_no);
-        for (int h = 0; h < halves && ok; ++h) {
-          ok = bar_wait_warp(&sh.p_full[h], tile_no[h] & 1, failed);
-          ++tile_no[h];
-          if (ok && j == 0) ok = bar_wait_warp(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed);
-          if (!ok) break;
-          tmem_after_sync();
-          sums(h, v, j > 0);
-          if (j + 1 < n) {
-            if (h == 0) ok = filled(next_key, info_no + 1);
-            if (!ok) break;
-            scores(h, next_key);
-          } else {
-            commit(&sh.o_full[h]);
-          }
+    int32_t units = 0;  // of the item
+    int halves = 0;
+    // Tile j of the item, in the stages 2 B and 2 B + 1.
+    auto tile = [&](int32_t j, auto parity) {
+      constexpr int B = decltype(parity)::value;
+      using Key = std::integral_constant<int, 2 * B>;
+      using Value = std::integral_constant<int, 2 * B + 1>;
+      using NextKey = std::integral_constant<int, 2 - 2 * B>;
+      const uint32_t v = stage_no + 1, next_key = stage_no + 2;
+      if (j == 0) {
+        if (!(ok = filled(stage_no, info_no))) return;
+        tmem_after_sync();
+        scores(Zero{}, Key{});
+        if (halves == 2) scores(One{}, Key{});
+        commit(&sh.kv_empty[Key::value]);
+        if (units == 1) commit(&sh.q_empty);
+      }
+      if (!(ok = filled(v, info_no))) return;
+      auto half = [&](auto which) -> bool {
+        constexpr int h = decltype(which)::value;
+        if (!bar_wait_warp(&sh.p_full[h], tile_no[h]++ & 1, failed)) return false;
+        if (j == 0 && !bar_wait_warp(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed)) return false;
+        tmem_after_sync();
+        sums(which, Value{}, j > 0);
+        if (j + 1 < units) {
+          if (h == 0 && !filled(next_key, info_no + 1)) return false;
+          scores(which, NextKey{});
+        } else {
+          commit(&sh.o_full[h]);
         }
-        if (!ok) break;
-        commit(&sh.kv_empty[v % S::kStages]);
-        if (j + 1 < n) commit(&sh.kv_empty[next_key % S::kStages]);
-        if (j + 2 == n) commit(&sh.q_empty);
-        stage_no += 2;
-        ++info_no;
+        return true;
+      };
+      if (!(ok = half(Zero{}))) return;
+      if (halves == 2 && !(ok = half(One{}))) return;
+      commit(&sh.kv_empty[Value::value]);
+      if (j + 1 < units) commit(&sh.kv_empty[NextKey::value]);
+      if (j + 2 == units) commit(&sh.q_empty);
+      stage_no += 2;
+      ++info_no;
+    };
+    while (ok && walk.next(it)) {
+      halves = it.rows > 128 ? 2 : 1;
+      units = it.unit1 - it.unit0;
+      if (!(ok = bar_wait_warp(&sh.q_full, item_no & 1, failed))) break;
+      for (int32_t j = 0; j < units && ok; ++j) {
+        if (stage_no & 2) {
+          tile(j, One{});
+        } else {
+          tile(j, Zero{});
+        }
       }
       ++item_no;
     }
@@ -1068,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == kMmaWarp) {
     if (sh.failed) kv_flag(reinterpret_cast<int32_t*>(k.a.status), PF_KV_TIMED_OUT);
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem));
   }
 }
 
