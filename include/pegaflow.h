@@ -611,7 +611,8 @@ typedef struct pf_kv_rows {
   int64_t head_stride;
 } pf_kv_rows;
 
-/* Writes n tokens' K and V into the slots of a cache: slot = block *
+/* Writes n tokens' K and V (dense rows [n, heads, head_dim]: addresses, strides
+ * in elements, last axis contiguous) into the slots of a cache: slot = block *
  * block_size + offset; a negative slot is skipped (padding). Slots of one call
  * are distinct: of two equal ones either token may be left, or a mixture. Rows
  * are bf16, fp16 or fp32; a 16-bit cache takes them rounded to its type. An
@@ -620,8 +621,10 @@ typedef struct pf_kv_rows {
  * in fp32, with q = 448 (E4M3) or 127 (INT8), ties to even. A row that holds a
  * NaN or an infinity reads back as NaN. With given_scales != 0 the scales are
  * read, not written, and values beyond them saturate. */
-int pf_kv_write(int32_t device_id, const pf_kv_cache* cache,
-                const pf_kv_rows* key, const pf_kv_rows* value, uint32_t dtype,
+int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, uint64_t key,
+                int64_t key_token_stride, int64_t key_head_stride,
+                uint64_t value, int64_t value_token_stride,
+                int64_t value_head_stride, uint32_t dtype,
                 const int64_t* slots, uint64_t n, int given_scales,
                 int32_t* status, void* stream);
 
@@ -634,8 +637,10 @@ int pf_kv_write(int32_t device_id, const pf_kv_cache* cache,
 int pf_kv_read(int32_t device_id, const pf_kv_cache* cache,
                const int32_t* block_table, int64_t table_stride,
                uint32_t max_blocks, uint32_t n_seqs, const int32_t* starts,
-               const pf_kv_rows* key, const pf_kv_rows* value, uint32_t dtype,
-               uint64_t n_rows, int32_t* status, void* stream);
+               uint64_t key, int64_t key_token_stride, int64_t key_head_stride,
+               uint64_t value, int64_t value_token_stride,
+               int64_t value_head_stride, uint32_t dtype, uint64_t n_rows,
+               int32_t* status, void* stream);
 
 /* Attention of a chunk of new tokens over the cache, which already holds their
  * K and V: sequence s has the queries q_start[s] .. q_start[s + 1] and kv_len[s]

@@ -81,9 +81,10 @@ int null_arg(const char* what) {
 
 extern "C" {
 
-int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, const pf_kv_rows* key, const pf_kv_rows* value,
+int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, uint64_t key, int64_t key_token_stride,
+                int64_t key_head_stride, uint64_t value, int64_t value_token_stride, int64_t value_head_stride,
                 uint32_t dtype, const int64_t* slots, uint64_t n, int given_scales, int32_t* status, void* stream) {
-  if (!cache || !key || !value) return null_arg("cache or rows");
+  if (!cache) return null_arg("cache");
   return pf::guarded([&] {
     using namespace pf;
     check_cache(*cache);
@@ -99,19 +100,21 @@ int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, const pf_kv_rows* k
     }
     if (n > INT32_MAX || n * cache->heads > UINT32_MAX) refuse("too many tokens");
     if (!n) return;
-    check_rows(*key, dtype, "key");
-    check_rows(*value, dtype, "value");
+    const pf_kv_rows k{key, key_token_stride, key_head_stride}, v{value, value_token_stride, value_head_stride};
+    check_rows(k, dtype, "key");
+    check_rows(v, dtype, "value");
     if (!slots) refuse("no slots");
     DeviceGuard g(device_id);
-    const KvWriteArgs args{*cache, *key, *value, slots, n, status, dtype, given_scales ? 1u : 0u};
+    const KvWriteArgs args{*cache, k, v, slots, n, status, dtype, given_scales ? 1u : 0u};
     cuda_check(launch_kv_write(args, static_cast<cudaStream_t>(stream)), "kv_write launch");
   });
 }
 
 int pf_kv_read(int32_t device_id, const pf_kv_cache* cache, const int32_t* block_table, int64_t table_stride,
-               uint32_t max_blocks, uint32_t n_seqs, const int32_t* starts, const pf_kv_rows* key,
-               const pf_kv_rows* value, uint32_t dtype, uint64_t n_rows, int32_t* status, void* stream) {
-  if (!cache || !key || !value) return null_arg("cache or rows");
+               uint32_t max_blocks, uint32_t n_seqs, const int32_t* starts, uint64_t key, int64_t key_token_stride,
+               int64_t key_head_stride, uint64_t value, int64_t value_token_stride, int64_t value_head_stride,
+               uint32_t dtype, uint64_t n_rows, int32_t* status, void* stream) {
+  if (!cache) return null_arg("cache");
   return pf::guarded([&] {
     using namespace pf;
     check_cache(*cache);
@@ -120,11 +123,12 @@ int pf_kv_read(int32_t device_id, const pf_kv_cache* cache, const int32_t* block
     if (n_seqs > INT32_MAX / 2) refuse("too many sequences");
     if (!n_rows || !n_seqs) return;
     if (uint64_t(max_blocks) * cache->block_size > INT32_MAX) refuse("block table names more tokens than an int32 can count");
-    check_rows(*key, dtype, "key");
-    check_rows(*value, dtype, "value");
+    const pf_kv_rows k{key, key_token_stride, key_head_stride}, v{value, value_token_stride, value_head_stride};
+    check_rows(k, dtype, "key");
+    check_rows(v, dtype, "value");
     if ((!block_table && max_blocks) || !starts) refuse("no block table or starts");
     DeviceGuard g(device_id);
-    const KvReadArgs args{*cache, *key, *value, block_table, starts, status, table_stride, n_rows, max_blocks, n_seqs, dtype};
+    const KvReadArgs args{*cache, k, v, block_table, starts, status, table_stride, n_rows, max_blocks, n_seqs, dtype};
     cuda_check(launch_kv_read(args, static_cast<cudaStream_t>(stream)), "kv_read launch");
   });
 }

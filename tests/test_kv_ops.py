@@ -162,8 +162,8 @@ def test_library_refuses_caches(native, make, words):
     from ctypes import byref
 
     N = native
-    c, r = make(N), N.KvRows(4096, 128, 64)
-    rc = N.lib.pf_kv_write(0, byref(c), byref(r), byref(r), N.PF_DTYPE_BF16, 4096, 3, 0, 0, 0)
+    c, r = make(N), (4096, 128, 64)
+    rc = N.lib.pf_kv_write(0, byref(c), *r, *r, N.PF_DTYPE_BF16, 4096, 3, 0, 0, 0)
     assert rc == N.PF_ERR_INVALID_ARGUMENT and words in message(N), message(N)
 
 
@@ -171,12 +171,12 @@ def test_library_refuses_given_scales_of_16_bits(native):
     from ctypes import byref
 
     N = native
-    c, r = c_cache(N, N.PF_DTYPE_BF16), N.KvRows(4096, 128, 64)
-    rc = N.lib.pf_kv_write(0, byref(c), byref(r), byref(r), N.PF_DTYPE_BF16, 4096, 3, 1, 0, 0)
+    c, r = c_cache(N, N.PF_DTYPE_BF16), (4096, 128, 64)
+    rc = N.lib.pf_kv_write(0, byref(c), *r, *r, N.PF_DTYPE_BF16, 4096, 3, 1, 0, 0)
     assert rc == N.PF_ERR_INVALID_ARGUMENT and "no scales" in message(N)
-    rc = N.lib.pf_kv_write(0, byref(c), byref(r), byref(r), N.PF_DTYPE_E4M3, 4096, 3, 0, 0, 0)
+    rc = N.lib.pf_kv_write(0, byref(c), *r, *r, N.PF_DTYPE_E4M3, 4096, 3, 0, 0, 0)
     assert rc == N.PF_ERR_INVALID_ARGUMENT and "rows must be" in message(N)
-    assert N.lib.pf_kv_write(0, None, byref(r), byref(r), 0, 4096, 3, 0, 0, 0) == N.PF_ERR_INVALID_ARGUMENT
+    assert N.lib.pf_kv_write(0, None, *r, *r, 0, 4096, 3, 0, 0, 0) == N.PF_ERR_INVALID_ARGUMENT
 
 
 @pytest.mark.parametrize("make, change, words", [
@@ -216,9 +216,9 @@ def test_empty_calls_need_nothing(native):
     from ctypes import byref
 
     N = native
-    c, r = c_cache(N, N.PF_DTYPE_BF16), N.KvRows(0, 0, 0)
-    assert N.lib.pf_kv_write(0, byref(c), byref(r), byref(r), 0, None, 0, 0, 0, 0) == N.PF_OK
-    assert N.lib.pf_kv_read(0, byref(c), None, 0, 0, 0, None, byref(r), byref(r), 0, 5, 0, 0) == N.PF_OK
+    c, r = c_cache(N, N.PF_DTYPE_BF16), (0, 0, 0)
+    assert N.lib.pf_kv_write(0, byref(c), *r, *r, 0, None, 0, 0, 0, 0) == N.PF_OK
+    assert N.lib.pf_kv_read(0, byref(c), None, 0, 0, 0, None, *r, *r, 0, 5, 0, 0) == N.PF_OK
     a = attention(N, c, n_tokens=0)
     assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_OK
 
