@@ -3,18 +3,23 @@
 //
 // For one sequence and one KV head, the rows (its queries times the heads of the
 // group) are at most 8 or 16. A CTA takes a part of the tokens for them; its four
-// warps take batches of 64 tokens in turn, each warp on its own: its running
+// warps take batches of 32 tokens in turn, each warp on its own: its running
 // maximum, its sums, its accumulators, joined at the end of the part. Parts of a
 // sequence are joined by a second kernel.
+//
+// Each warp copies its rows (16-byte cp.async, from wherever the block table says)
+// into a ring of its own in shared memory, two steps of 16 tokens ahead: with 8 to
+// 16 warps on an SM 128 KB and more are on their way, what HBM's latency takes at
+// full rate. (Loads into registers, one step ahead, reached 60 % of it.)
 //
 // The products are transposed, so that a warp's matrix instructions (m16n8k16)
 // have 16 tokens or 16 values on the long side and 8 rows on the short one:
 //   S^T = K Q^T (16 tokens x 8 rows),  O^T += V^T P^T (16 values x 8 rows).
 // Their sums run over the head's values and over the tokens, whose order is free:
-// a lane takes as its share of a row whatever 16 bytes it can load at once, so K
-// and V go from global memory into registers in full sectors and from there into
-// the instructions, with no shared memory in between. A V^T fragment pairs two
-// tokens' values: one byte permutation. P^T is S^T transposed: one movmatrix.
+// a lane takes as its share of a row whatever 16 bytes it can read at once, and no
+// fragment needs a transposing read: codes and values alike go from 16-byte reads
+// into the instructions. A V^T fragment pairs two tokens' values: one byte
+// permutation. P^T is S^T transposed: one movmatrix.
 //
 // 8-bit codes become fp16, which holds all of e4m3 and int8 exactly; the scales
 // stay in fp32: K's multiplies the score, V's the weight. Weights are rounded to
@@ -33,11 +38,12 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kBatch = 64;  // tokens whose addresses and scales a warp stages at once
+constexpr int kBatch = 32;  // tokens whose addresses and scales a warp stages at once, one a lane
 constexpr int kStep = 16;   // tokens of one matrix instruction
+constexpr int kRing = 3;    // steps in a warp's ring
 
 struct Staged {
-  int64_t key;    // element offset of the token's K row, -1 if it has none
+  int64_t key;    // byte offset of the token's K row, -1 if it has none
   int64_t value;
   float key_scale;
   float value_scale;
@@ -55,6 +61,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+}
+
+// 16 bytes into shared memory, zeros if they are not there.
+__device__ __forceinline__ void copy16(void* to, const char* from, const char* valid, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(to))),
+               "l"(there ? from : valid), "r"(there ? 16 : 0)
+               : "memory");
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -89,17 +102,6 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
   return r;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void load_once(uint32_t (&r)[BYTES / 4], const void* p) {
-  if constexpr (BYTES == 16) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "l"(p));
-  } else {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
-  }
-}
-
 // Q, STORE: types. DP: head_dim rounded up to 64 or 128. NT: 8-row tiles.
 template <uint32_t Q, uint32_t STORE, int DP, int NT>
 struct Stream {
@@ -107,25 +109,40 @@ struct Stream {
   static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;  // type of the products
   static constexpr int kElt = kQuant ? 1 : 2;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kChunk = 16 / kElt;           // values of a 16-byte load
-  static constexpr int kKeyLoads = DP * kElt / 64;   // 16-byte loads of a lane for one K row
+  static constexpr int kChunk = 16 / kElt;           // values of 16 bytes
+  static constexpr int kKeyReads = DP * kElt / 64;   // 16-byte reads of a lane for one K row
   static constexpr int kValueBytes = DP / 8 * kElt;  // of a lane for one V row
-  static constexpr int kValueLoad = kValueBytes < 16 ? kValueBytes : 16;
-  static constexpr int kValueLoads = kValueBytes / kValueLoad;
+  static constexpr int kValueRead = kValueBytes < 16 ? kValueBytes : 16;
+  static constexpr int kValueReads = kValueBytes / kValueRead;
   static constexpr int kTiles = DP / 16;
-  using Elem = typename KvElem<STORE>::type;
+  static constexpr int kRowBytes = DP * kElt;
+  static constexpr int kPieces = kRowBytes / 16;
+  // CTAs on an SM: as many as shared memory holds (DP 128 in 16 bits: two), registers permitting.
+  static constexpr int kCtas = kRowBytes == 256 ? 2 : NT == 1 ? 4 : 2;
 
+  // A step's rows. 16-byte pieces are swizzled by the row so that a quarter warp's reads meet all banks: K's are
+  // of two neighbouring rows and four pieces, V's of four even (or odd) rows and two pieces.
+  struct Step {
+    unsigned char key[kStep][kRowBytes];
+    unsigned char value[kStep][kRowBytes];
+  };
+  static __device__ __forceinline__ int key_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row & 1) << 2 : piece; }
+  static __device__ __forceinline__ int value_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row >> 1 & 3) << 1 : piece ^ (row >> 1 & 3); }
   struct Shared {
+    union {
+      Step ring[kWarps][kRing];
+      float o[kWarps][sizeof(Step) * kRing / 4];  // [row][value] of a warp, when its ring is done with
+    };
     Staged staged[kWarps][2][kBatch];
-    float o[kWarps][kRows][DP];
     float m[kWarps][kRows];
     float l[kWarps][kRows];
     int bad[kRows];
   };
+  static_assert(sizeof(Step) * kRing >= kRows * DP * 4, "a warp's sums fit into its ring");
 };
 
 template <uint32_t Q, uint32_t STORE, int DP, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     kv_attend_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
   using S = Stream<Q, STORE, DP, NT>;
   using T = typename KvElem<Q>::type;
@@ -138,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
   const uint32_t seq = blockIdx.z / plan.tiles;
   const int32_t group = int32_t(k.a.q_heads / c.heads);
   let_next_kernel_start();
+  auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
 
   const KvSeq s = kv_sequence(k, seq);
   const int32_t rows = s.n * group;
@@ -164,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
                    int64_t(int32_t(head) * group + (on ? r - i * group : 0)) * k.a.query.head_stride;
       uint32_t raw[S::kTiles * 2];
 #pragma unroll
-      for (int j = 0; j < S::kKeyLoads; ++j) {
+      for (int j = 0; j < S::kKeyReads; ++j) {
         const int d = (t + 4 * j) * S::kChunk;
 #pragma unroll
         for (int h = 0; h < S::kChunk / 8; ++h) {
@@ -218,228 +236,229 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     const char* key_base = reinterpret_cast<const char*>(c.key.data);
     const char* value_base = reinterpret_cast<const char*>(c.value.data);
 
-    // Staging a batch takes three steps, so that no load is waited for at once:
-    // its tokens' blocks, then addresses and scales, then shared memory.
-    int32_t blocks[2];
-    Staged fresh[2];
+    // A batch's addresses and scales are made two batches ahead: its blocks are read first, a batch later the
+    // scales, and they go to shared memory when the batch before is begun. No read is waited for at once.
+    int32_t block = -1;
+    Staged fresh;
     auto stage_blocks = [&](int32_t batch) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int32_t j = lo + batch * kBatch + u * 32 + lane;
-        blocks[u] = j < hi ? kv_block(k, seq, uint32_t(j) / c.block_size) : -1;
-      }
+      const int32_t j = lo + batch * kBatch + lane;
+      block = j < hi ? kv_block(k, seq, page_of(j)) : -1;
     };
     auto stage_addresses = [&](int32_t batch) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Staged x{-1, -1, 0.0f, 0.0f};
-        if (blocks[u] >= 0) {
-          const int64_t b = blocks[u];
-          const int64_t at = uint32_t(lo + batch * kBatch + u * 32 + lane) % c.block_size;
-          x.key = b * c.key.block_stride + at * c.key.token_stride + int64_t(head) * c.key.head_stride;
-          x.value = b * c.value.block_stride + at * c.value.token_stride + int64_t(head) * c.value.head_stride;
-          if constexpr (S::kQuant) {
-            x.key_scale = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride +
-                                                                      int64_t(head) * c.key.scale_head_stride];
-            x.value_scale = reinterpret_cast<const float*>(
-                c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride +
-                               int64_t(head) * c.value.scale_head_stride];
-          }
-        }
-        fresh[u] = x;
-      }
-    };
-    auto stage_store = [&](int buf) {
-      sh.staged[warp][buf][lane] = fresh[0];
-      sh.staged[warp][buf][32 + lane] = fresh[1];
-      __syncwarp();
-    };
-
-    uint32_t kr[2][S::kKeyLoads][4];
-    uint32_t vr[4][S::kValueLoads][S::kValueLoad / 4];
-    auto load_keys = [&](int buf, int step) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t at = sh.staged[warp][buf][step * kStep + g + 8 * h].key;
-#pragma unroll
-        for (int j = 0; j < S::kKeyLoads; ++j) {
-          const int d = (t + 4 * j) * S::kChunk;
-          if (at >= 0 && d < int(c.head_dim)) {
-            load_once<16>(kr[h][j], key_base + (at + d) * S::kElt);
-          } else {
-            kr[h][j][0] = kr[h][j][1] = kr[h][j][2] = kr[h][j][3] = 0;
-          }
+      fresh = Staged{-1, -1, 0.0f, 0.0f};
+      if (block >= 0) {
+        const int64_t b = block;
+        const int32_t j = lo + batch * kBatch + lane;
+        const int64_t at = uint32_t(j) - page_of(j) * c.block_size;
+        fresh.key = (b * c.key.block_stride + at * c.key.token_stride + int64_t(head) * c.key.head_stride) * S::kElt;
+        fresh.value = (b * c.value.block_stride + at * c.value.token_stride + int64_t(head) * c.value.head_stride) * S::kElt;
+        if constexpr (S::kQuant) {
+          fresh.key_scale = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride +
+                                                                        int64_t(head) * c.key.scale_head_stride];
+          fresh.value_scale = reinterpret_cast<const float*>(
+              c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride +
+                             int64_t(head) * c.value.scale_head_stride];
         }
       }
     };
-    auto load_values = [&](int buf, int step) {
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int64_t at = sh.staged[warp][buf][step * kStep + 2 * t + (h & 1) + 8 * (h >> 1)].value;
-#pragma unroll
-        for (int j = 0; j < S::kValueLoads; ++j) {
-          const int d = (8 * j + g) * (S::kValueLoad / S::kElt);
-          if (at >= 0 && d < int(c.head_dim)) {
-            load_once<S::kValueLoad>(vr[h][j], value_base + (at + d) * S::kElt);
-          } else {
-#pragma unroll
-            for (int w = 0; w < S::kValueLoad / 4; ++w) vr[h][j][w] = 0;
-          }
-        }
-      }
-    };
-
     const int32_t batches = (max(0, hi - lo) + kBatch - 1) / kBatch;
-    int buf = 0;
-    if (warp < batches) {
+    // This warp's batches: warp, warp + 4, ...; step i is half of its batch i / 2.
+    const int32_t mine = warp < batches ? (batches - warp + kWarps - 1) / kWarps : 0;
+    typename S::Step* ring = sh.ring[warp];
+    auto copy_step = [&](int32_t i) {
+      if (i < 2 * mine) {
+        typename S::Step& to = ring[i % kRing];
+        const Staged* rows = &sh.staged[warp][i >> 1 & 1][(i & 1) * kStep];
+        constexpr int kRowsAtOnce = 32 / S::kPieces;
+        const int piece = lane % S::kPieces;
+        const bool there = piece * S::kChunk < int(c.head_dim);
+        int64_t key_at[kStep / kRowsAtOnce], value_at[kStep / kRowsAtOnce];
+#pragma unroll
+        for (int x = 0; x < kStep / kRowsAtOnce; ++x) {
+          key_at[x] = rows[x * kRowsAtOnce + lane / S::kPieces].key;
+          value_at[x] = rows[x * kRowsAtOnce + lane / S::kPieces].value;
+        }
+#pragma unroll
+        for (int x = 0; x < kStep / kRowsAtOnce; ++x) {
+          const int row = x * kRowsAtOnce + lane / S::kPieces;
+          copy16(to.key[row] + S::key_piece(row, piece) * 16, key_base + key_at[x] + piece * 16, key_base, there && key_at[x] >= 0);
+          copy16(to.value[row] + S::value_piece(row, piece) * 16, value_base + value_at[x] + piece * 16, value_base, there && value_at[x] >= 0);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    if (mine) {
       stage_blocks(warp);
       stage_addresses(warp);
-      stage_store(0);
-      load_keys(0, 0);
-      load_values(0, 0);
+      stage_blocks(warp + kWarps);
+      sh.staged[warp][0][lane] = fresh;
+      __syncwarp();
     }
-    for (int32_t batch = warp; batch < batches; batch += kWarps) {
-      const bool more = batch + kWarps < batches;
+    copy_step(0);
+    copy_step(1);
+    if (mine) {
+      stage_addresses(warp + kWarps);
+      stage_blocks(warp + 2 * kWarps);
+    }
+#pragma unroll 1
+    for (int32_t i = 0; i < 2 * mine; ++i) {
+      const int32_t batch = warp + (i >> 1) * kWarps, j0 = lo + batch * kBatch + (i & 1) * kStep;
+      if ((i & 1) == 0) {
+        // The next batch's addresses: its buffer's last readers are behind the end of the batch before.
+        sh.staged[warp][(i >> 1 & 1) ^ 1][lane] = fresh;
+        stage_addresses(batch + 2 * kWarps);
+        stage_blocks(batch + 3 * kWarps);
+      }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();  // this step's rows are there for all lanes, and all are done with the one before
+      copy_step(i + 2);
+      const typename S::Step& now = ring[i % kRing];
+      const Staged s0 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g], s1 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g + 8];
+
       float v_inv = 1.0f;
       if constexpr (S::kQuant) {
-        const uint32_t mine = max(__float_as_uint(sh.staged[warp][buf][lane].value_scale) & 0x7fffffffu,
-                                  __float_as_uint(sh.staged[warp][buf][32 + lane].value_scale) & 0x7fffffffu);
-        const uint32_t e = min(__reduce_max_sync(0xffffffffu, mine) >> 23, 253u);
+        const uint32_t largest = __float_as_uint(fmaxf(fabsf(s0.value_scale), fabsf(s1.value_scale)));
+        const uint32_t e = min(__reduce_max_sync(0xffffffffu, largest) >> 23, 253u);
         if (e > v_exp) {
           const float keep = e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int i = 0; i < S::kTiles; ++i) {
+            for (int x = 0; x < S::kTiles; ++x) {
 #pragma unroll
-              for (int x = 0; x < 4; ++x) o[n][i][x] *= keep;
+              for (int y = 0; y < 4; ++y) o[n][x][y] *= keep;
             }
           }
           v_exp = e;
         }
         v_inv = __uint_as_float((254 - v_exp) << 23);
       }
+      // S^T: c0, c1 are token g's scores for the rows 2 t and 2 t + 1, c2, c3 token g + 8's.
+      float x[NT][4];
 #pragma unroll
-      for (int step = 0; step < kBatch / kStep; ++step) {
-        const int32_t j0 = lo + batch * kBatch + step * kStep;
-        // S^T: c0, c1 are token g's scores for the rows 2 t and 2 t + 1, c2, c3 token g + 8's.
-        float x[NT][4];
+      for (int n = 0; n < NT; ++n) {
+        x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+      }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-        }
+      for (int j = 0; j < S::kKeyReads; ++j) {
+        const uint4 r0 = *reinterpret_cast<const uint4*>(now.key[g] + S::key_piece(g, t + 4 * j) * 16);
+        const uint4 r1 = *reinterpret_cast<const uint4*>(now.key[g + 8] + S::key_piece(g + 8, t + 4 * j) * 16);
+        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
+        for (int u = 0; u < S::kChunk / 4; ++u) {
+          const int tile = j * (S::kChunk / 4) + u;
           uint32_t a0, a1, a2, a3;
           if constexpr (S::kQuant) {
-            const uint32_t w0 = kr[0][i / 4][i % 4], w1 = kr[1][i / 4][i % 4];
-            a0 = codes_to_half2<STORE, false>(w0), a2 = codes_to_half2<STORE, true>(w0);
-            a1 = codes_to_half2<STORE, false>(w1), a3 = codes_to_half2<STORE, true>(w1);
+            a0 = codes_to_half2<STORE, false>(w0[u]), a2 = codes_to_half2<STORE, true>(w0[u]);
+            a1 = codes_to_half2<STORE, false>(w1[u]), a3 = codes_to_half2<STORE, true>(w1[u]);
           } else {
-            a0 = kr[0][i / 2][i % 2 * 2], a2 = kr[0][i / 2][i % 2 * 2 + 1];
-            a1 = kr[1][i / 2][i % 2 * 2], a3 = kr[1][i / 2][i % 2 * 2 + 1];
+            a0 = w0[2 * u], a2 = w0[2 * u + 1], a1 = w1[2 * u], a3 = w1[2 * u + 1];
           }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<S::kBf16>(x[n], a0, a1, a2, a3, q[n][i][0], q[n][i][1]);
-        }
-        const Staged s0 = sh.staged[warp][buf][step * kStep + g], s1 = sh.staged[warp][buf][step * kStep + g + 8];
-        // The next step's keys are on their way while this one's weights are made.
-        if (step + 1 < kBatch / kStep) {
-          load_keys(buf, step + 1);
-        } else if (more) {
-          stage_store(buf ^ 1);
-          load_keys(buf ^ 1, 0);
-        }
-        if (more && step == 0) stage_blocks(batch + kWarps);
-        if (more && step == 1) stage_addresses(batch + kWarps);
-
-        const bool masked = j0 < all_lo || j0 + kStep > all_hi || __any_sync(0xffffffffu, s0.key < 0 || s1.key < 0);
-        bool raise = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = x[n][e] * f[n][e & 1];
-            if constexpr (S::kQuant) y *= e < 2 ? s0.key_scale : s1.key_scale;
-            x[n][e] = y;
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int32_t j = j0 + g + (e < 2 ? 0 : 8);
-              const bool on = (e < 2 ? s0.key : s1.key) >= 0 && j >= row_lo[n][e & 1] && j < row_hi[n][e & 1];
-              x[n][e] = on ? x[n][e] : -INFINITY;
-            }
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          raise = raise || fmaxf(x[n][0], x[n][2]) > m[n][0] + kRaise || fmaxf(x[n][1], x[n][3]) > m[n][1] + kRaise;
-        }
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float keep[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(x[n][e], x[n][e + 2]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              top = fmaxf(top, m[n][e]);
-              keep[e] = top == -INFINITY ? 0.0f : fast_exp2(m[n][e] - top);
-              m[n][e] = top;
-              l[n][e] *= keep[e];
-            }
-#pragma unroll
-            for (int i = 0; i < S::kTiles; ++i) {
-              o[n][i][0] *= keep[0], o[n][i][1] *= keep[1], o[n][i][2] *= keep[0], o[n][i][3] *= keep[1];
-            }
-          }
-        }
-        uint32_t p[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float base = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-            w[e] = fast_exp2(x[n][e] - base);
-            l[n][e & 1] += w[e];
-            if constexpr (S::kQuant) w[e] *= (e < 2 ? s0.value_scale : s1.value_scale) * v_inv;
-          }
-          p[n][0] = transpose_8x8(pack2<S::kBf16>(w[0], w[1]));
-          p[n][1] = transpose_8x8(pack2<S::kBf16>(w[2], w[3]));
-        }
-#pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (S::kQuant) {
-            const int w = i / 2;
-            const uint32_t sel = i % 2 ? 0x7362 : 0x5140;
-            const uint32_t u = __byte_perm(vr[0][0][w], vr[1][0][w], sel), v = __byte_perm(vr[2][0][w], vr[3][0][w], sel);
-            a0 = codes_to_half2<STORE, false>(u), a1 = codes_to_half2<STORE, true>(u);
-            a2 = codes_to_half2<STORE, false>(v), a3 = codes_to_half2<STORE, true>(v);
-          } else {
-            a0 = __byte_perm(vr[0][i / 4][i % 4], vr[1][i / 4][i % 4], 0x5410);
-            a1 = __byte_perm(vr[0][i / 4][i % 4], vr[1][i / 4][i % 4], 0x7632);
-            a2 = __byte_perm(vr[2][i / 4][i % 4], vr[3][i / 4][i % 4], 0x5410);
-            a3 = __byte_perm(vr[2][i / 4][i % 4], vr[3][i / 4][i % 4], 0x7632);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma<S::kBf16>(o[n][i], a0, a1, a2, a3, p[n][0], p[n][1]);
-        }
-        if (step + 1 < kBatch / kStep) {
-          load_values(buf, step + 1);
-        } else if (more) {
-          load_values(buf ^ 1, 0);
+          for (int n = 0; n < NT; ++n) mma<S::kBf16>(x[n], a0, a1, a2, a3, q[n][tile][0], q[n][tile][1]);
         }
       }
-      buf ^= 1;
+
+      const bool masked = j0 < all_lo || j0 + kStep > all_hi || __any_sync(0xffffffffu, s0.key < 0 || s1.key < 0);
+      bool raise = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = x[n][e] * f[n][e & 1];
+          if constexpr (S::kQuant) y *= e < 2 ? s0.key_scale : s1.key_scale;
+          x[n][e] = y;
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t j = j0 + g + (e < 2 ? 0 : 8);
+            const bool on = (e < 2 ? s0.key : s1.key) >= 0 && j >= row_lo[n][e & 1] && j < row_hi[n][e & 1];
+            x[n][e] = on ? x[n][e] : -INFINITY;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        raise = raise || fmaxf(x[n][0], x[n][2]) > m[n][0] + kRaise || fmaxf(x[n][1], x[n][3]) > m[n][1] + kRaise;
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(x[n][e], x[n][e + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[n][e]);
+            keep[e] = top == -INFINITY ? 0.0f : fast_exp2(m[n][e] - top);
+            m[n][e] = top;
+            l[n][e] *= keep[e];
+          }
+#pragma unroll
+          for (int y = 0; y < S::kTiles; ++y) {
+            o[n][y][0] *= keep[0], o[n][y][1] *= keep[1], o[n][y][2] *= keep[0], o[n][y][3] *= keep[1];
+          }
+        }
+      }
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float base = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+          w[e] = fast_exp2(x[n][e] - base);
+          l[n][e & 1] += w[e];
+          if constexpr (S::kQuant) w[e] *= (e < 2 ? s0.value_scale : s1.value_scale) * v_inv;
+        }
+        p[n][0] = transpose_8x8(pack2<S::kBf16>(w[0], w[1]));
+        p[n][1] = transpose_8x8(pack2<S::kBf16>(w[2], w[3]));
+      }
+      // V^T: the tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of this lane's values.
+#pragma unroll
+      for (int j = 0; j < S::kValueReads; ++j) {
+        uint32_t w[4][S::kValueRead / 4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int row = 2 * t + (h & 1) + 8 * (h >> 1);
+          if constexpr (S::kValueRead == 16) {
+            const uint4 r = *reinterpret_cast<const uint4*>(now.value[row] + S::value_piece(row, g + 8 * j) * 16);
+            w[h][0] = r.x, w[h][1] = r.y, w[h][2] = r.z, w[h][3] = r.w;
+          } else {
+            const uint2 r = *reinterpret_cast<const uint2*>(now.value[row] + S::value_piece(row, g >> 1) * 16 + (g & 1) * 8);
+            w[h][0] = r.x, w[h][1] = r.y;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < S::kValueRead / 4; ++u) {
+          if constexpr (S::kQuant) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t sel = z ? 0x7362 : 0x5140;
+              const uint32_t lo2 = __byte_perm(w[0][u], w[1][u], sel), hi2 = __byte_perm(w[2][u], w[3][u], sel);
+              const uint32_t a0 = codes_to_half2<STORE, false>(lo2), a1 = codes_to_half2<STORE, true>(lo2);
+              const uint32_t a2 = codes_to_half2<STORE, false>(hi2), a3 = codes_to_half2<STORE, true>(hi2);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma<S::kBf16>(o[n][2 * u + z], a0, a1, a2, a3, p[n][0], p[n][1]);
+            }
+          } else {
+            const uint32_t a0 = __byte_perm(w[0][u], w[1][u], 0x5410), a1 = __byte_perm(w[0][u], w[1][u], 0x7632);
+            const uint32_t a2 = __byte_perm(w[2][u], w[3][u], 0x5410), a3 = __byte_perm(w[2][u], w[3][u], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<S::kBf16>(o[n][4 * j + u], a0, a1, a2, a3, p[n][0], p[n][1]);
+          }
+        }
+      }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();  // the ring is free for the sums
 
     // The warps' shares, then the part's: [row][value] in shared memory.
     const float v_unit = S::kQuant ? __uint_as_float(v_exp << 23) : 1.0f;
@@ -460,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
       for (int i = 0; i < S::kTiles; ++i) {
         const int d = S::kQuant ? g * (DP / 8) + 2 * i : (i / 4 * 8 + g) * 8 + i % 4 * 2;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh.o[warp][n * 8 + 2 * t + (e & 1)][d + (e >> 1)] = o[n][i][e] * v_unit;
+        for (int e = 0; e < 4; ++e) sh.o[warp][(n * 8 + 2 * t + (e & 1)) * DP + d + (e >> 1)] = o[n][i][e] * v_unit;
       }
     }
     if (threadIdx.x < S::kRows) sh.bad[threadIdx.x] = 0;
@@ -498,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
       for (int w = 0; w < kWarps; ++w) {
         const float keep = top == -INFINITY ? 1.0f : exp2f(sh.m[w][row] - top);
         sum += sh.l[w][row] * keep;
-        value += sh.o[w][row][d] * keep;
+        value += sh.o[w][row * DP + int32_t(d)] * keep;
       }
       if (uneven && sum == sum && !isfinite(value)) {
         sh.bad[row] = 1;
@@ -527,14 +546,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
   }
 }
 
-// Joins the parts of the rows that have several, a warp for each row: weights
-// 2^(m_part - max) over the parts' sums. Reads the parts once: HBM or L2.
+// Joins the parts of the rows that have several: weights 2^(m_part - max) over the
+// parts' sums. A block takes a row, its warps parts in turn, so that as many loads
+// are in flight as a row has parts; a lane has 4 values.
+constexpr int kJoinWarps = 8;
 template <uint32_t Q, int DP>
-__global__ void __launch_bounds__(128) kv_join_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
+__global__ void __launch_bounds__(kJoinWarps * 32) kv_join_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
   using T = typename KvElem<Q>::type;
-  const int lane = threadIdx.x & 31;
-  const uint64_t id = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (id >= k.a.n_tokens * k.a.q_heads) return;
+  __shared__ float4 values[kJoinWarps][32];
+  __shared__ float sums[kJoinWarps], tops[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t id = blockIdx.x;
   const uint32_t token = uint32_t(id / k.a.q_heads), qh = uint32_t(id % k.a.q_heads);
   const uint32_t seq = kv_find_seq(reinterpret_cast<const int32_t*>(k.a.q_start), k.a.n_seqs, token);
   if (seq == k.a.n_seqs) return;
@@ -548,21 +570,47 @@ __global__ void __launch_bounds__(128) kv_join_stream_kernel(const __grid_consta
   if (used == 1) return;
   wait_for_previous_kernel();
   const float* ws = reinterpret_cast<const float*>(k.a.workspace) + id * plan.parts * (DP + 4);
-  float top = -INFINITY;
-  for (int32_t p = lane; p < used; p += 32) top = fmaxf(top, ws[int64_t(p) * (DP + 4)]);
-  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
+  // The warp's own running maximum, then the block's.
+  float top = -INFINITY, sum = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int32_t p = 0; p < used; ++p) {
-    const float* w = ws + int64_t(p) * (DP + 4);
-    const float keep = exp2f(w[0] - base);
-    sum += w[1] * keep;
-    if (lane * 4 < DP) {
-      const float4 v = *reinterpret_cast<const float4*>(w + 4 + lane * 4);
-      o.x += v.x * keep, o.y += v.y * keep, o.z += v.z * keep, o.w += v.w * keep;
+  const bool mine = lane * 4 < DP;
+#pragma unroll 1
+  for (int32_t p0 = warp; p0 < used; p0 += 4 * kJoinWarps) {
+    float m[4], l[4];
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int32_t p = p0 + u * kJoinWarps;
+      const float* w = ws + int64_t(p) * (DP + 4);
+      m[u] = p < used ? w[0] : -INFINITY;
+      l[u] = p < used ? w[1] : 0.0f;
+      v[u] = p < used && mine ? *reinterpret_cast<const float4*>(w + 4 + lane * 4) : make_float4(0, 0, 0, 0);
     }
+    const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+    const float base = now == -INFINITY ? 0.0f : now;
+    const float keep = exp2f(top - base);
+    sum *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+    top = now;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float by = exp2f(m[u] - base);
+      sum += l[u] * by;
+      o.x += v[u].x * by, o.y += v[u].y * by, o.z += v[u].z * by, o.w += v[u].w * by;
+    }
+  }
+  values[warp][lane] = o;
+  if (lane == 0) sums[warp] = sum, tops[warp] = top;
+  __syncthreads();
+  if (warp) return;
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  sum = 0.0f, o = make_float4(0, 0, 0, 0);
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float by = exp2f(tops[w] - base);
+    const float4 v = values[w][lane];
+    sum += sums[w] * by;
+    o.x += v.x * by, o.y += v.y * by, o.z += v.z * by, o.w += v.w * by;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (lane * 4 < int(k.cache.head_dim)) {
@@ -582,6 +630,12 @@ uint32_t most_queries(const KvAttendArgs& k) {
   return static_cast<uint32_t>(k.a.max_q ? std::min<uint64_t>(k.a.max_q, n) : n);
 }
 
+// Stream<>::kCtas for a call.
+uint32_t ctas_per_sm(const KvAttendArgs& k, const KvStreamPlan& p) {
+  const uint32_t row = (k.cache.head_dim <= 64 ? 64 : 128) * kv_dtype_bytes(k.cache.dtype);
+  return row == 256 ? 2 : p.row_tiles == 1 ? 4 : 2;
+}
+
 template <uint32_t Q, uint32_t STORE, int DP, int NT>
 cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
   using S = Stream<Q, STORE, DP, NT>;
@@ -599,8 +653,8 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<uint32_t>((k.a.n_tokens * k.a.q_heads + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<uint32_t>(k.a.n_tokens * k.a.q_heads));
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
@@ -628,6 +682,7 @@ cudaError_t launch_store(const KvAttendArgs& k, const KvStreamPlan& p, cudaStrea
 
 KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   KvStreamPlan p;
+  p.page_shift = page_shift(k.cache);
   const uint32_t rows = most_queries(k) * (k.a.q_heads / k.cache.heads);
   p.row_tiles = rows <= 8 ? 1 : 2;
   p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
@@ -635,14 +690,23 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   if (k.a.max_kv) longest = std::min<uint64_t>(longest, k.a.max_kv);
   if (k.a.window) longest = std::min<uint64_t>(longest, uint64_t(k.a.window) + most_queries(k));
   longest = std::max<uint64_t>(longest, 1);
-  // About twelve CTAs for each SM, four rounds of the three that fit: the last round's idle share is small, and a
-  // part's start (addresses, queries) and end (joining) stay small beside its tokens.
+  // Parts of equal length: the CTAs run in rounds of as many as fit, each round as long as a part and its start and
+  // end (queries, addresses, joining: about 128 tokens' time). Few sequences: one round, whose parts are as short as
+  // that leaves them. Many: sequences are rarely equally long, so among splits that are within a tenth of the best
+  // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 315 us in one round, 228 in seven).
   const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * p.tiles * k.cache.heads);
-  uint64_t parts = std::max<uint64_t>(1, uint64_t(num_sms) * 12 / items);
-  uint64_t tokens = (longest + parts - 1) / parts;
-  tokens = (tokens + kStreamMinPart - 1) / kStreamMinPart * kStreamMinPart;
-  tokens = std::max<uint64_t>(tokens, 4 * kStreamMinPart);
-  p.part_tokens = static_cast<int32_t>(std::min<uint64_t>(tokens, 1u << 30));
+  const uint64_t slots = uint64_t(num_sms) * ctas_per_sm(k, p);
+  const uint64_t units = (longest + kStreamMinPart - 1) / kStreamMinPart;  // shortest parts
+  auto cost = [&](uint64_t per) {
+    const uint64_t parts = (units + per - 1) / per;
+    return (items * parts + slots - 1) / slots * (per + 1);
+  };
+  uint64_t best = UINT64_MAX;
+  for (uint64_t per = 1; per <= units; per += (per + 15) / 16) best = std::min(best, cost(per));
+  uint64_t per = 1;
+  while (per < units && cost(per) * 10 > best * 11) per += (per + 15) / 16;
+  per = std::min(per, units);
+  p.part_tokens = static_cast<int32_t>(std::min<uint64_t>(per * kStreamMinPart, 1u << 30));
   p.parts = static_cast<uint32_t>((longest + p.part_tokens - 1) / p.part_tokens);
   return p;
 }

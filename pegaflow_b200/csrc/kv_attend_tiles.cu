@@ -1235,10 +1235,7 @@ KvTilePlan tile_plan(const KvAttendArgs& k, int num_sms) {
   KvTilePlan p{};
   p.ctas = uint32_t(num_sms);
   const uint32_t page = k.cache.block_size;
-  p.page_shift = -1;
-  for (int i = 0; i < 31; ++i) {
-    if (page == 1u << i) p.page_shift = i;
-  }
+  p.page_shift = page_shift(k.cache);
   // Boxes of whole swizzle groups (8 rows) that tile 128 rows.
   p.box_rows = page % kTileKeys == 0 ? kTileKeys : page >= 8 && kTileKeys % page == 0 ? page : 0;
   auto take = [&p](uint64_t bytes) {

@@ -21,6 +21,14 @@ inline uint32_t kv_dtype_bytes(uint32_t dtype) {
   return dtype == PF_DTYPE_FP32 ? 4 : kv_quantised(dtype) ? 1 : 2;
 }
 
+// log2 of the block size, -1 if it is no power of two.
+inline int32_t page_shift(const pf_kv_cache& c) {
+  for (int32_t i = 0; i < 31; ++i) {
+    if (c.block_size == 1u << i) return i;
+  }
+  return -1;
+}
+
 struct KvWriteArgs {
   pf_kv_cache cache;
   pf_kv_rows key;
