@@ -27,7 +27,7 @@ void check_cache(const pf_kv_cache& c) {
   if (c.dtype == PF_DTYPE_FP32 || c.dtype > PF_DTYPE_INT8) refuse("cache dtype must be bf16, fp16, e4m3 or int8");
   if (!c.num_blocks || !c.block_size || !c.heads) refuse("cache must have blocks, tokens and heads");
   if (c.num_blocks > INT32_MAX) refuse("cache has more blocks than an int32 can name");
-  if (c.block_size > (1u << 20) || c.heads > (1u << 16)) refuse("cache block_size or heads out of range");
+  if (c.block_size > (1u << 20) || c.heads > (1u << 14)) refuse("cache block_size or heads out of range");
   if (!c.head_dim || c.head_dim > kKvMaxHeadDim) refuse("head_dim must be 1 to 256");
   check_side(c, c.key, "key");
   check_side(c, c.value, "value");
