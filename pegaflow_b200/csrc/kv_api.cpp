@@ -105,7 +105,7 @@ int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, uint64_t key, int64
     check_rows(v, dtype, "value");
     if (!slots) refuse("no slots");
     DeviceGuard g(device_id);
-    const KvWriteArgs args{*cache, k, v, slots, n, status, dtype, given_scales ? 1u : 0u};
+    const KvWriteArgs args{*cache, k, v, slots, n, status, dtype, given_scales ? 1u : 0u, uint32_t(num_sms(device_id))};
     cuda_check(launch_kv_write(args, static_cast<cudaStream_t>(stream)), "kv_write launch");
   });
 }

@@ -38,6 +38,7 @@ struct KvWriteArgs {
   int32_t* status;
   uint32_t dtype;
   uint32_t given_scales;
+  uint32_t num_sms;
 };
 
 struct KvReadArgs {

@@ -35,9 +35,26 @@ template <uint32_t STORE>
 constexpr int kReadElems = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8 ? 16 : 8;
 constexpr uint32_t kReadMaxTokens = 64;  // of a block
 
+// Strides in bytes that fit 32 bits, so that a step of an address is one
+// multiplication (32 x 32 + 64 bits).
+struct Strides {
+  uint32_t a, b, c;
+};
+template <typename T>
+__device__ __forceinline__ T* address(uint64_t base, const Strides& s, uint32_t a, uint32_t b, uint32_t c) {
+  return reinterpret_cast<T*>(base + uint64_t(a) * s.a + uint64_t(b) * s.b + uint64_t(c) * s.c);
+}
+struct RowStrides {
+  Strides key, value, key_scale, value_scale;  // block, token, head
+  Strides key_rows, value_rows;                // token, head, -
+};
+
 struct WritePlan {
   uint32_t log_l;        // lanes of a row: a power of two
-  uint32_t tokens;       // of a block
+  uint32_t tokens;       // whose rows a block takes together
+  uint32_t turns;        // that it needs for them, each a row for each group of lanes
+  uint32_t all_turns;
+  RowStrides strides;
   float heads_inverse;
   int32_t page_shift;
 };
@@ -46,6 +63,7 @@ struct ReadPlan {
   uint32_t tokens;       // of a block
   uint32_t pieces;       // 16-byte pieces of a token's rows of one side
   uint32_t row_pieces;   // of one row
+  RowStrides strides;
   float pieces_inverse;
   float row_inverse;
   int32_t page_shift;
@@ -244,51 +262,63 @@ __device__ __forceinline__ uint2 eight_codes(const float2 (&x)[4], float inv, bo
   return make_uint2(r[0], r[1]);
 }
 
+constexpr uint32_t kWriteBlocks = 6;  // of 256 threads and 40 registers
 template <uint32_t IN, uint32_t STORE>
-__global__ void __launch_bounds__(kThreads) kv_write_rows_kernel(const __grid_constant__ KvWriteArgs a, const WritePlan plan) {
+__global__ void __launch_bounds__(kThreads, kWriteBlocks) kv_write_rows_kernel(const __grid_constant__ KvWriteArgs a, const WritePlan plan) {
   using T = typename KvElem<IN>::type;
   using S = typename KvElem<STORE>::type;
   constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
   const uint32_t lane = threadIdx.x & ((1u << plan.log_l) - 1), d = lane * 8;
   const uint32_t heads = a.cache.heads;
   const bool inside = d < a.cache.head_dim;
-  const uint32_t first = blockIdx.x * plan.tokens;
-  const uint32_t rows = uint32_t(min(uint64_t(plan.tokens), a.n - first)) * heads;
-  // All lanes of a warp go on together: their groups' shuffles are warp-wide.
-  for (uint32_t row0 = 0; row0 < rows; row0 += kThreads >> plan.log_l) {
-    const uint32_t row = row0 + (threadIdx.x >> plan.log_l);
-    bool on = row < rows;
-    const uint32_t in = on ? divide(row, plan.heads_inverse) : 0;
-    const uint32_t head = on ? row - in * heads : 0, token = first + in;
-    const int64_t slot = on ? a.slots[token] : -1;
-    EightRaw<IN> k{}, v{};
+  // A turn's row: read while the turn before is worked on.
+  struct Row {
+    EightRaw<IN> k, v;
+    int64_t slot;
+    uint32_t head;
+  };
+  auto read = [&](uint32_t turn) {
+    Row r{};
+    r.slot = -1;
+    if (turn >= plan.all_turns) return r;
+    const uint32_t set = plan.turns == 1 ? turn : turn / plan.turns;
+    const uint32_t row = (turn - set * plan.turns) * (kThreads >> plan.log_l) + (threadIdx.x >> plan.log_l);
+    const uint32_t in = divide(row, plan.heads_inverse);
+    const uint64_t token = uint64_t(set) * plan.tokens + in;
+    if (in >= plan.tokens || token >= a.n) return r;
+    r.head = row - in * heads;
+    r.slot = a.slots[token];
     if (inside) {
-      k = *reinterpret_cast<const EightRaw<IN>*>(reinterpret_cast<const T*>(a.key.data) + int64_t(token) * a.key.token_stride +
-                                                 int64_t(head) * a.key.head_stride + d);
-      v = *reinterpret_cast<const EightRaw<IN>*>(reinterpret_cast<const T*>(a.value.data) + int64_t(token) * a.value.token_stride +
-                                                 int64_t(head) * a.value.head_stride + d);
+      r.k = *address<const EightRaw<IN>>(a.key.data, plan.strides.key_rows, uint32_t(token), r.head, d);
+      r.v = *address<const EightRaw<IN>>(a.value.data, plan.strides.value_rows, uint32_t(token), r.head, d);
     }
-    on = on && slot >= 0;
+    return r;
+  };
+  // All lanes of a warp go on together: their groups' shuffles are warp-wide.
+  Row next = read(blockIdx.x);
+  for (uint32_t turn = blockIdx.x; turn < plan.all_turns; turn += gridDim.x) {
+    const EightRaw<IN> k = next.k, v = next.v;
+    const int64_t slot = next.slot;
+    const uint32_t head = next.head;
+    next = read(turn + gridDim.x);
+    bool on = slot >= 0;
     if (on && uint64_t(slot) >= a.cache.num_blocks * a.cache.block_size) {
       kv_flag(a.status, PF_KV_BAD_BLOCK);
       on = false;
     }
-    const int64_t block = !on ? 0 : plan.page_shift >= 0 ? slot >> plan.page_shift : slot / int64_t(a.cache.block_size);
-    const int64_t offset = on ? slot - block * a.cache.block_size : 0;
+    // A slot of the cache: its block fits 31 bits.
+    const uint32_t block = !on ? 0 : uint32_t(plan.page_shift >= 0 ? slot >> plan.page_shift : slot / int64_t(a.cache.block_size));
+    const uint32_t offset = on ? uint32_t(slot) - block * a.cache.block_size : 0;
     float2 x[4], y[4];
     to_pairs<IN>(x, k);
     to_pairs<IN>(y, v);
-    S* kp = reinterpret_cast<S*>(a.cache.key.data) + block * a.cache.key.block_stride + offset * a.cache.key.token_stride +
-            int64_t(head) * a.cache.key.head_stride + d;
-    S* vp = reinterpret_cast<S*>(a.cache.value.data) + block * a.cache.value.block_stride + offset * a.cache.value.token_stride +
-            int64_t(head) * a.cache.value.head_stride + d;
+    S* kp = address<S>(a.cache.key.data, plan.strides.key, block, offset, head) + d;
+    S* vp = address<S>(a.cache.value.data, plan.strides.value, block, offset, head) + d;
     if constexpr (kQuant) {
       // Even lanes make K's scale, odd ones V's (a group of one lane both, one after the other).
       float ks, vs, ki, vi;
-      float* ksp = reinterpret_cast<float*>(a.cache.key.scale) + block * a.cache.key.scale_block_stride +
-                   offset * a.cache.key.scale_token_stride + int64_t(head) * a.cache.key.scale_head_stride;
-      float* vsp = reinterpret_cast<float*>(a.cache.value.scale) + block * a.cache.value.scale_block_stride +
-                   offset * a.cache.value.scale_token_stride + int64_t(head) * a.cache.value.scale_head_stride;
+      float* ksp = address<float>(a.cache.key.scale, plan.strides.key_scale, block, offset, head);
+      float* vsp = address<float>(a.cache.value.scale, plan.strides.value_scale, block, offset, head);
       if (a.given_scales) {
         ks = on ? *ksp : 1.0f, vs = on ? *vsp : 1.0f;
         ki = 1.0f / ks, vi = 1.0f / vs;
@@ -420,24 +450,20 @@ __global__ void __launch_bounds__(kThreads) kv_read_rows_kernel(const __grid_con
     const uint32_t head = divide(at, plan.row_inverse), d = (at - head * plan.row_pieces) * E;
     const int2 p = place[in];
     if (p.x == -2) continue;
-    const int64_t b = max(p.x, 0), offset = p.y;
+    const uint32_t b = uint32_t(max(p.x, 0)), offset = uint32_t(p.y);
     uint4 k = make_uint4(0, 0, 0, 0), v = k;
     float ks = 0.0f, vs = 0.0f;
     if (p.x >= 0) {
-      k = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.cache.key.data) + b * a.cache.key.block_stride +
-                                          offset * a.cache.key.token_stride + int64_t(head) * a.cache.key.head_stride + d);
-      v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.cache.value.data) + b * a.cache.value.block_stride +
-                                          offset * a.cache.value.token_stride + int64_t(head) * a.cache.value.head_stride + d);
+      k = *reinterpret_cast<const uint4*>(address<const T>(a.cache.key.data, plan.strides.key, b, offset, head) + d);
+      v = *reinterpret_cast<const uint4*>(address<const T>(a.cache.value.data, plan.strides.value, b, offset, head) + d);
       if constexpr (kQuant) {
-        ks = reinterpret_cast<const float*>(a.cache.key.scale)[b * a.cache.key.scale_block_stride + offset * a.cache.key.scale_token_stride +
-                                                               int64_t(head) * a.cache.key.scale_head_stride];
-        vs = reinterpret_cast<const float*>(a.cache.value.scale)[b * a.cache.value.scale_block_stride + offset * a.cache.value.scale_token_stride +
-                                                                 int64_t(head) * a.cache.value.scale_head_stride];
+        ks = *address<const float>(a.cache.key.scale, plan.strides.key_scale, b, offset, head);
+        vs = *address<const float>(a.cache.value.scale, plan.strides.value_scale, b, offset, head);
       }
     }
-    const int64_t row = int64_t(first) + in;
-    store_piece<STORE, OUT>(reinterpret_cast<O*>(a.key.data) + row * a.key.token_stride + int64_t(head) * a.key.head_stride + d, k, ks);
-    store_piece<STORE, OUT>(reinterpret_cast<O*>(a.value.data) + row * a.value.token_stride + int64_t(head) * a.value.head_stride + d, v, vs);
+    const uint32_t row = first + in;
+    store_piece<STORE, OUT>(address<O>(a.key.data, plan.strides.key_rows, row, head, 0) + d, k, ks);
+    store_piece<STORE, OUT>(address<O>(a.value.data, plan.strides.value_rows, row, head, 0) + d, v, vs);
   }
 }
 
@@ -456,6 +482,24 @@ bool rows_pack(const pf_kv_rows& r, uint32_t dtype, int e) {
   return r.data % bytes == 0 && multiple(r.token_stride, r.head_stride, 0, int64_t(bytes / kv_dtype_bytes(dtype)));
 }
 
+// The strides in bytes, if they fit 32 bits.
+bool fit(const int64_t (&s)[3], uint64_t bytes, Strides* out) {
+  for (int64_t x : s) {
+    if (x < 0 || uint64_t(x) * bytes > UINT32_MAX) return false;
+  }
+  *out = Strides{uint32_t(s[0] * bytes), uint32_t(s[1] * bytes), uint32_t(s[2] * bytes)};
+  return true;
+}
+bool fit_all(const pf_kv_cache& c, const pf_kv_rows& key, const pf_kv_rows& value, uint32_t dtype, RowStrides* out) {
+  const uint64_t n = kv_dtype_bytes(c.dtype), m = kv_dtype_bytes(dtype);
+  return fit({c.key.block_stride, c.key.token_stride, c.key.head_stride}, n, &out->key) &&
+         fit({c.value.block_stride, c.value.token_stride, c.value.head_stride}, n, &out->value) &&
+         fit({c.key.scale_block_stride, c.key.scale_token_stride, c.key.scale_head_stride}, 4, &out->key_scale) &&
+         fit({c.value.scale_block_stride, c.value.scale_token_stride, c.value.scale_head_stride}, 4, &out->value_scale) &&
+         fit({key.token_stride, key.head_stride, 1}, m, &out->key_rows) &&
+         fit({value.token_stride, value.head_stride, 1}, m, &out->value_rows);
+}
+
 // Lanes of a row's group: the power of two that covers dim / 8, at most 32.
 uint32_t group_log(uint32_t dim) {
   uint32_t l = 0;
@@ -466,11 +510,15 @@ uint32_t group_log(uint32_t dim) {
 template <uint32_t IN, uint32_t STORE>
 void write_as(const KvWriteArgs& a, cudaStream_t stream) {
   const uint32_t log_l = group_log(a.cache.head_dim), heads = a.cache.heads, groups = kThreads >> log_l;
+  RowStrides strides;
   if (side_packs(a.cache, a.cache.key, 8) && side_packs(a.cache, a.cache.value, 8) && rows_pack(a.key, IN, 8) &&
-      rows_pack(a.value, IN, 8)) {
-    const uint32_t tokens = std::max(1u, groups / heads);
-    const WritePlan plan{log_l, tokens, 1.0f / float(heads), page_shift(a.cache)};
-    kv_write_rows_kernel<IN, STORE><<<static_cast<uint32_t>((a.n + tokens - 1) / tokens), kThreads, 0, stream>>>(a, plan);
+      rows_pack(a.value, IN, 8) && fit_all(a.cache, a.key, a.value, IN, &strides)) {
+    const uint32_t tokens = std::max(1u, groups / heads), turns = (tokens * heads + groups - 1) / groups;
+    const uint32_t all = static_cast<uint32_t>((a.n + tokens - 1) / tokens) * turns;
+    const WritePlan plan{log_l, tokens, turns, all, strides, 1.0f / float(heads), page_shift(a.cache)};
+    // As many blocks as an SM holds, so that all but a small call's rows are read a turn ahead.
+    const uint32_t grid = std::min(all, a.num_sms * kWriteBlocks);
+    kv_write_rows_kernel<IN, STORE><<<grid, kThreads, 0, stream>>>(a, plan);
   } else {
     kv_write_elements_kernel<IN, STORE><<<static_cast<uint32_t>((a.n * heads + groups - 1) / groups), kThreads, 0, stream>>>(a, log_l);
   }
@@ -490,12 +538,13 @@ template <uint32_t STORE, uint32_t OUT>
 void read_as(const KvReadArgs& a, cudaStream_t stream) {
   constexpr int E = kReadElems<STORE>;
   const uint32_t heads = a.cache.heads;
+  RowStrides strides;
   if (side_packs(a.cache, a.cache.key, E) && side_packs(a.cache, a.cache.value, E) && rows_pack(a.key, OUT, E) &&
-      rows_pack(a.value, OUT, E)) {
+      rows_pack(a.value, OUT, E) && fit_all(a.cache, a.key, a.value, OUT, &strides)) {
     const uint32_t row = a.cache.head_dim / E, pieces = heads * row;
     // Two pieces for each thread; more tokens than kReadMaxTokens only where a token has few pieces.
     const uint32_t tokens = std::min(kReadMaxTokens, std::max(1u, 2 * kThreads / pieces));
-    const ReadPlan plan{tokens, pieces, row, 1.0f / float(pieces), 1.0f / float(row), page_shift(a.cache)};
+    const ReadPlan plan{tokens, pieces, row, strides, 1.0f / float(pieces), 1.0f / float(row), page_shift(a.cache)};
     kv_read_rows_kernel<STORE, OUT><<<static_cast<uint32_t>((a.n_rows + tokens - 1) / tokens), kThreads, 0, stream>>>(a, plan);
   } else {
     const uint64_t pairs = a.n_rows * heads;
