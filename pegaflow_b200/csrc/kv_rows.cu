@@ -262,9 +262,11 @@ __device__ __forceinline__ uint2 eight_codes(const float2 (&x)[4], float inv, bo
   return make_uint2(r[0], r[1]);
 }
 
-constexpr uint32_t kWriteBlocks = 6;  // of 256 threads and 40 registers
+// Blocks that an SM holds: 256 threads of 40 registers, of 64 where a lane's eight values are fp32.
+template <uint32_t IN>
+constexpr uint32_t kWriteBlocks = IN == PF_DTYPE_FP32 ? 4 : 6;
 template <uint32_t IN, uint32_t STORE>
-__global__ void __launch_bounds__(kThreads, kWriteBlocks) kv_write_rows_kernel(const __grid_constant__ KvWriteArgs a, const WritePlan plan) {
+__global__ void __launch_bounds__(kThreads, kWriteBlocks<IN>) kv_write_rows_kernel(const __grid_constant__ KvWriteArgs a, const WritePlan plan) {
   using T = typename KvElem<IN>::type;
   using S = typename KvElem<STORE>::type;
   constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
@@ -517,7 +519,7 @@ void write_as(const KvWriteArgs& a, cudaStream_t stream) {
     const uint32_t all = static_cast<uint32_t>((a.n + tokens - 1) / tokens) * turns;
     const WritePlan plan{log_l, tokens, turns, all, strides, 1.0f / float(heads), page_shift(a.cache)};
     // As many blocks as an SM holds, so that all but a small call's rows are read a turn ahead.
-    const uint32_t grid = std::min(all, a.num_sms * kWriteBlocks);
+    const uint32_t grid = std::min(all, a.num_sms * kWriteBlocks<IN>);
     kv_write_rows_kernel<IN, STORE><<<grid, kThreads, 0, stream>>>(a, plan);
   } else {
     kv_write_elements_kernel<IN, STORE><<<static_cast<uint32_t>((a.n * heads + groups - 1) / groups), kThreads, 0, stream>>>(a, log_l);
