@@ -21,10 +21,11 @@
 // at a time by 16-byte copies, with zeros for tokens that are not there: any
 // block size works, and nothing behind a sequence's end is ever multiplied.
 //
-// 8-bit codes become fp16, which holds all of e4m3 and int8 exactly, on the way
-// into shared memory. K's scales stay in fp32 and multiply the scores; V's are
-// multiplied into the values there, which rounds them to fp16 (2^-11, the weights'
-// own rounding) after division by a power of two that follows the largest scale.
+// 8-bit codes are copied into their stage as they are and become fp16, which holds
+// all of e4m3 and int8 exactly, there. K's scales stay in fp32 and multiply the scores; V's are
+// multiplied into the values there, in fp16, after division by a power of two that
+// follows the largest scale: two roundings of 2^-11, the weights' own. (In fp32 it
+// took the loading warps longer than all else that they do.)
 // As in the streaming kernel a bf16 query is brought into fp16's range by a power
 // of two for each row.
 #include <cuda.h>
@@ -108,6 +109,7 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
 // wait of this CTA gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* failed) {
   if (bar_try(bar, parity)) return true;
+  if (*reinterpret_cast<volatile int*>(failed)) return false;
   const long long t0 = clock64();
   for (;;) {
 #pragma unroll 1
@@ -252,10 +254,10 @@ __device__ __forceinline__ uint2 codes_to_half4(uint32_t x) {
   return r;
 }
 
-// Four codes times a scale: the product in fp32, rounded once to fp16.
-__device__ __forceinline__ uint2 times_half4(uint2 x, float by) {
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
-  return make_uint2(pack_pair<false>(a.x * by, a.y * by), pack_pair<false>(b.x * by, b.y * by));
+// Four codes times a scale, in fp16.
+__device__ __forceinline__ uint2 times_half4(uint2 x, __half2 by) {
+  const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&x.x), by), b = __hmul2(*reinterpret_cast<const __half2*>(&x.y), by);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 // One CTA's walk along its span: every role does it for itself.
@@ -599,6 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------- loading
     const int tid = threadIdx.x - kSoftmaxWarps * 32;
     uint32_t tile_no = 0, stage_no = 0, item_no = 0;
+    // A thread whose wait gave up goes on without copying to the next place where all loading threads meet.
+    bool ok = true;
     // Copies rows of 16-bit values; their arrival counts for the stage's barrier by itself (the products' thread
     // orders them before its instructions' reads).
     auto copy_rows = [&](const int64_t* at, uint64_t data) -> bool {
@@ -630,26 +634,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++stage_no;
       return true;
     };
-    // Rows of codes: loaded ahead into registers, written as fp16.
-    constexpr int kCodePieces = DP / 16;  // 16-byte loads of a row
+    // Rows of codes: copied as they are into the stage's upper half, then read by all loading threads and, when all
+    // have, written over it as fp16.
+    constexpr int kCodePieces = DP / 16;  // 16-byte pieces of a row
     constexpr int kCodeRows = kLoadThreads / kCodePieces;
     constexpr int kCodeLoads = (kTileKeys + kCodeRows - 1) / kCodeRows;
-    using Codes = uint4[S::kQuant ? kCodeLoads : 1];
-    auto load_codes = [&](Codes& codes, const int64_t* at, uint64_t data) {
-      const int piece = tid % kCodePieces;
-      const bool there = piece * 16 < int(c.head_dim);
+    auto copy_codes = [&](uint32_t stage, const int64_t* at, uint64_t data) -> bool {
+      const bool free = bar_wait(&sh.kv_empty[stage % S::kStages], (stage / S::kStages & 1) ^ 1, failed);
+      if (free) {
+        const int piece = tid % kCodePieces;
+        const bool there = piece * 16 < int(c.head_dim);
+        const uint32_t base = smem_u32(sh.kv[stage % S::kStages]) + S::kTileBytes / 2 + piece * 16;
+        const char* from = reinterpret_cast<const char*>(data) + piece * 16;
+        int64_t off[kCodeLoads];
+#pragma unroll
+        for (int i = 0; i < kCodeLoads; ++i) {
+          const int r = tid / kCodePieces + i * kCodeRows;
+          off[i] = r < kTileKeys ? at[r] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kCodeLoads; ++i) {
+          const int r = tid / kCodePieces + i * kCodeRows;
+          const bool on = there && off[i] >= 0;
+          if (r < kTileKeys) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + r * DP),
+                         "l"(on ? from + off[i] : reinterpret_cast<const char*>(data)), "r"(on ? 16 : 0)
+                         : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      return free;
+    };
+    auto expand_codes = [&](uint32_t stage, const float* scales, float inv) -> bool {
+      if (!loaders_agree(ok)) return false;  // all copies are there
+      unsigned char* base = sh.kv[stage % S::kStages];
+      uint4 codes[kCodeLoads];
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
         const int r = tid / kCodePieces + i * kCodeRows;
-        const int64_t off = r < kTileKeys ? at[r] : -1;
-        codes[i] = make_uint4(0, 0, 0, 0);
-        if (there && off >= 0) codes[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(data) + off + piece * 16);
+        if (r < kTileKeys) codes[i] = *reinterpret_cast<const uint4*>(base + S::kTileBytes / 2 + r * DP + tid % kCodePieces * 16);
       }
-    };
-    auto store_codes = [&](const Codes& codes, const float* scales, float inv) -> bool {
-      if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
+      loaders_agree(true);  // and read
       const int piece = tid % kCodePieces * 2;  // of 16 bytes of fp16
-      unsigned char* base = sh.kv[stage_no % S::kStages] + (piece >> 3) * 16384;
+      base += (piece >> 3) * 16384;
 #pragma unroll
       for (int i = 0; i < kCodeLoads; ++i) {
         const int r = tid / kCodePieces + i * kCodeRows;
@@ -657,33 +685,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint2 x = codes_to_half4<STORE>(codes[i].x), y = codes_to_half4<STORE>(codes[i].y);
         uint2 z = codes_to_half4<STORE>(codes[i].z), w = codes_to_half4<STORE>(codes[i].w);
         if (scales) {
-          const float by = scales[r] * inv;  // below 2
+          const __half2 by = __float2half2_rn(scales[r] * inv);  // below 2
           x = times_half4(x, by), y = times_half4(y, by), z = times_half4(z, by), w = times_half4(w, by);
         }
-        *reinterpret_cast<uint4*>(base + r * 128 + ((piece & 7) ^ (r & 7)) * 16) = make_uint4(x.x, x.y, y.x, y.y);
-        *reinterpret_cast<uint4*>(base + r * 128 + (((piece & 7) + 1) ^ (r & 7)) * 16) = make_uint4(z.x, z.y, w.x, w.y);
+        // Eight threads write a row: those of its second block the other piece first, so that all banks are met.
+        const uint4 lo = make_uint4(x.x, x.y, y.x, y.y), hi = make_uint4(z.x, z.y, w.x, w.y);
+        const int swapped = piece >> 3;
+        *reinterpret_cast<uint4*>(base + r * 128 + (((piece & 7) + swapped) ^ (r & 7)) * 16) = swapped ? hi : lo;
+        *reinterpret_cast<uint4*>(base + r * 128 + (((piece & 7) + (swapped ^ 1)) ^ (r & 7)) * 16) = swapped ? lo : hi;
       }
       fence_async_shared();
-      bar_arrive(&sh.kv_full[stage_no++ % S::kStages]);
+      bar_arrive(&sh.kv_full[stage % S::kStages]);
       return true;
     };
 
-    // A thread whose wait gave up goes on without copying to the next place where all loading threads meet.
-    bool ok = true;
     while (loaders_agree(ok) && walk.next(it)) {
       auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
       // Each thread's tokens of a tile: tid and, for the first warp, tid + 96.
       auto token_of = [&](int32_t unit, int u) { return it.begin + unit * kTileKeys + tid + u * kLoadThreads; };
-      int32_t block[2];
-      auto look_up = [&](int32_t unit) {
+      int32_t block[2], ahead[2] = {-1, -1};
+      auto look_up = [&](int32_t unit, int32_t (&to)[2]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int32_t j = token_of(unit, u);
           const bool on = unit < it.unit1 && tid + u * kLoadThreads < kTileKeys && j >= it.first && j < it.end;
-          block[u] = on ? kv_block(k, it.seq, page_of(j)) : -1;
+          to[u] = on ? kv_block(k, it.seq, page_of(j)) : -1;
         }
       };
-      look_up(it.unit0);
+      // A tile's scales, a tile ahead: `block` is its own by then.
+      float ks[2] = {0.0f, 0.0f}, vs[2] = {0.0f, 0.0f};
+      auto load_scales = [&](int32_t unit) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ks[u] = vs[u] = 0.0f;
+          if (block[u] >= 0) {
+            const int32_t j = token_of(unit, u);
+            const int64_t b = block[u], at = uint32_t(j) - page_of(j) * c.block_size;
+            ks[u] = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride + it.head * c.key.scale_head_stride];
+            vs[u] = reinterpret_cast<const float*>(c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride + it.head * c.value.scale_head_stride];
+          }
+        }
+      };
+      look_up(it.unit0, block);
+      if constexpr (S::kQuant) load_scales(it.unit0);
 
       // Q: a thread for a row at a time, of both tiles.
       ok = loaders_agree(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
@@ -745,14 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           info.key_at[x] = b < 0 ? -1 : (b * c.key.block_stride + at * c.key.token_stride + it.head * c.key.head_stride) * kElt;
           info.value_at[x] = b < 0 ? -1 : (b * c.value.block_stride + at * c.value.token_stride + it.head * c.value.head_stride) * kElt;
           if constexpr (S::kQuant) {
-            float ks = 0.0f, vs = 0.0f;
-            if (b >= 0) {
-              ks = reinterpret_cast<const float*>(c.key.scale)[b * c.key.scale_block_stride + at * c.key.scale_token_stride + it.head * c.key.scale_head_stride];
-              vs = reinterpret_cast<const float*>(c.value.scale)[b * c.value.scale_block_stride + at * c.value.scale_token_stride + it.head * c.value.scale_head_stride];
-            }
-            info.key_scale[x] = ks;
-            info.value_scale[x] = vs;
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs) & 0x7fffffffu);
+            info.key_scale[x] = ks[u];
+            info.value_scale[x] = vs[u];
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs[u]) & 0x7fffffffu);
             if (lane == 0) sh.warp_max[tile_no & 1][x >> 5] = top;
           }
         }
@@ -809,23 +848,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       if constexpr (S::kQuant) {
-        // A tile's V is on its way while its K is converted, the next tile's K while this one's V is.
-        Codes key, value;
+        // Two stages' copies are on their way while one is expanded: this tile's V and the next one's K.
         if (!prepare(it.unit0)) break;
-        load_codes(key, sh.info[tile_no % kInfos].key_at, c.key.data);
+        const KeyInfo* info = &sh.info[tile_no % kInfos];
+        ok = copy_codes(stage_no, info->key_at, c.key.data);
+        ok = copy_codes(stage_no + 1, info->value_at, c.value.data) && ok;
+        look_up(it.unit0 + 1, block);
+        bool broken = false;
         for (int32_t unit = it.unit0; unit < it.unit1; ++unit) {
-          const KeyInfo& info = sh.info[tile_no % kInfos];
           const float inv = v_inv;
-          look_up(unit + 1);
-          load_codes(value, info.value_at, c.value.data);
-          ok = ok && store_codes(key, nullptr, 0.0f);
+          const float* scales = info->value_scale;
+          const bool more = unit + 1 < it.unit1;
+          // What the next tile needs is read while this one's K is expanded.
+          load_scales(unit + 1);
+          look_up(unit + 2, ahead);
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          broken = !expand_codes(stage_no, nullptr, 0.0f);
+          if (broken) break;
           ++tile_no;
-          if (unit + 1 < it.unit1) {
-            if (!prepare(unit + 1)) break;
-            load_codes(key, sh.info[tile_no % kInfos].key_at, c.key.data);
+          if (more) {
+            broken = !prepare(unit + 1);
+            if (broken) break;
+            info = &sh.info[tile_no % kInfos];
+            ok = copy_codes(stage_no + 2, info->key_at, c.key.data);
+            block[0] = ahead[0], block[1] = ahead[1];
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
           }
-          ok = ok && store_codes(value, info.value_scale, inv);
+          broken = !expand_codes(stage_no + 1, scales, inv);
+          if (broken) break;
+          if (more) ok = copy_codes(stage_no + 3, info->value_at, c.value.data);
+          stage_no += 2;
         }
+        if (broken) break;
       } else {
         for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
           if (!prepare(unit)) break;
@@ -840,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!loaders_agree(true)) break;  // the offsets are written
             ok = copy_rows(info.key_at, c.key.data) && copy_rows(info.value_at, c.value.data);
           }
-          look_up(unit + 1);
+          look_up(unit + 1, block);
         }
       }
       ++item_no;
