@@ -12,8 +12,8 @@
 // units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
 // 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
 //
-// Warps 0-3 and 4-7: the softmax of the two tiles. 8-10: load Q, K and V. 11:
-// issues the products. mbarriers order them; every wait is bounded, and one that
+// Warps 0-3 and 4-7: the softmax of the two halves. Three, or seven over an 8-bit
+// cache: load Q, K and V. The last: issues the products. mbarriers order them; every wait is bounded, and one that
 // runs out ends the call with a status bit and no hang.
 //
 // A tile of 128 16-bit keys comes by TMA, a box of each block, where all 128 are
@@ -40,10 +40,6 @@ namespace pf {
 namespace {
 
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 3;
-constexpr int kLoadThreads = kLoadWarps * 32;
-constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;  // 12 warps: 168 registers each
 constexpr int kInfos = 4;
 constexpr long long kWaitClocks = 2000000000ll;  // of the SM, for each wait: a second or a little more
 
@@ -69,6 +65,11 @@ struct Tiles {
   static constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
   static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;
   static constexpr int kStages = 4;  // two tiles' K and V
+  // 16 bits: 12 warps of 168 registers. 8 bits: expanding codes keeps seven warps busy, so 16 of 128 registers.
+  static constexpr int kLoadWarps = kQuant ? 7 : 3;
+  static constexpr int kLoadThreads = kLoadWarps * 32;
+  static constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kTileBytes = 128 * DP * 2;  // 128 rows of Q, K or V: DP / 64 blocks of [128][128 bytes]
   struct Shared {
     unsigned char q[2][kTileBytes];
@@ -129,12 +130,13 @@ __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, in
   return __all_sync(0xffffffffu, bar_wait(bar, parity, failed));
 }
 // Meets the other loading threads; whether all of them say yes.
+template <int THREADS>
 __device__ __forceinline__ bool loaders_agree(bool ok) {
   uint32_t all;
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
       : "=r"(all)
-      : "r"(uint32_t(ok)), "n"(kLoadThreads)
+      : "r"(uint32_t(ok)), "n"(THREADS)
       : "memory");
   return all;
 }
@@ -557,11 +559,12 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
 }
 
 template <uint32_t Q, uint32_t STORE, int DP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
     kv_attend_tiles_kernel(const __grid_constant__ KvAttendArgs k, const __grid_constant__ KvTilePlan plan,
                            const __grid_constant__ KvBoxMaps maps) {
   using S = Tiles<Q, STORE, DP>;
   using T = typename KvElem<Q>::type;
+  constexpr int kLoadThreads = S::kLoadThreads, kMmaWarp = S::kMmaWarp;
   extern __shared__ unsigned char raw_smem[];
   typename S::Shared& sh =
       *reinterpret_cast<typename S::Shared*>(raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023));
@@ -667,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return free;
     };
     auto expand_codes = [&](uint32_t stage, const float* scales, float inv) -> bool {
-      if (!loaders_agree(ok)) return false;  // all copies are there
+      if (!loaders_agree<kLoadThreads>(ok)) return false;  // all copies are there
       unsigned char* base = sh.kv[stage % S::kStages];
       uint4 codes[kCodeLoads];
 #pragma unroll
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r = tid / kCodePieces + i * kCodeRows;
         if (r < kTileKeys) codes[i] = *reinterpret_cast<const uint4*>(base + S::kTileBytes / 2 + r * DP + tid % kCodePieces * 16);
       }
-      loaders_agree(true);  // and read
+      loaders_agree<kLoadThreads>(true);  // and read
       const int piece = tid % kCodePieces * 2;  // of 16 bytes of fp16
       base += (piece >> 3) * 16384;
 #pragma unroll
@@ -699,9 +702,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
 
-    while (loaders_agree(ok) && walk.next(it)) {
+    while (loaders_agree<kLoadThreads>(ok) && walk.next(it)) {
       auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
-      // Each thread's tokens of a tile: tid and, for the first warp, tid + 96.
+      // Each thread's tokens of a tile: tid and, with three warps, tid + 96 for the first.
       auto token_of = [&](int32_t unit, int u) { return it.begin + unit * kTileKeys + tid + u * kLoadThreads; };
       int32_t block[2], ahead[2] = {-1, -1};
       auto look_up = [&](int32_t unit, int32_t (&to)[2]) {
@@ -730,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (S::kQuant) load_scales(it.unit0);
 
       // Q: a thread for a row at a time, of both tiles.
-      ok = loaders_agree(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
+      ok = loaders_agree<kLoadThreads>(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
       if (!ok) break;
 #pragma unroll 1
       for (int r = tid; r < kTileRows; r += kLoadThreads) {
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         KeyInfo& info = sh.info[tile_no % kInfos];
         ok = ok && bar_wait(&sh.info_empty[tile_no % kInfos], (tile_no / kInfos & 1) ^ 1, failed);
         const uint32_t seen = __ballot_sync(0xffffffffu, block[0] >= 0);
-        if (lane == 0) info.seen[tid >> 5] = seen;
+        if (lane == 0 && tid < kTileKeys) info.seen[tid >> 5] = seen;
         if (tid < kTileKeys - kLoadThreads) {
           const uint32_t last = __ballot_sync(0xffffffffu, block[1] >= 0);
           if (lane == 0) info.seen[kLoadThreads / 32] = last;
@@ -808,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (S::kQuant) offsets(unit, info);
         // Meeting here also keeps the slots apart: who writes a slot again (kInfos tiles on; warp_max: two) has
         // met those who read it last.
-        ok = loaders_agree(ok);
+        ok = loaders_agree<kLoadThreads>(ok);
         if (!ok) return false;
         if constexpr (S::kQuant) {
           const uint32_t* w = sh.warp_max[tile_no & 1];
@@ -893,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = load_boxes(unit, maps.key) && load_boxes(unit, maps.value);
           } else {
             offsets(unit, info);
-            if (!loaders_agree(true)) break;  // the offsets are written
+            if (!loaders_agree<kLoadThreads>(true)) break;  // the offsets are written
             ok = copy_rows(info.key_at, c.key.data) && copy_rows(info.value_at, c.value.data);
           }
           look_up(unit + 1, block);
@@ -1267,7 +1270,7 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t s
   }
   kv_tile_spans_kernel<<<1, 1024, 0, stream>>>(k, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  if ((err = launch_early(kernel, dim3(p.ctas), kThreads, shm, stream, k, plan, maps)) != cudaSuccess) return err;
+  if ((err = launch_early(kernel, dim3(p.ctas), Tiles<Q, STORE, DP>::kThreads, shm, stream, k, plan, maps)) != cudaSuccess) return err;
   return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 4), 256, 0, stream, k, p);
 }
 
