@@ -595,7 +595,11 @@ def fp8_evict_result(args) -> dict:
     warm prefix is restored layer by layer while a dummy per-layer compute
     kernel (0.5 ms) runs on a second stream as soon as its layer is in place,
     then the cold half is saved. Compared with waiting for the whole load
-    before computing."""
+    before computing.
+
+    With ``--fp8-compute attention`` the compute of a layer is what a model does
+    there: the request's new tokens (up to 2,048) are quantised into their blocks
+    and attend, 32 query heads on 8, over the restored prefix and themselves."""
     import torch
 
     from pegaflow_b200 import Layout, PegaEngine, PyLoadState
@@ -609,6 +613,18 @@ def fp8_evict_result(args) -> dict:
     kv = [torch.randint(0, 256, (2, nb, 16, 8, 128), generator=g, device="cuda:0", dtype=torch.uint8)
           for _ in range(layers)]
     sc = [torch.rand((nb,), generator=g, device="cuda:0", dtype=torch.float32) for _ in range(layers)]
+    attend = args.fp8_compute == "attention"
+    if attend:
+        from pegaflow_b200 import KVCache, chunk_attention, kv_write
+
+        # Codes of normal values (random bit patterns hold NaNs) at scales that make them about 1.
+        for t, s in zip(kv, sc):
+            t.copy_((torch.randn((nb, 16, 8, 128), generator=g, device="cuda:0") * 100).to(torch.float8_e4m3fn)
+                    .view(torch.uint8))
+            s.mul_(0.01).add_(0.005)
+        caches = [KVCache.from_tensor(t, s) for t, s in zip(kv, sc)]
+        new_kv = torch.randn((2, 2048, 8, 128), generator=g, device="cuda:0").to(torch.bfloat16)
+        query = torch.randn((2048, 32, 128), generator=g, device="cuda:0").to(torch.bfloat16)
     # Forward order, each layer's KV next to its scales: a load restores its
     # layers in the order the request lists them, so layer i is usable once
     # entries 2i and 2i+1 are in place.
@@ -646,11 +662,30 @@ def fp8_evict_result(args) -> dict:
             if time.perf_counter() > deadline:
                 raise TimeoutError("load did not complete")
 
+    def chunk_of(hit, dst):
+        """The request's new tokens: their slots, and what attention needs to know (made once, for all layers)."""
+        n = min((len(dst) - hit) * 16, 2048)
+        pos = torch.arange(hit * 16, hit * 16 + n)
+        ids = torch.tensor(dst)
+        with torch.cuda.stream(compute):
+            return (n, hit * 16 + n, (ids[pos // 16] * 16 + pos % 16).cuda(), ids.to(torch.int32).view(1, -1).cuda(),
+                    torch.tensor([0, n], dtype=torch.int32).cuda(),
+                    torch.tensor([hit * 16 + n], dtype=torch.int32).cuda())
+
+    def compute_layer(li, chunk):
+        if not attend:
+            torch.cuda._sleep(cycles)
+            return
+        n, total, slots, table, q_start, kv_len = chunk
+        kv_write(caches[li], new_kv[0, :n], new_kv[1, :n], slots, given_scales=True)
+        chunk_attention(query[:n], caches[li], table, q_start, kv_len, max_q=n, max_kv=total)
+
     def serve(r, overlap):
         nblk = blocks_per_req[r]
         hs_all = hashes(r, 0, nblk)
         hit = eng.count_prefix_hit_blocks("fp8", hs_all)
         dst = ids_for(50_000 + r, nblk)
+        chunk = chunk_of(hit, dst) if attend else None
         t0 = time.perf_counter()
         state = PyLoadState(len(names))
         if hit:
@@ -664,7 +699,7 @@ def fp8_evict_result(args) -> dict:
             elif hit and li == 0:
                 wait_ready(state)
             with torch.cuda.stream(compute):
-                torch.cuda._sleep(cycles)
+                compute_layer(li, chunk)
         t_issue = time.perf_counter()
         wait_ready(state)
         load_done = time.perf_counter()
@@ -700,7 +735,8 @@ def fp8_evict_result(args) -> dict:
         "vs_baseline": None, "dtype": "u8", "data": "synthetic (seeded e4m3 bit patterns + fp32 scales)",
         "config": {"workload": "llama8b_fp8_evict", "layers": "32 KV + 32 scale", "pool_gb": args.fp8_pool_gb,
                    "requests": n_req, "prefix_tokens": "U[1024,16384] seed 6", "warm_fraction": 0.5,
-                   "compute_ms_per_layer": args.fp8_compute_ms},
+                   "compute_ms_per_layer": args.fp8_compute_ms if not attend else
+                   "attention of up to 2048 new tokens, 32 heads on 8"},
         "layerwise_overlap": out["overlap"], "load_then_compute": out["serial"],
         "overlap_speedup": round(out["serial"]["total_s"] / out["overlap"]["total_s"], 3),
         "engine": {k: m[k] for k in ("cache_block_evictions", "cache_block_hits", "cache_block_misses",
@@ -1356,6 +1392,9 @@ def main() -> int:
     ap.add_argument("--fp8-requests", type=int, default=64)
     ap.add_argument("--fp8-pool-gb", type=int, default=30)
     ap.add_argument("--fp8-compute-ms", type=float, default=0.5)
+    ap.add_argument("--fp8-compute", choices=["sleep", "attention"], default="sleep",
+                    help="llama8b_fp8_evict: a layer's compute is a wait of --fp8-compute-ms, or the request's new "
+                         "tokens written into the cache and attending over it")
     ap.add_argument("--pd-requests", type=int, default=200)
     ap.add_argument("--pd-bounce-requests", type=int, default=20)
     ap.add_argument("--order", choices=["shuffled", "sorted"], default="shuffled")
