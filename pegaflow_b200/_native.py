@@ -369,9 +369,8 @@ _SIGNATURES = {
         [c_int32, POINTER(KvCache), c_void_p, c_int64, c_uint32, c_uint32, c_void_p, c_uint64, c_int64, c_int64, c_uint64,
          c_int64, c_int64, c_uint32, c_uint64, c_void_p, c_void_p],
     ),
-    # The KvAttention, or its bytes (packing them takes a third of a Structure's time).
-    "pf_kv_attention_workspace": (c_int, [c_int32, POINTER(KvCache), c_void_p, POINTER(c_uint64)]),
-    "pf_kv_attention_run": (c_int, [c_int32, POINTER(KvCache), c_void_p, c_void_p]),
+    "pf_kv_attention_workspace": (c_int, [c_int32, POINTER(KvCache), POINTER(KvAttention), POINTER(c_uint64)]),
+    "pf_kv_attention_run": (c_int, [c_int32, POINTER(KvCache), POINTER(KvAttention), c_void_p]),
 }
 
 SYMBOLS = tuple(_SIGNATURES)

@@ -2,6 +2,8 @@
 
 Every translation unit is compiled by nvcc for sm_100a only; the shared
 library lands next to this file so it travels with the source tree.
+The binding of the paged-cache operators for torch tensors (_kv_torch.so) is
+compiled with the host compiler against the installed torch and this library.
 Run: python -m pegaflow_b200.build [--force]
 """
 
@@ -20,6 +22,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libpegaflow_b200.so"
+TORCH_BINDING = PKG / "_kv_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = [
@@ -55,8 +58,22 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _torch_command(src: Path, target: Path) -> list[str]:
+    import sysconfig
+    from importlib.util import find_spec
+
+    torch = Path(find_spec("torch").origin).parent  # found, not imported: the build needs its headers alone
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+                cuda / "include", ROOT / "include"]
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *(f"-I{i}" for i in includes),
+            str(src), "-o", str(target), f"-L{PKG}", "-lpegaflow_b200", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
+            "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile and link the library if any source or header changed."""
+    """Compile and link the library and the torch binding if any source or
+    header changed."""
     BUILD.mkdir(exist_ok=True)
     cc = nvcc()
     headers = _headers()
@@ -85,6 +102,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         cmd = [cc, *ARCH, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static", "-lrt", "-lpthread"]
         run(cmd)
         os.replace(tmp, LIB)
+    binding = CSRC / "torch" / "kv_binding.cpp"
+    if force or _stale(TORCH_BINDING, [binding, ROOT / "include" / "pegaflow.h", Path(__file__)]):
+        tmp = TORCH_BINDING.with_suffix(".so.tmp")
+        run(_torch_command(binding, tmp))
+        os.replace(tmp, TORCH_BINDING)
     return LIB
 
 

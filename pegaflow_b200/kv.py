@@ -23,27 +23,25 @@ as soon as their stream is behind it; the same tensors are registered with
 
 from __future__ import annotations
 
-import math
-import struct
-from ctypes import byref, c_uint64
+from ctypes import addressof
 from typing import Optional
 
 import torch
 
-from . import _native as N
+from . import _native as N  # loads the library that the binding is linked to
+
+try:
+    from . import _kv_torch as _ops
+except ImportError as e:
+    raise ImportError(f"{e}: build the torch binding with `python -m pegaflow_b200.build`") from e
 
 BAD_BLOCK = N.PF_KV_BAD_BLOCK
 BAD_LENGTH = N.PF_KV_BAD_LENGTH
 TIMED_OUT = N.PF_KV_TIMED_OUT
 
-_ROWS = {torch.bfloat16: N.PF_DTYPE_BF16, torch.float16: N.PF_DTYPE_FP16, torch.float32: N.PF_DTYPE_FP32}
 _CACHE = {torch.bfloat16: N.PF_DTYPE_BF16, torch.float16: N.PF_DTYPE_FP16, torch.float8_e4m3fn: N.PF_DTYPE_E4M3,
           torch.uint8: N.PF_DTYPE_E4M3, torch.int8: N.PF_DTYPE_INT8}
 _QUANTISED = (N.PF_DTYPE_E4M3, N.PF_DTYPE_INT8)
-_pack_attention = struct.Struct("=QqqQqqQQqQQQQQQIIIIIIfIII").pack  # N.KvAttention, field by field
-# The handle of torch's current stream of a device.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _need(ok: bool, message: str) -> None:
@@ -61,8 +59,7 @@ class KVCache:
     token and head, or shared (``[num_blocks, 1, 1]``: one for each block).
     """
 
-    __slots__ = ("key", "value", "key_scale", "value_scale", "device", "dtype", "_c", "_ref", "_index",
-                 "_heads", "_dim", "_quantised", "_scratch")
+    __slots__ = ("key", "value", "key_scale", "value_scale", "device", "dtype", "_c", "_at", "_index")
 
     def __init__(self, key: torch.Tensor, value: torch.Tensor, key_scale: Optional[torch.Tensor] = None,
                  value_scale: Optional[torch.Tensor] = None):
@@ -100,9 +97,7 @@ class KVCache:
 
         self._c = N.KvCache(side(key, scales[0]), side(value, scales[1]), key.shape[0], key.shape[1], key.shape[2],
                             key.shape[3], code)
-        self._ref = byref(self._c)
-        self._heads, self._dim, self._quantised = key.shape[2], key.shape[3], code in _QUANTISED
-        self._scratch = {}  # sizes of an attention call -> bytes of its workspace
+        self._at = addressof(self._c)
 
     @staticmethod
     def from_tensor(t: torch.Tensor, scale: Optional[torch.Tensor] = None) -> "KVCache":
@@ -155,41 +150,6 @@ class KVCache:
     def head_dim(self) -> int:
         return self._c.head_dim
 
-    def _stream(self, stream: Optional[int]) -> int:
-        if self._index < 0:
-            raise ValueError("the cache must be on a CUDA device")
-        return _raw_stream(self._index) if stream is None else stream
-
-    def _new(self, shape: tuple, dtype: torch.dtype, stream: Optional[int]) -> torch.Tensor:
-        """A new tensor that belongs to the stream that fills it."""
-        if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
-            return torch.empty(shape, dtype=dtype, device=self.device)
-
-    def _ints(self, t: torch.Tensor, dtype: torch.dtype, dim: int, what: str) -> torch.Size:
-        """The shape of a tensor of indices, lengths or offsets."""
-        shape = t.shape
-        if (t.dtype is not dtype or len(shape) != dim or t.get_device() != self._index
-                or (shape[-1] > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"{what} must be {dtype} with {dim} axes, the last contiguous, on {self.device}")
-        return shape
-
-    def _status(self, status: Optional[torch.Tensor]) -> int:
-        if status is None:
-            return 0
-        if status.dtype != torch.int32 or status.numel() != 1 or status.get_device() != self._index:
-            raise ValueError(f"status must be one int32 on {self.device}")
-        return status.data_ptr()
-
-    def _rows(self, t: torch.Tensor, n: int, heads: int, what: str) -> tuple:
-        """Address and strides of dense rows."""
-        s = t.stride()
-        if t.shape != (n, heads, self._dim) or t.get_device() != self._index or (s[2] != 1 and self._dim > 1):
-            raise ValueError(f"{what} must be [{n}, {heads}, {self._dim}] with a contiguous last axis on "
-                             f"{self.device}, not {tuple(t.shape)} with strides {s} on {t.device}")
-        return t.data_ptr(), s[0], s[1]
-
 
 def kv_write(cache: KVCache, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, *,
              given_scales: bool = False, status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
@@ -202,19 +162,7 @@ def kv_write(cache: KVCache, key: torch.Tensor, value: torch.Tensor, slots: torc
     2^-126, and codes = x / scale rounded to nearest; a row that holds a NaN or an
     infinity reads back as NaN. With ``given_scales`` the scales stay as they are
     (calibrated, or shared by a block), and values beyond them saturate."""
-    n = key.shape[0]
-    dtype = _ROWS.get(key.dtype)
-    if dtype is None or value.dtype is not key.dtype:
-        raise ValueError(f"key and value must both be bfloat16, float16 or float32, not {key.dtype} and {value.dtype}")
-    heads = cache._heads
-    k, kt, kh = cache._rows(key, n, heads, "key")
-    v, vt, vh = cache._rows(value, n, heads, "value")
-    if cache._ints(slots, torch.int64, 1, "slots")[0] != n:
-        raise ValueError(f"{slots.shape[0]} slots for {n} tokens")
-    rc = N.lib.pf_kv_write(cache._index, cache._ref, k, kt, kh, v, vt, vh, dtype, slots.data_ptr(), n,
-                           1 if given_scales else 0, cache._status(status), cache._stream(stream))
-    if rc:
-        N.check(rc)
+    _ops.write(cache._at, cache._index, key, value, slots, given_scales, status, stream)
 
 
 def kv_read(cache: KVCache, block_table: torch.Tensor, starts: torch.Tensor, total: Optional[int] = None, *,
@@ -229,37 +177,7 @@ def kv_read(cache: KVCache, block_table: torch.Tensor, starts: torch.Tensor, tot
     default the cache's, bf16 for 8-bit codes) size new outputs; ``out`` gives
     them instead, and rows outside the sequences are left as they are. A token
     on a bad block reads as zeros."""
-    seqs, blocks = cache._ints(block_table, torch.int32, 2, "block_table")
-    if cache._ints(starts, torch.int32, 1, "starts")[0] != seqs + 1:
-        raise ValueError(f"{starts.shape[0]} starts for {seqs} sequences: one more is needed")
-    raw = cache._stream(stream)
-    heads = cache._heads
-    if out is None:
-        if total is None or total < 0:
-            raise ValueError("total, the rows of the result, must be given without out")
-        if dtype is None:
-            dtype = torch.bfloat16 if cache._quantised else cache.dtype
-        code = _ROWS.get(dtype)
-        if code is None:
-            raise ValueError(f"dtype must be bfloat16, float16 or float32, not {dtype}")
-        both = cache._new((2, total, heads, cache._dim), dtype, stream)
-        key, value = both.unbind(0)
-        n, t, h = total, heads * cache._dim, cache._dim
-        k = (both.data_ptr(), t, h)
-        v = (k[0] + n * t * both.element_size(), t, h)
-    else:
-        key, value = out
-        n, code = key.shape[0], _ROWS.get(key.dtype)
-        if code is None or value.dtype is not key.dtype:
-            raise ValueError(f"outputs must both be bfloat16, float16 or float32, not {key.dtype} and {value.dtype}")
-        if (total is not None and total != n) or (dtype is not None and dtype is not key.dtype):
-            raise ValueError("total or dtype and out differ")
-        k, v = cache._rows(key, n, heads, "key"), cache._rows(value, n, heads, "value")
-    rc = N.lib.pf_kv_read(cache._index, cache._ref, block_table.data_ptr(), block_table.stride(0), blocks, seqs,
-                          starts.data_ptr(), *k, *v, code, n, cache._status(status), raw)
-    if rc:
-        N.check(rc)
-    return key, value
+    return _ops.read(cache._at, cache._index, block_table, starts, total, dtype, out, status, stream)
 
 
 def chunk_attention(query: torch.Tensor, cache: KVCache, block_table: torch.Tensor, q_start: torch.Tensor,
@@ -285,53 +203,5 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, block_table: torch.Tens
     ``[n_tokens, q_heads]``, with which outputs over parts of a sequence can be
     joined. A query that sees nothing gets zeros and -inf; rows outside the
     sequences are left as they are."""
-    code = _ROWS.get(query.dtype)
-    shape = query.shape
-    if len(shape) != 3 or code is None:
-        raise ValueError(f"query must be bfloat16 or float16 [n_tokens, q_heads, head_dim], not {query.dtype} "
-                         f"{tuple(shape)}")
-    n, heads, dim = shape
-    q, qt, qh = cache._rows(query, n, heads, "query")
-    seqs, blocks = cache._ints(block_table, torch.int32, 2, "block_table")
-    if (cache._ints(q_start, torch.int32, 1, "q_start")[0] != seqs + 1
-            or cache._ints(kv_len, torch.int32, 1, "kv_len")[0] != seqs):
-        raise ValueError(f"{q_start.shape[0]} q_start and {kv_len.shape[0]} kv_len for {seqs} sequences")
-    max_q, max_kv = max_q or 0, max_kv or 0
-    if window < 0 or max_q < 0 or max_kv < 0:
-        raise ValueError("window, max_q and max_kv cannot be negative")
-    raw = cache._stream(stream)
-    if out is None:
-        out = cache._new(shape, query.dtype, stream)
-        o, ot, oh = out.data_ptr(), heads * dim, dim
-    else:
-        if out.dtype is not query.dtype:
-            raise ValueError(f"out must be {query.dtype}, not {out.dtype}")
-        o, ot, oh = cache._rows(out, n, heads, "out")
-    lse = cache._new((n, heads), torch.float32, stream) if return_lse else None
-    if scale is None:
-        scale = 1.0 / math.sqrt(dim)
-    sizes = (n, seqs, blocks, heads, code, max_q, max_kv, window)
-    need = cache._scratch.get(sizes)
-    if need is None:
-        need = _workspace(cache, sizes, scale)
-    scratch = cache._new((need,), torch.uint8, stream) if need else None
-    args = _pack_attention(q, qt, qh, o, ot, oh, lse.data_ptr() if return_lse else 0, block_table.data_ptr(),
-                           block_table.stride(0), q_start.data_ptr(), kv_len.data_ptr(), cache._status(status),
-                           scratch.data_ptr() if need else 0, need, n, seqs, blocks, heads, code, max_q, max_kv, scale,
-                           1 if causal else 0, window, 0)
-    rc = N.lib.pf_kv_attention_run(cache._index, cache._ref, args, raw)
-    if rc:
-        N.check(rc)
-    return (out, lse) if return_lse else out
-
-
-def _workspace(cache: KVCache, sizes: tuple, scale: float) -> int:
-    n, seqs, blocks, heads, code, max_q, max_kv, window = sizes
-    args = _pack_attention(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, n, seqs, blocks, heads, code, max_q, max_kv, scale, 1,
-                           window, 0)
-    need = c_uint64()
-    N.check(N.lib.pf_kv_attention_workspace(cache._index, cache._ref, args, byref(need)))
-    if len(cache._scratch) >= 1024:  # a server's sizes change with every step
-        cache._scratch.clear()
-    cache._scratch[sizes] = need.value
-    return need.value
+    return _ops.attend(cache._at, cache._index, query, block_table, q_start, kv_len, scale, causal, window, max_q, max_kv,
+                       out, return_lse, status, stream)
