@@ -128,7 +128,7 @@ int pf_kv_read(int32_t device_id, const pf_kv_cache* cache, const int32_t* block
     check_rows(v, dtype, "value");
     if ((!block_table && max_blocks) || !starts) refuse("no block table or starts");
     DeviceGuard g(device_id);
-    const KvReadArgs args{*cache, k, v, block_table, starts, status, table_stride, n_rows, max_blocks, n_seqs, dtype};
+    const KvReadArgs args{*cache, k, v, block_table, starts, status, table_stride, n_rows, max_blocks, n_seqs, dtype, uint32_t(num_sms(device_id))};
     cuda_check(launch_kv_read(args, static_cast<cudaStream_t>(stream)), "kv_read launch");
   });
 }

@@ -53,6 +53,7 @@ struct KvReadArgs {
   uint32_t max_blocks;
   uint32_t n_seqs;
   uint32_t dtype;
+  uint32_t num_sms;
 };
 
 struct KvAttendArgs {

@@ -30,9 +30,10 @@ __device__ __forceinline__ float row_scale(float top) {
   return s < kKvSmallestScale ? kKvSmallestScale : s == INFINITY ? NAN : s;
 }
 
-// Values of a row that a lane holds.
-template <uint32_t STORE>
-constexpr int kReadElems = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8 ? 16 : 8;
+// Values of a row that a thread moves when reading: 16 bytes of a 16-bit result, so
+// that a warp's stores fill whole sectors (with 16 codes and two stores 32 bytes
+// apart, 10,240 tokens of 8 x 128 took 15.1 us instead of 12.1).
+constexpr int kReadElems = 8;
 constexpr uint32_t kReadMaxTokens = 64;  // of a block
 
 // Strides in bytes that fit 32 bits, so that a step of an address is one
@@ -61,7 +62,7 @@ struct WritePlan {
 
 struct ReadPlan {
   uint32_t tokens;       // of a block
-  uint32_t pieces;       // 16-byte pieces of a token's rows of one side
+  uint32_t pieces;       // of kReadElems values, of a token's rows of one side
   uint32_t row_pieces;   // of one row
   RowStrides strides;
   float pieces_inverse;
@@ -359,14 +360,16 @@ __global__ void __launch_bounds__(kThreads, kWriteBlocks<IN>) kv_write_rows_kern
 
 // ------------------------------------------------------- aligned rows: reading
 
-// A thread's piece: 16 codes, or 8 values of 16 bits. In: one 16-byte word; out: two or four.
+// A thread's piece: 8 codes, or 8 values of 16 bits.
+template <uint32_t STORE>
+using PieceRaw = KvPack<uint32_t, STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8 ? 2 : 4>;
 template <uint32_t STORE, uint32_t OUT>
-__device__ __forceinline__ void store_piece(typename KvElem<OUT>::type* to, const uint4& raw, float s) {
-  constexpr int E = kReadElems<STORE>;
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ void store_piece(typename KvElem<OUT>::type* to, const PieceRaw<STORE>& raw, float s) {
+  constexpr int E = kReadElems;
+  const auto& w = raw.v;
   float2 x[E / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < int(sizeof(w) / 4); ++i) {
     if constexpr (STORE == PF_DTYPE_E4M3) {
       uint32_t lo, hi;
       asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(uint16_t(w[i])));
@@ -416,7 +419,7 @@ __device__ __forceinline__ void store_piece(typename KvElem<OUT>::type* to, cons
 // looked up once each, by one thread, then the threads go over the rows' pieces.
 template <uint32_t STORE, uint32_t OUT>
 __global__ void __launch_bounds__(kThreads) kv_read_rows_kernel(const __grid_constant__ KvReadArgs a, const ReadPlan plan) {
-  constexpr int E = kReadElems<STORE>;
+  constexpr int E = kReadElems;
   constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
   using T = typename KvElem<STORE>::type;
   using O = typename KvElem<OUT>::type;
@@ -453,11 +456,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_rows_kernel(const __grid_con
     const int2 p = place[in];
     if (p.x == -2) continue;
     const uint32_t b = uint32_t(max(p.x, 0)), offset = uint32_t(p.y);
-    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    PieceRaw<STORE> k{}, v{};
     float ks = 0.0f, vs = 0.0f;
     if (p.x >= 0) {
-      k = *reinterpret_cast<const uint4*>(address<const T>(a.cache.key.data, plan.strides.key, b, offset, head) + d);
-      v = *reinterpret_cast<const uint4*>(address<const T>(a.cache.value.data, plan.strides.value, b, offset, head) + d);
+      k = *reinterpret_cast<const PieceRaw<STORE>*>(address<const T>(a.cache.key.data, plan.strides.key, b, offset, head) + d);
+      v = *reinterpret_cast<const PieceRaw<STORE>*>(address<const T>(a.cache.value.data, plan.strides.value, b, offset, head) + d);
       if constexpr (kQuant) {
         ks = *address<const float>(a.cache.key.scale, plan.strides.key_scale, b, offset, head);
         vs = *address<const float>(a.cache.value.scale, plan.strides.value_scale, b, offset, head);
@@ -538,14 +541,18 @@ void write_from(const KvWriteArgs& a, cudaStream_t stream) {
 
 template <uint32_t STORE, uint32_t OUT>
 void read_as(const KvReadArgs& a, cudaStream_t stream) {
-  constexpr int E = kReadElems<STORE>;
+  constexpr int E = kReadElems;
   const uint32_t heads = a.cache.heads;
   RowStrides strides;
   if (side_packs(a.cache, a.cache.key, E) && side_packs(a.cache, a.cache.value, E) && rows_pack(a.key, OUT, E) &&
       rows_pack(a.value, OUT, E) && fit_all(a.cache, a.key, a.value, OUT, &strides)) {
     const uint32_t row = a.cache.head_dim / E, pieces = heads * row;
-    // Two pieces for each thread; more tokens than kReadMaxTokens only where a token has few pieces.
-    const uint32_t tokens = std::min(kReadMaxTokens, std::max(1u, 2 * kThreads / pieces));
+    // Two pieces for each thread, up to eight as long as an SM gets a dozen blocks: fewer blocks look rows up and wait
+    // less (46,000 rows of 5 heads of 80: 23.2 us with two, 20.0 with eight; 2,048 rows of 12 of 64 with a write
+    // before: 7.8 us with two, 10.7 with eight).
+    const uint64_t each = a.n_rows * pieces / (uint64_t(kThreads) * 12 * a.num_sms);
+    const uint32_t turns = static_cast<uint32_t>(std::min<uint64_t>(8, std::max<uint64_t>(2, each)));
+    const uint32_t tokens = std::min(kReadMaxTokens, std::max(1u, turns * kThreads / pieces));
     const ReadPlan plan{tokens, pieces, row, strides, 1.0f / float(pieces), 1.0f / float(row), page_shift(a.cache)};
     kv_read_rows_kernel<STORE, OUT><<<static_cast<uint32_t>((a.n_rows + tokens - 1) / tokens), kThreads, 0, stream>>>(a, plan);
   } else {
