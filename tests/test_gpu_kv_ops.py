@@ -360,6 +360,53 @@ def test_attention_layouts(cuda, pattern, store, layout):
     check_attention(torch, got, 128, max(lens), store in QMAX)
 
 
+@pytest.mark.parametrize("store", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [2, 8, 32, 64, 256, 384, 100])
+@pytest.mark.parametrize("dim", [16, 48, 80, 112, 128])
+def test_attention_block_sizes(cuda, dim, page, store):
+    """Blocks that are part of a tile of keys, a whole number of them or neither, heads of every width."""
+    torch = cuda
+    counts, lens = [70, 1, 33], [900, 300, 33]
+    got = run_attention(torch, "bf16", store, dim, 2, 4, page, counts, lens, seed=dim + page)
+    check_attention(torch, got, dim, max(lens), store in QMAX)
+
+
+@pytest.mark.parametrize("heads, group", [(1, 128), (1, 40), (3, 17), (12, 1)])
+@pytest.mark.parametrize("pattern", ["decode", "verify", "mixed"])
+@pytest.mark.parametrize("store", ["fp16", "int8"])
+def test_attention_groups(cuda, pattern, heads, group, store):
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+    got = run_attention(torch, "fp16", store, 64, heads, group, 16, counts, lens, seed=group)
+    check_attention(torch, got, 64, max(lens), store in QMAX)
+
+
+@pytest.mark.parametrize("n_q", [1, 20])
+def test_attention_many_sequences(cuda, n_q):
+    """More sequences than some of a grid's axes have room for; each its own block."""
+    torch = cuda
+    from pegaflow_b200 import chunk_attention
+
+    n, page, dim = 70_000 if n_q == 1 else 5_000, 32, 64
+    cache, k, v, ks, vs = make_cache(torch, "bf16", n, page, 1, dim, fill=4)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn((n * n_q, 1, dim), generator=g, device="cuda").bfloat16()
+    lens = torch.randint(n_q, page + 1, (n,), generator=g, device="cuda", dtype=torch.int32)
+    order = torch.randperm(n, generator=g, device="cuda").to(torch.int32).view(n, 1)
+    starts = torch.arange(n + 1, device="cuda", dtype=torch.int32) * n_q
+    o = chunk_attention(q, cache, order, starts, lens, max_q=n_q, max_kv=page)
+    keys, values = k[order[:, 0].long(), :, 0].double(), v[order[:, 0].long(), :, 0].double()
+    qq = q.view(n, n_q, dim).double()
+    s = torch.einsum("nid,njd->nij", qq, keys) / math.sqrt(dim)
+    pos = lens[:, None] - n_q + torch.arange(n_q, device="cuda")
+    seen = torch.arange(page, device="cuda") <= pos[:, :, None]
+    w = torch.where(seen, s, -math.inf).softmax(2)
+    want, mag = torch.einsum("nij,njd->nid", w, values), torch.einsum("nij,njd->nid", w, values.abs())
+    dot = torch.einsum("nid,njd->nij", qq.abs(), keys.abs()).amax(2) / math.sqrt(dim)
+    tol, _ = attend_bound(torch, o.dtype, False, want, mag, dot, page, dim)
+    assert ((o.view(n, n_q, dim).double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("window", [1, 2, 100, 129, 5000])
 @pytest.mark.parametrize("pattern", ["decode_long", "verify", "mixed", "prefill", "short"])
 @pytest.mark.parametrize("store", ["fp16", "int8"])

@@ -189,6 +189,7 @@ def test_library_refuses_given_scales_of_16_bits(native):
     (lambda N: c_cache(N, N.PF_DTYPE_BF16, address=4104), {}, "aligned to 16 bytes"),
     (lambda N: c_cache(N, N.PF_DTYPE_BF16), {"q_start": 0}, "no q_start"),
     (lambda N: c_cache(N, N.PF_DTYPE_BF16), {"max_blocks": 1 << 28}, "block table"),
+    (lambda N: c_cache(N, N.PF_DTYPE_BF16), {"n_tokens": 1 << 29}, "too many query tokens"),
 ])
 def test_library_refuses_attention(native, make, change, words):
     from ctypes import byref
