@@ -170,70 +170,6 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     const int32_t hi = min(end, lo + per);
     if (part && lo >= end) continue;
 
-    // This lane's query rows: g of each tile (as an operand), 2 t and 2 t + 1 (as results).
-    uint32_t q[NT][S::kTiles][2];
-    float f[NT][2];
-    int32_t row_lo[NT][2], row_hi[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int32_t r = row0 + n * 8 + g;
-      const bool on = r < rows;
-      const int32_t i = on ? r / group : 0;
-      const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(s.first + i) * k.a.query.token_stride +
-                   int64_t(int32_t(head) * group + (on ? r - i * group : 0)) * k.a.query.head_stride;
-      uint32_t raw[S::kTiles * 2];
-#pragma unroll
-      for (int j = 0; j < S::kKeyReads; ++j) {
-        const int d = (t + 4 * j) * S::kChunk;
-#pragma unroll
-        for (int h = 0; h < S::kChunk / 8; ++h) {
-          const uint4 v = on && d < int(c.head_dim) ? *reinterpret_cast<const uint4*>(p + d + h * 8) : make_uint4(0, 0, 0, 0);
-          const int at = j * (S::kChunk / 2) + h * 4;
-          raw[at] = v.x, raw[at + 1] = v.y, raw[at + 2] = v.z, raw[at + 3] = v.w;
-        }
-      }
-      float unit = 1.0f;
-      if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
-        // The row's largest exponent, over its four lanes.
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < S::kTiles * 2; ++j) top = max(top, max(raw[j] & 0x7fffu, (raw[j] >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^(14 - e) brings it to [2^14, 2^15); both powers are kept within fp32's normal range.
-        const int e = min(max(int(top >> 7) - 127, -100), 127);
-        const float bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
-        unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
-#pragma unroll
-        for (int j = 0; j < S::kTiles * 2; ++j) {
-          raw[j] = pack2<false>(__uint_as_float(raw[j] << 16) * bring, __uint_as_float(raw[j] & 0xffff0000u) * bring);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < S::kTiles; ++j) q[n][j][0] = raw[2 * j], q[n][j][1] = raw[2 * j + 1];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        // Row 2 t + e of the tile has its unit in lane (2 t + e) * 4.
-        f[n][e] = k.a.scale * kLog2e * __shfl_sync(0xffffffffu, unit, (2 * t + e) * 4);
-        const int32_t rr = row0 + n * 8 + 2 * t + e;
-        row_lo[n][e] = rr < rows ? kv_row_begin(k, s, rr / group) : 0;
-        row_hi[n][e] = rr < rows ? kv_row_end(k, s, rr / group) : INT32_MAX;  // a row that is none: nothing is kept of it
-      }
-    }
-    // Tokens that every row of the tile sees.
-    const int32_t all_lo = kv_row_begin(k, s, row_last / group), all_hi = kv_row_end(k, s, row0 / group);
-
-    float o[NT][S::kTiles][4];
-    float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < S::kTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.0f;
-    }
-    uint32_t v_exp = 1;  // exponent field of the power of two that the weights are divided by
-
     const char* key_base = reinterpret_cast<const char*>(c.key.data);
     const char* value_base = reinterpret_cast<const char*>(c.value.data);
 
@@ -302,6 +238,70 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       stage_addresses(warp + kWarps);
       stage_blocks(warp + 2 * kWarps);
     }
+    // This lane's query rows: g of each tile (as an operand), 2 t and 2 t + 1 (as results).
+    uint32_t q[NT][S::kTiles][2];
+    float f[NT][2];
+    int32_t row_lo[NT][2], row_hi[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int32_t r = row0 + n * 8 + g;
+      const bool on = r < rows;
+      const int32_t i = on ? r / group : 0;
+      const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(s.first + i) * k.a.query.token_stride +
+                   int64_t(int32_t(head) * group + (on ? r - i * group : 0)) * k.a.query.head_stride;
+      uint32_t raw[S::kTiles * 2];
+#pragma unroll
+      for (int j = 0; j < S::kKeyReads; ++j) {
+        const int d = (t + 4 * j) * S::kChunk;
+#pragma unroll
+        for (int h = 0; h < S::kChunk / 8; ++h) {
+          const uint4 v = on && d < int(c.head_dim) ? *reinterpret_cast<const uint4*>(p + d + h * 8) : make_uint4(0, 0, 0, 0);
+          const int at = j * (S::kChunk / 2) + h * 4;
+          raw[at] = v.x, raw[at + 1] = v.y, raw[at + 2] = v.z, raw[at + 3] = v.w;
+        }
+      }
+      float unit = 1.0f;
+      if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+        // The row's largest exponent, over its four lanes.
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < S::kTiles * 2; ++j) top = max(top, max(raw[j] & 0x7fffu, (raw[j] >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(14 - e) brings it to [2^14, 2^15); both powers are kept within fp32's normal range.
+        const int e = min(max(int(top >> 7) - 127, -100), 127);
+        const float bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+        unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+#pragma unroll
+        for (int j = 0; j < S::kTiles * 2; ++j) {
+          raw[j] = pack2<false>(__uint_as_float(raw[j] << 16) * bring, __uint_as_float(raw[j] & 0xffff0000u) * bring);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < S::kTiles; ++j) q[n][j][0] = raw[2 * j], q[n][j][1] = raw[2 * j + 1];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // Row 2 t + e of the tile has its unit in lane (2 t + e) * 4.
+        f[n][e] = k.a.scale * kLog2e * __shfl_sync(0xffffffffu, unit, (2 * t + e) * 4);
+        const int32_t rr = row0 + n * 8 + 2 * t + e;
+        row_lo[n][e] = rr < rows ? kv_row_begin(k, s, rr / group) : 0;
+        row_hi[n][e] = rr < rows ? kv_row_end(k, s, rr / group) : INT32_MAX;  // a row that is none: nothing is kept of it
+      }
+    }
+    // Tokens that every row of the tile sees.
+    const int32_t all_lo = kv_row_begin(k, s, row_last / group), all_hi = kv_row_end(k, s, row0 / group);
+
+    float o[NT][S::kTiles][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < S::kTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+    }
+    uint32_t v_exp = 1;  // exponent field of the power of two that the weights are divided by
+
 #pragma unroll 1
     for (int32_t i = 0; i < 2 * mine; ++i) {
       const int32_t batch = warp + (i >> 1) * kWarps, j0 = lo + batch * kBatch + (i & 1) * kStep;
@@ -692,7 +692,7 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   if (k.a.window) longest = std::min<uint64_t>(longest, uint64_t(k.a.window) + most_queries(k));
   longest = std::max<uint64_t>(longest, 1);
   // Parts of equal length: the CTAs run in rounds of as many as fit, each round as long as a part and its start and
-  // end (queries, addresses, joining: about 128 tokens' time). Few sequences: one round, whose parts are as short as
+  // end (queries, addresses, joining: about 384 tokens' time). Few sequences: one round, whose parts are as short as
   // that leaves them. Many: sequences are rarely equally long, so among splits that are within a tenth of the best
   // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 315 us in one round, 228 in seven).
   const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * p.tiles * k.cache.heads);
@@ -700,7 +700,7 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   const uint64_t units = (longest + kStreamMinPart - 1) / kStreamMinPart;  // shortest parts
   auto cost = [&](uint64_t per) {
     const uint64_t parts = (units + per - 1) / per;
-    return (items * parts + slots - 1) / slots * (per + 1);
+    return (items * parts + slots - 1) / slots * (per + 3);
   };
   uint64_t best = UINT64_MAX;
   const uint64_t least = (units + kStreamMaxParts - 1) / kStreamMaxParts;
