@@ -279,6 +279,53 @@ struct Item {
   int32_t group;
 };
 
+// Units of a row tile of a sequence.
+__device__ __forceinline__ int32_t units_of(const KvAttendArgs& k, const KvSeq& s, int32_t group, int32_t tile) {
+  const int32_t last = min(s.n * group, (tile + 1) * kTileRows) - 1;
+  return tile_units(kv_row_begin(k, s, tile * kTileRows / group) & -kTileKeys, kv_row_end(k, s, last / group));
+}
+
+// Where the span of CTA `cta` begins; a warp finds it together.
+__device__ __forceinline__ KvSpan find_span(const KvAttendArgs& k, const KvTilePlan& p, int64_t cta, int64_t* span) {
+  const int lane = threadIdx.x & 31;
+  const int32_t n_seqs = int32_t(k.a.n_seqs), heads = int32_t(k.cache.heads), group = int32_t(k.a.q_heads) / heads;
+  const int64_t* costs = reinterpret_cast<const int64_t*>(reinterpret_cast<const char*>(k.a.workspace) + p.costs_at);
+  const int64_t total = costs[n_seqs];
+  *span = span_units(total, p.ctas);
+  const int64_t at = cta * *span;
+  if (at >= total) return KvSpan{n_seqs, 0, 0, 0};
+  int32_t lo = 0, hi = n_seqs;  // the last sequence with costs[lo] <= at
+  while (hi - lo > 1) {
+    // 31 places between them at a time.
+    const int32_t step = (hi - lo + 31) / 32, mid = lo + (lane + 1) * step;
+    const uint32_t past = __ballot_sync(0xffffffffu, mid >= hi || costs[mid] > at);
+    const int first = __ffs(past) - 1;  // lane 31's is at or past hi
+    hi = min(hi, lo + (first + 1) * step);
+    lo += first * step;
+  }
+  const KvSeq s = kv_sequence(k, uint32_t(lo));
+  const int32_t tiles = (s.n * group + kTileRows - 1) / kTileRows;
+  int64_t rest = at - costs[lo];
+  for (int32_t base = 0; base < tiles; base += 32) {
+    const int32_t t = base + lane;
+    const int32_t units = t < tiles ? units_of(k, s, group, t) : 0;
+    int64_t sum = int64_t(units) * heads;
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
+      if (lane >= w) sum += x;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, sum > rest);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      const int32_t u = __shfl_sync(0xffffffffu, units, l);
+      const int64_t in = rest - (__shfl_sync(0xffffffffu, sum, l) - int64_t(u) * heads);
+      return KvSpan{lo, base + l, int32_t(in / u), int32_t(in % u)};
+    }
+    rest -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return KvSpan{n_seqs, 0, 0, 0};
+}
+
 struct Walk {
   const KvAttendArgs& k;
   int32_t seq, tile, head, unit;
@@ -287,10 +334,8 @@ struct Walk {
   bool first;
 
   __device__ Walk(const KvAttendArgs& args, const KvTilePlan& p) : k(args), cta(int32_t(blockIdx.x)), first(true) {
-    const char* ws = reinterpret_cast<const char*>(args.a.workspace);
-    const int4 span = *reinterpret_cast<const int4*>(ws + p.spans_at + blockIdx.x * sizeof(KvSpan));
-    seq = span.x, tile = span.y, head = span.z, unit = span.w;
-    left = span_units(reinterpret_cast<const int64_t*>(ws + p.costs_at)[args.a.n_seqs], p.ctas);
+    const KvSpan span = find_span(args, p, blockIdx.x, &left);
+    seq = span.seq, tile = span.tile, head = span.head, unit = span.unit;
   }
 
   __device__ bool next(Item& it) {
@@ -323,87 +368,39 @@ struct Walk {
   }
 };
 
-// Cost of each sequence, then where each CTA's span begins. One block; a warp for
-// a sequence, its lanes over the row tiles, then a warp for each span.
-__global__ void __launch_bounds__(1024) kv_tile_spans_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan p) {
+// What the sequences in front of each cost, and all of them: one block, a warp for
+// a sequence, its lanes over the row tiles.
+__global__ void __launch_bounds__(1024) kv_tile_costs_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan p) {
   let_next_kernel_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t n_seqs = int32_t(k.a.n_seqs), heads = int32_t(k.cache.heads);
   const int32_t group = int32_t(k.a.q_heads) / heads;
-  char* ws = reinterpret_cast<char*>(k.a.workspace);
-  int64_t* costs = reinterpret_cast<int64_t*>(ws + p.costs_at);
-  int4* spans = reinterpret_cast<int4*>(ws + p.spans_at);
-  __shared__ int64_t part[32];
-  __shared__ int64_t front;
-
-  auto units_of = [&](const KvSeq& s, int32_t tile) {
-    const int32_t last = min(s.n * group, (tile + 1) * kTileRows) - 1;
-    return tile_units(kv_row_begin(k, s, tile * kTileRows / group) & -kTileKeys, kv_row_end(k, s, last / group));
-  };
-  if (threadIdx.x == 0) front = 0;
-  __syncthreads();
+  int64_t* costs = reinterpret_cast<int64_t*>(reinterpret_cast<char*>(k.a.workspace) + p.costs_at);
+  __shared__ int64_t part[2][32];
+  int64_t front = 0;
   for (int32_t base = 0; base < n_seqs; base += 32) {
     const int32_t seq = base + warp;
     int64_t cost = 0;
     if (seq < n_seqs) {
       const KvSeq s = kv_sequence(k, uint32_t(seq));
       const int32_t tiles = (s.n * group + kTileRows - 1) / kTileRows;
-      for (int32_t t = lane; t < tiles; t += 32) cost += units_of(s, t);
+      for (int32_t t = lane; t < tiles; t += 32) cost += units_of(k, s, group, t);
       for (int w = 16; w; w >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, w);
       cost *= heads;
     }
-    if (lane == 0) part[warp] = cost;
+    int64_t* sums = part[base >> 5 & 1];  // the other's readers may still be at it
+    if (lane == 0) sums[warp] = cost;
     __syncthreads();
-    if (warp == 0) {
-      const int64_t mine = part[lane];
-      int64_t sum = mine;
-      for (int w = 1; w < 32; w <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
-        if (lane >= w) sum += x;
-      }
-      const int64_t before = front;
-      if (base + lane < n_seqs) costs[base + lane] = before + sum - mine;
-      __syncwarp();
-      if (lane == 31) front = before + sum;
+    int64_t sum = sums[lane];
+    const int64_t mine = sum;
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
+      if (lane >= w) sum += x;
     }
-    __syncthreads();
+    if (warp == 0 && base + lane < n_seqs) costs[base + lane] = front + sum - mine;
+    front += __shfl_sync(0xffffffffu, sum, 31);
   }
-  const int64_t total = front, span = span_units(total, p.ctas);
-  if (threadIdx.x == 0) costs[n_seqs] = total;
-  __syncthreads();
-  for (uint32_t c = uint32_t(warp); c <= p.ctas; c += 32) {
-    const int64_t at = int64_t(c) * span;
-    int4 out = make_int4(n_seqs, 0, 0, 0);
-    if (at < total) {
-      int32_t lo = 0, hi = n_seqs;  // the last sequence with costs[lo] <= at
-      while (hi - lo > 1) {
-        const int32_t mid = (lo + hi) >> 1;
-        if (costs[mid] <= at) lo = mid; else hi = mid;
-      }
-      const KvSeq s = kv_sequence(k, uint32_t(lo));
-      const int32_t tiles = (s.n * group + kTileRows - 1) / kTileRows;
-      int64_t rest = at - costs[lo];
-      for (int32_t base = 0; base < tiles; base += 32) {
-        const int32_t t = base + lane;
-        const int32_t units = t < tiles ? units_of(s, t) : 0;
-        int64_t sum = int64_t(units) * heads;
-        for (int w = 1; w < 32; w <<= 1) {
-          const int64_t x = __shfl_up_sync(0xffffffffu, sum, w);
-          if (lane >= w) sum += x;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, sum > rest);
-        if (past) {
-          const int l = __ffs(past) - 1;
-          const int32_t u = __shfl_sync(0xffffffffu, units, l);
-          const int64_t in = rest - (__shfl_sync(0xffffffffu, sum, l) - int64_t(u) * heads);
-          out = make_int4(lo, base + l, int32_t(in / u), int32_t(in % u));
-          break;
-        }
-        rest -= __shfl_sync(0xffffffffu, sum, 31);
-      }
-    }
-    if (lane == 0) spans[c] = out;
-  }
+  if (threadIdx.x == 0) costs[n_seqs] = front;
 }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -594,7 +591,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
   tmem_after_sync();
   const uint32_t tmem = 0;
   if (sh.tmem != 0) sh.failed = 1;  // cannot be: the waits would end the call
-  wait_for_previous_kernel();  // the spans
+  wait_for_previous_kernel();  // the costs
   let_next_kernel_start();
 
   Walk walk(k, plan);
@@ -1163,38 +1160,48 @@ __global__ void __launch_bounds__(256) kv_join_tiles_kernel(const __grid_constan
   wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const char* ws = reinterpret_cast<const char*>(k.a.workspace);
-  const int64_t span = span_units(reinterpret_cast<const int64_t*>(ws + plan.costs_at)[k.a.n_seqs], plan.ctas);
   const int64_t cta = blockIdx.x;
-  const int4 next = *reinterpret_cast<const int4*>(ws + plan.spans_at + (cta + 1) * sizeof(KvSpan));
-  if (next.x >= int32_t(k.a.n_seqs) || next.w == 0) return;
-  const int64_t at = (cta + 1) * span - next.w;  // where the item begins
+  int64_t span;
+  const KvSpan next = find_span(k, plan, cta + 1, &span);
+  if (next.seq >= int32_t(k.a.n_seqs) || next.unit == 0) return;
+  const int64_t at = (cta + 1) * span - next.unit;  // where the item begins
   if (at / span != cta) return;
-  const KvSeq s = kv_sequence(k, uint32_t(next.x));
+  const KvSeq s = kv_sequence(k, uint32_t(next.seq));
   const int32_t group = int32_t(k.a.q_heads / k.cache.heads);
-  const int32_t row0 = next.y * kTileRows, rows = min(kTileRows, s.n * group - row0);
+  const int32_t row0 = next.tile * kTileRows, rows = min(kTileRows, s.n * group - row0);
   const KvSplit split =
       item_split(at, tile_units(kv_row_begin(k, s, row0 / group) & -kTileKeys, kv_row_end(k, s, (row0 + rows - 1) / group)), span);
   const float* parts = reinterpret_cast<const float*>(ws + plan.parts_at);
   for (int32_t r = int32_t(blockIdx.y) * 8 + warp; r < rows; r += int32_t(gridDim.y) * 8) {
-    float top = -INFINITY;
-    for (int64_t p = split.first; p <= split.last; ++p) {
-      top = fmaxf(top, parts[(part_slot(at, p, span) * kTileRows + r) * (DP + 4)]);
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    // A lane for a part's maximum and sum, then all lanes for each part's values.
+    float top = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 2
-    for (int64_t p = split.first; p <= split.last; ++p) {
-      const float* w = parts + (part_slot(at, p, span) * kTileRows + r) * (DP + 4);
-      const float keep = exp2f(w[0] - base);
-      sum += w[1] * keep;
-      if (lane * 4 < DP) {
-        const float4 v = *reinterpret_cast<const float4*>(w + 4 + lane * 4);
-        o.x += v.x * keep, o.y += v.y * keep, o.z += v.z * keep, o.w += v.w * keep;
+    for (int64_t p0 = split.first; p0 <= split.last; p0 += 32) {
+      const bool on = p0 + lane <= split.last;
+      const float* mine = parts + (part_slot(at, on ? p0 + lane : p0, span) * kTileRows + r) * (DP + 4);
+      const float m = on ? mine[0] : -INFINITY, l = on ? mine[1] : 0.0f;
+      float now = m;
+      for (int w = 16; w; w >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, w));
+      now = fmaxf(now, top);
+      const float base = now == -INFINITY ? 0.0f : now;
+      const float keep = exp2f(top - base), by = exp2f(m - base);
+      float part_sum = l * by;
+      for (int w = 16; w; w >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, w);
+      sum = sum * keep + part_sum;
+      o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+      top = now;
+      const int count = int(min(int64_t(32), split.last - p0 + 1));
+#pragma unroll 4
+      for (int u = 0; u < count; ++u) {
+        const float weight = __shfl_sync(0xffffffffu, by, u);
+        if (lane * 4 < DP) {
+          const float4 v = *reinterpret_cast<const float4*>(parts + (part_slot(at, p0 + u, span) * kTileRows + r) * (DP + 4) + 4 + lane * 4);
+          o.x += v.x * weight, o.y += v.y * weight, o.z += v.z * weight, o.w += v.w * weight;
+        }
       }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int32_t i = (row0 + r) / group, qh = next.z * group + row0 + r - i * group;
+    const int32_t i = (row0 + r) / group, qh = next.head * group + row0 + r - i * group;
     const int64_t token = int64_t(s.first) + i;
     if (lane * 4 < int(k.cache.head_dim)) {
       KvPack<T, 4> y;
@@ -1268,10 +1275,10 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t s
   if (Tiles<Q, STORE, DP>::kQuant || !box_map(k.cache, k.cache.key, &maps.key) || !box_map(k.cache, k.cache.value, &maps.value)) {
     plan.box_rows = 0;
   }
-  kv_tile_spans_kernel<<<1, 1024, 0, stream>>>(k, p);
+  kv_tile_costs_kernel<<<1, 1024, 0, stream>>>(k, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
   if ((err = launch_early(kernel, dim3(p.ctas), Tiles<Q, STORE, DP>::kThreads, shm, stream, k, plan, maps)) != cudaSuccess) return err;
-  return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 4), 256, 0, stream, k, p);
+  return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 16), 256, 0, stream, k, p);
 }
 
 template <uint32_t Q, uint32_t STORE>
@@ -1302,7 +1309,6 @@ KvTilePlan tile_plan(const KvAttendArgs& k, int num_sms) {
     p.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  p.spans_at = take((uint64_t(p.ctas) + 1) * sizeof(KvSpan));
   p.costs_at = take((uint64_t(k.a.n_seqs) + 1) * sizeof(int64_t));
   const uint64_t dp = k.cache.head_dim <= 64 ? 64 : 128;
   p.parts_at = take(2 * uint64_t(p.ctas) * kTileRows * (dp + 4) * sizeof(float));

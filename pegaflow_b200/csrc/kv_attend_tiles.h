@@ -24,8 +24,7 @@ struct KvTilePlan {
   int32_t page_shift;    // log2 of the block size, -1 if it is no power of two
   uint32_t box_rows;     // tokens of a TMA box, 0: none
   uint32_t reserved;
-  uint64_t spans_at;     // byte offsets in the workspace: KvSpan[ctas + 1]
-  uint64_t costs_at;     // int64[n_seqs + 1], units in front of each sequence
+  uint64_t costs_at;     // byte offsets in the workspace: int64[n_seqs + 1], units in front of each sequence
   uint64_t parts_at;     // float[2 * ctas][kTileRows][dp + 4]
   uint64_t bytes;
 };
