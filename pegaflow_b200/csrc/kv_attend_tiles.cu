@@ -76,6 +76,7 @@ struct Tiles {
     unsigned char kv[kStages][kTileBytes];
     KeyInfo info[kInfos];
     float q_unit[2][kTileRows];  // by the item's parity
+    int64_t q_at[kTileRows];
     uint32_t warp_max[2][kTileKeys / 32];  // by the tile's parity
     uint64_t q_full, q_empty;
     uint64_t kv_full[kStages], kv_empty[kStages];
@@ -729,51 +730,82 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       look_up(it.unit0, block);
       if constexpr (S::kQuant) load_scales(it.unit0);
 
-      // Q: a thread for a row at a time, of both tiles.
+      // Q: the rows' places first, a thread for each; then 16-byte pieces, neighbouring threads on one row.
       ok = loaders_agree<kLoadThreads>(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
       if (!ok) break;
-#pragma unroll 1
       for (int r = tid; r < kTileRows; r += kLoadThreads) {
-        if (r >= 128 && it.rows <= 128) break;
-        const bool on = r < it.rows;
-        const int32_t row = it.row0 + (on ? r : 0), i = row / it.group;
-        const T* p = reinterpret_cast<const T*>(k.a.query.data) + int64_t(it.s.first + i) * k.a.query.token_stride +
-                     int64_t(it.head * it.group + row - i * it.group) * k.a.query.head_stride;
-        uint4 v[DP / 8];
+        const int32_t row = it.row0 + r, i = row / it.group;
+        sh.q_at[r] = r < it.rows ? (int64_t(it.s.first + i) * k.a.query.token_stride +
+                                    int64_t(it.head * it.group + row - i * it.group) * k.a.query.head_stride) * 2 : -1;
+      }
+      loaders_agree<kLoadThreads>(true);
+      {
+        constexpr int kPieces = DP / 8, kRows = kLoadThreads / kPieces, kAhead = 8;
+        const int piece = tid % kPieces;
+        const bool there = piece * 8 < int(c.head_dim);
+        const char* from = reinterpret_cast<const char*>(k.a.query.data) + piece * 16;
+        const int q_rows = it.rows <= 128 ? 128 : kTileRows;
+        if (!S::kQuant && k.a.scale >= 0.0f) {
+          // As they are: asynchronous copies, whose arrival counts for the barrier.
+          for (int r0 = tid / kPieces; r0 < q_rows; r0 += kRows * kAhead) {
 #pragma unroll
-        for (int piece = 0; piece < DP / 8; ++piece) {
-          v[piece] = make_uint4(0, 0, 0, 0);
-          if (on && piece * 8 < int(c.head_dim)) v[piece] = *reinterpret_cast<const uint4*>(p + piece * 8);
-        }
-        const uint32_t flip = k.a.scale < 0.0f ? 0x80008000u : 0u;
-        float bring = 1.0f, unit = 1.0f;
-        if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int piece = 0; piece < DP / 8; ++piece) {
-            for (uint32_t x : {v[piece].x, v[piece].y, v[piece].z, v[piece].w}) top = max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu));
+            for (int i = 0; i < kAhead; ++i) {
+              const int r = r0 + i * kRows;
+              if (r < q_rows) {
+                const int64_t off = sh.q_at[r];
+                const bool on = there && off >= 0;
+                const uint32_t to = smem_u32(sh.q[r >> 7]) + (piece >> 3) * 16384 + (r & 127) * 128 + ((piece & 7) ^ (r & 7)) * 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(on ? from + off : from - piece * 16), "r"(on ? 16 : 0)
+                             : "memory");
+              }
+            }
           }
-          const int e = min(max(int(top >> 7) - 127, -100), 127);
-          bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
-          unit = __uint_as_float(uint32_t(127 - 14 + e) << 23);
-        }
-        sh.q_unit[item_no & 1][r] = unit;
-        auto convert = [&](uint32_t x) {
-          x ^= flip;
-          if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
-            x = pack_pair<false>(__uint_as_float(x << 16) * bring, __uint_as_float(x & 0xffff0000u) * bring);
-          }
-          return x;
-        };
-        unsigned char* to = sh.q[r >> 7] + (r & 127) * 128;
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sh.q_full)) : "memory");
+          for (int r = tid; r < kTileRows; r += kLoadThreads) sh.q_unit[item_no & 1][r] = 1.0f;
+        } else {
+          const uint32_t flip = k.a.scale < 0.0f ? 0x80008000u : 0u;
+          for (int r0 = tid / kPieces; r0 < q_rows; r0 += kRows * kAhead) {
+            uint4 v[kAhead];
 #pragma unroll
-        for (int piece = 0; piece < DP / 8; ++piece) {
-          *reinterpret_cast<uint4*>(to + (piece >> 3) * 16384 + ((piece & 7) ^ (r & 7)) * 16) =
-              make_uint4(convert(v[piece].x), convert(v[piece].y), convert(v[piece].z), convert(v[piece].w));
+            for (int i = 0; i < kAhead; ++i) {
+              const int r = r0 + i * kRows;
+              const int64_t off = r < q_rows ? sh.q_at[r] : -1;
+              v[i] = make_uint4(0, 0, 0, 0);
+              if (there && off >= 0) v[i] = *reinterpret_cast<const uint4*>(from + off);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+              const int r = r0 + i * kRows;
+              float bring = 1.0f;
+              if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+                // The row's largest exponent, over its threads (all lanes come along, whatever their row).
+                uint32_t top = 0;
+                for (uint32_t x : {v[i].x, v[i].y, v[i].z, v[i].w}) top = max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu));
+#pragma unroll
+                for (int w = kPieces >> 1; w; w >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, w));
+                const int e = min(max(int(top >> 7) - 127, -100), 127);
+                bring = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+                if (piece == 0 && r < q_rows) sh.q_unit[item_no & 1][r] = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+              } else {
+                if (piece == 0 && r < q_rows) sh.q_unit[item_no & 1][r] = 1.0f;
+              }
+              auto convert = [&](uint32_t x) {
+                x ^= flip;
+                if constexpr (S::kQuant && Q == PF_DTYPE_BF16) {
+                  x = pack_pair<false>(__uint_as_float(x << 16) * bring, __uint_as_float(x & 0xffff0000u) * bring);
+                }
+                return x;
+              };
+              if (r < q_rows) {
+                *reinterpret_cast<uint4*>(sh.q[r >> 7] + (piece >> 3) * 16384 + (r & 127) * 128 + ((piece & 7) ^ (r & 7)) * 16) =
+                    make_uint4(convert(v[i].x), convert(v[i].y), convert(v[i].z), convert(v[i].w));
+              }
+            }
+          }
+          fence_async_shared();
+          bar_arrive(&sh.q_full);
         }
       }
-      fence_async_shared();
-      bar_arrive(&sh.q_full);
 
       // What the softmax needs of a tile, and where its rows are.
       uint32_t v_exp = 1;
@@ -998,6 +1030,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       halves = it.rows > 128 ? 2 : 1;
       units = it.unit1 - it.unit0;
       if (!(ok = bar_wait_warp(&sh.q_full, item_no & 1, failed))) break;
+      if constexpr (!S::kQuant) fence_async_shared();
       for (int32_t j = 0; j < units && ok; ++j) {
         if (stage_no & 2) {
           tile(j, One{});
@@ -1072,7 +1105,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       const int32_t qh = it.head * it.group + row - i * it.group;
       T* out = reinterpret_cast<T*>(k.a.out.data) + token * k.a.out.token_stride + int64_t(qh) * k.a.out.head_stride;
       float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
-                    (int64_t(max(it.slot, 0)) * kTileRows + r) * (DP + 4);
+                    int64_t(max(it.slot, 0)) * kTileRows * (DP + 2) + r;
       const float times = it.slot >= 0 ? v_unit : l == 0.0f ? 0.0f : v_unit / l;
       bool bad = false;
 #pragma unroll 1
@@ -1087,7 +1120,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
         }
         if (mine && it.slot >= 0) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + 4 + piece * 32 + x) = make_uint4(s[x], s[x + 1], s[x + 2], s[x + 3]);
+          for (int x = 0; x < 32; ++x) part[(2 + piece * 32 + x) * kTileRows] = __uint_as_float(s[x]);
         } else if (mine) {
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
@@ -1108,12 +1141,13 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       bar_arrive(&sh.o_free[h]);
       if (mine) {
         if (it.slot >= 0) {
-          part[0] = m, part[1] = l;
+          part[0] = m, part[kTileRows] = l;
         } else if (k.a.lse) {
           reinterpret_cast<float*>(k.a.lse)[token * k.a.q_heads + qh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
       }
       uint32_t again = __ballot_sync(0xffffffffu, mine && bad && l == l);
+      __syncwarp();
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
@@ -1126,9 +1160,12 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
                                      min(it.begin + it.unit1 * kTileKeys, kv_row_end(k, it.s, i_r)), m_r, l_r, v);
         if (it.slot >= 0) {
           float* to = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
-                      (int64_t(it.slot) * kTileRows + (r & ~31) + src) * (DP + 4);
-          if (lane == 0) to[0] = m_r, to[1] = l_r;
-          if (lane * 4 < DP) *reinterpret_cast<float4*>(to + 4 + lane * 4) = v;
+                      int64_t(it.slot) * kTileRows * (DP + 2) + (r & ~31) + src;
+          if (lane == 0) to[0] = m_r, to[kTileRows] = l_r;
+          if (lane * 4 < DP) {
+            float* at = to + (2 + lane * 4) * kTileRows;
+            at[0] = v.x, at[kTileRows] = v.y, at[2 * kTileRows] = v.z, at[3 * kTileRows] = v.w;
+          }
         } else {
           const float inv = l_r == 0.0f ? 0.0f : 1.0f / l_r;
           if (lane * 4 < int(c.head_dim)) {
@@ -1152,14 +1189,17 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
   }
 }
 
-// Joins the parts of an item that lies in several spans: the block of the CTA in
-// whose span it begins, a warp for a row, weights 2^(m - max).
+// Joins the parts of an item that lies in several spans: blocks of the CTA in whose
+// span it begins, 32 rows each. A part is stored value by value, 256 rows side by
+// side, as the threads that hold a row each write it; here a lane has a row and a
+// warp an eighth of its values, and the results change places in shared memory.
 template <uint32_t Q, int DP>
 __global__ void __launch_bounds__(256) kv_join_tiles_kernel(const __grid_constant__ KvAttendArgs k, const KvTilePlan plan) {
   using T = typename KvElem<Q>::type;
+  constexpr int kValues = DP / 8;  // of a warp
+  __shared__ float rows[32][DP + 1];
   wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const char* ws = reinterpret_cast<const char*>(k.a.workspace);
   const int64_t cta = blockIdx.x;
   int64_t span;
   const KvSpan next = find_span(k, plan, cta + 1, &span);
@@ -1168,50 +1208,46 @@ __global__ void __launch_bounds__(256) kv_join_tiles_kernel(const __grid_constan
   if (at / span != cta) return;
   const KvSeq s = kv_sequence(k, uint32_t(next.seq));
   const int32_t group = int32_t(k.a.q_heads / k.cache.heads);
-  const int32_t row0 = next.tile * kTileRows, rows = min(kTileRows, s.n * group - row0);
+  const int32_t row0 = next.tile * kTileRows, count = min(kTileRows, s.n * group - row0);
   const KvSplit split =
-      item_split(at, tile_units(kv_row_begin(k, s, row0 / group) & -kTileKeys, kv_row_end(k, s, (row0 + rows - 1) / group)), span);
-  const float* parts = reinterpret_cast<const float*>(ws + plan.parts_at);
-  for (int32_t r = int32_t(blockIdx.y) * 8 + warp; r < rows; r += int32_t(gridDim.y) * 8) {
-    // A lane for a part's maximum and sum, then all lanes for each part's values.
-    float top = -INFINITY, sum = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    for (int64_t p0 = split.first; p0 <= split.last; p0 += 32) {
-      const bool on = p0 + lane <= split.last;
-      const float* mine = parts + (part_slot(at, on ? p0 + lane : p0, span) * kTileRows + r) * (DP + 4);
-      const float m = on ? mine[0] : -INFINITY, l = on ? mine[1] : 0.0f;
-      float now = m;
-      for (int w = 16; w; w >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, w));
-      now = fmaxf(now, top);
-      const float base = now == -INFINITY ? 0.0f : now;
-      const float keep = exp2f(top - base), by = exp2f(m - base);
-      float part_sum = l * by;
-      for (int w = 16; w; w >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, w);
-      sum = sum * keep + part_sum;
-      o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
-      top = now;
-      const int count = int(min(int64_t(32), split.last - p0 + 1));
-#pragma unroll 4
-      for (int u = 0; u < count; ++u) {
-        const float weight = __shfl_sync(0xffffffffu, by, u);
-        if (lane * 4 < DP) {
-          const float4 v = *reinterpret_cast<const float4*>(parts + (part_slot(at, p0 + u, span) * kTileRows + r) * (DP + 4) + 4 + lane * 4);
-          o.x += v.x * weight, o.y += v.y * weight, o.z += v.z * weight, o.w += v.w * weight;
-        }
-      }
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int32_t i = (row0 + r) / group, qh = next.head * group + row0 + r - i * group;
-    const int64_t token = int64_t(s.first) + i;
+      item_split(at, tile_units(kv_row_begin(k, s, row0 / group) & -kTileKeys, kv_row_end(k, s, (row0 + count - 1) / group)), span);
+  const int32_t first = int32_t(blockIdx.y) * 32;
+  if (first >= count) return;
+  const float* parts = reinterpret_cast<const float*>(reinterpret_cast<const char*>(k.a.workspace) + plan.parts_at) + first + lane;
+  float top = -INFINITY, sum = 0.0f, o[kValues];
+#pragma unroll
+  for (int x = 0; x < kValues; ++x) o[x] = 0.0f;
+  for (int64_t p = split.first; p <= split.last; ++p) {
+    const float* part = parts + part_slot(at, p, span) * kTileRows * (DP + 2);
+    float v[kValues];
+    const float m = part[0], l = part[kTileRows];
+#pragma unroll
+    for (int x = 0; x < kValues; ++x) v[x] = part[(2 + warp * kValues + x) * kTileRows];
+    const float now = fmaxf(top, m), base = now == -INFINITY ? 0.0f : now;
+    const float keep = exp2f(top - base), by = exp2f(m - base);
+    sum = sum * keep + l * by;
+#pragma unroll
+    for (int x = 0; x < kValues; ++x) o[x] = o[x] * keep + v[x] * by;
+    top = now;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int x = 0; x < kValues; ++x) rows[lane][warp * kValues + x] = o[x] * inv;
+  if (warp == 0 && k.a.lse && first + lane < count) {
+    const int32_t row = row0 + first + lane, i = row / group;
+    reinterpret_cast<float*>(k.a.lse)[(int64_t(s.first) + i) * k.a.q_heads + next.head * group + row - i * group] =
+        sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+  __syncthreads();
+  for (int r = warp; r < 32 && first + r < count; r += 8) {
+    const int32_t row = row0 + first + r, i = row / group;
+    T* out = reinterpret_cast<T*>(k.a.out.data) + (int64_t(s.first) + i) * k.a.out.token_stride +
+             int64_t(next.head * group + row - i * group) * k.a.out.head_stride;
     if (lane * 4 < int(k.cache.head_dim)) {
       KvPack<T, 4> y;
-      y.v[0] = kv_from_float<Q>(o.x * inv), y.v[1] = kv_from_float<Q>(o.y * inv);
-      y.v[2] = kv_from_float<Q>(o.z * inv), y.v[3] = kv_from_float<Q>(o.w * inv);
-      *reinterpret_cast<KvPack<T, 4>*>(reinterpret_cast<T*>(k.a.out.data) + token * k.a.out.token_stride +
-                                       int64_t(qh) * k.a.out.head_stride + lane * 4) = y;
-    }
-    if (lane == 0 && k.a.lse) {
-      reinterpret_cast<float*>(k.a.lse)[token * k.a.q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y.v[x] = kv_from_float<Q>(rows[r][lane * 4 + x]);
+      *reinterpret_cast<KvPack<T, 4>*>(out + lane * 4) = y;
     }
   }
 }
@@ -1278,7 +1314,7 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvTilePlan& p, cudaStream_t s
   kv_tile_costs_kernel<<<1, 1024, 0, stream>>>(k, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
   if ((err = launch_early(kernel, dim3(p.ctas), Tiles<Q, STORE, DP>::kThreads, shm, stream, k, plan, maps)) != cudaSuccess) return err;
-  return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, 16), 256, 0, stream, k, p);
+  return launch_early(kv_join_tiles_kernel<Q, DP>, dim3(p.ctas, kTileRows / 32), 256, 0, stream, k, p);
 }
 
 template <uint32_t Q, uint32_t STORE>
@@ -1311,7 +1347,7 @@ KvTilePlan tile_plan(const KvAttendArgs& k, int num_sms) {
   };
   p.costs_at = take((uint64_t(k.a.n_seqs) + 1) * sizeof(int64_t));
   const uint64_t dp = k.cache.head_dim <= 64 ? 64 : 128;
-  p.parts_at = take(2 * uint64_t(p.ctas) * kTileRows * (dp + 4) * sizeof(float));
+  p.parts_at = take(2 * uint64_t(p.ctas) * kTileRows * (dp + 2) * sizeof(float));
   return p;
 }
 

@@ -25,7 +25,7 @@ struct KvTilePlan {
   uint32_t box_rows;     // tokens of a TMA box, 0: none
   uint32_t reserved;
   uint64_t costs_at;     // byte offsets in the workspace: int64[n_seqs + 1], units in front of each sequence
-  uint64_t parts_at;     // float[2 * ctas][kTileRows][dp + 4]
+  uint64_t parts_at;     // float[2 * ctas][dp + 2][kTileRows]: maxima, sums, values
   uint64_t bytes;
 };
 
