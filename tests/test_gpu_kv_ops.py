@@ -271,14 +271,15 @@ def attend_plain(torch, q, k, v, lens, counts, table, page, scale, causal=True, 
 
 
 def attend_bound(torch, dtype, quantised, out, mag, dot, longest, dim):
-    """How far an output element may be: its own rounding (u of the output's type); the weights' rounding to 16 bits for
-    the second product (u of that type: bf16 over an 8-bit cache) and the scores' error, both times sum_j w_j |v_j|.
-    A score is a sum of dim products (exact) in fp32, an addition off by at most 2^-23 (accumulation may truncate), then
-    two products: e = (dim + 4) 2^-23 max_j sum_d |q_d k_jd|. It moves a weight, and the sum it is divided by, by
-    exp(e) each. The exponential is off by 2^-21, the sums of `longest` terms by 2^-23 an addition in tiles of
-    128 at most that are then added up."""
+    """How far an output element may be: its own rounding (u of the output's type); the roundings to 16 bits in front
+    of the second product, and the scores' error, both times sum_j w_j |v_j|. Those roundings: the weight's (u of the
+    type; over an 8-bit cache fp16's, and for a bf16 output V's scale and V times it too, 2^-11 each). A score is a sum
+    of dim products (exact) in fp32, an addition off by at most 2^-23 (accumulation may truncate), then two products:
+    e = (dim + 4) 2^-23 max_j sum_d |q_d k_jd|. It moves a weight, and the sum it is divided by, by exp(e) each. The
+    exponential is off by 2^-21, the sums of `longest` terms by 2^-23 an addition in tiles of 128 at most that are then
+    added up."""
     u_out = torch.finfo(dtype).eps / 2
-    u_p = torch.finfo(torch.bfloat16 if quantised else dtype).eps / 2
+    u_p = torch.finfo(dtype).eps / 2 if not quantised else 2.0 ** -11 * (3 if dtype == torch.bfloat16 else 1)
     e = (dim + 4) * 2.0 ** -23 * dot[..., None]
     sums = (128 + longest / 128 + 64) * 2.0 ** -23
     return u_out * out.abs() + (u_p + 2 * torch.expm1(e) + 2 * sums + 2.0 ** -20) * mag * 1.01 + 1e-30, \
