@@ -51,7 +51,7 @@ void check_attention(const pf_kv_cache& c, const pf_kv_attention& a) {
   if (!a.q_heads || a.q_heads % c.heads) refuse("query heads must be a multiple of the cache's heads");
   if (a.q_heads > (1u << 16)) refuse("query heads out of range");
   if (a.n_tokens > INT32_MAX / 2 || a.n_tokens * a.q_heads > INT32_MAX) refuse("too many query tokens");
-  if (a.n_seqs > INT32_MAX / 2 || a.max_blocks > INT32_MAX) refuse("too many sequences or blocks");
+  if (uint64_t(a.n_seqs) * c.heads > INT32_MAX / 2 || a.max_blocks > INT32_MAX) refuse("too many sequences or blocks");
   if (uint64_t(a.max_blocks) * c.block_size > INT32_MAX) refuse("block table names more tokens than an int32 can count");
   const uint32_t elt = kv_dtype_bytes(c.dtype);
   if (!aligned_rows(c.key.data, c.key.block_stride, c.key.token_stride, c.key.head_stride, elt) ||

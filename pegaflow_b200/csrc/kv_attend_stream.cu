@@ -154,9 +154,10 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
   const pf_kv_cache& c = k.cache;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  // Sequences along x, the axis that has room for any number of them.
-  const uint32_t part = blockIdx.z, head = blockIdx.y;
-  const uint32_t seq = blockIdx.x / plan.tiles;
+  // Along x, the axis that has room for any number: the heads of a sequence side by side, because in most layouts
+  // their rows of a token are, and run at the same time they meet in HBM's open pages.
+  const uint32_t part = blockIdx.y, item = blockIdx.x / c.heads, head = blockIdx.x - item * c.heads;
+  const uint32_t seq = item / plan.tiles;
   const int32_t group = int32_t(k.a.q_heads / c.heads);
   let_next_kernel_start();
   auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
   const KvSeq s = kv_sequence(k, seq);
   const int32_t rows = s.n * group;
   // Tiles beyond the bound that the grid was made for are taken by its CTAs in turn.
-  for (int32_t row0 = int32_t(blockIdx.x % plan.tiles) * S::kRows; row0 < rows; row0 += int32_t(plan.tiles) * S::kRows) {
+  for (int32_t row0 = int32_t(item % plan.tiles) * S::kRows; row0 < rows; row0 += int32_t(plan.tiles) * S::kRows) {
     const int32_t row_last = min(rows, row0 + S::kRows) - 1;
     const int32_t begin = kv_row_begin(k, s, row0 / group);
     const int32_t end = kv_row_end(k, s, row_last / group);
@@ -658,7 +659,7 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shm);
     if (err != cudaSuccess) return err;
   }
-  kernel<<<dim3(k.a.n_seqs * p.tiles, k.cache.heads, p.parts), kThreads, shm, stream>>>(k, p);
+  kernel<<<dim3(k.a.n_seqs * p.tiles * k.cache.heads, p.parts), kThreads, shm, stream>>>(k, p);
   if (p.parts == 1) return cudaGetLastError();
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;

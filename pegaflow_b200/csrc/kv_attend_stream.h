@@ -10,7 +10,7 @@
 namespace pf {
 
 constexpr uint32_t kStreamMaxRows = 16;  // queries times heads of a group that one CTA takes
-constexpr uint32_t kStreamMaxParts = 32768;  // a grid's z axis ends at 65,535
+constexpr uint32_t kStreamMaxParts = 32768;  // a grid's y axis ends at 65,535
 constexpr uint32_t kStreamMinPart = 128;  // tokens: a batch for each warp
 
 struct KvStreamPlan {
