@@ -70,6 +70,10 @@ __device__ __forceinline__ void copy16(void* to, const char* from, const char* v
                : "memory");
 }
 
+__device__ __forceinline__ void copy16(void* to, const char* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -206,6 +210,13 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     // This warp's batches: warp, warp + 4, ...; step i is half of its batch i / 2.
     const int32_t mine = warp < batches ? (batches - warp + kWarps - 1) / kWarps : 0;
     typename S::Step* ring = sh.ring[warp];
+    const char* key_from = key_base + lane % S::kPieces * 16;
+    const char* value_from = value_base + lane % S::kPieces * 16;
+    int32_t whole = 0;  // this warp's batches up to here have all their rows: most steps are copied without a look
+    auto stage_store = [&](int32_t n) {
+      sh.staged[warp][n & 1][lane] = fresh;
+      if (n == whole && __all_sync(0xffffffffu, fresh.key >= 0)) ++whole;
+    };
     auto copy_step = [&](int32_t i) {
       if (i < 2 * mine) {
         typename S::Step& to = ring[i % kRing];
@@ -219,11 +230,20 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
           key_at[x] = rows[x * kRowsAtOnce + lane / S::kPieces].key;
           value_at[x] = rows[x * kRowsAtOnce + lane / S::kPieces].value;
         }
+        if (i >> 1 < whole && int(c.head_dim) == DP) {
 #pragma unroll
-        for (int x = 0; x < kStep / kRowsAtOnce; ++x) {
-          const int row = x * kRowsAtOnce + lane / S::kPieces;
-          copy16(to.key[row] + S::key_piece(row, piece) * 16, key_base + key_at[x] + piece * 16, key_base, there && key_at[x] >= 0);
-          copy16(to.value[row] + S::value_piece(row, piece) * 16, value_base + value_at[x] + piece * 16, value_base, there && value_at[x] >= 0);
+          for (int x = 0; x < kStep / kRowsAtOnce; ++x) {
+            const int row = x * kRowsAtOnce + lane / S::kPieces;
+            copy16(to.key[row] + S::key_piece(row, piece) * 16, key_from + key_at[x]);
+            copy16(to.value[row] + S::value_piece(row, piece) * 16, value_from + value_at[x]);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < kStep / kRowsAtOnce; ++x) {
+            const int row = x * kRowsAtOnce + lane / S::kPieces;
+            copy16(to.key[row] + S::key_piece(row, piece) * 16, key_base + key_at[x] + piece * 16, key_base, there && key_at[x] >= 0);
+            copy16(to.value[row] + S::value_piece(row, piece) * 16, value_base + value_at[x] + piece * 16, value_base, there && value_at[x] >= 0);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -233,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       stage_blocks(warp);
       stage_addresses(warp);
       stage_blocks(warp + kWarps);
-      sh.staged[warp][0][lane] = fresh;
+      stage_store(0);
       __syncwarp();
     }
     copy_step(0);
@@ -311,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       const int32_t batch = warp + (i >> 1) * kWarps, j0 = lo + batch * kBatch + (i & 1) * kStep;
       if ((i & 1) == 0) {
         // The next batch's addresses: its buffer's last readers are behind the end of the batch before.
-        sh.staged[warp][(i >> 1 & 1) ^ 1][lane] = fresh;
+        stage_store((i >> 1) + 1);
         stage_addresses(batch + 2 * kWarps);
         stage_blocks(batch + 3 * kWarps);
       }
