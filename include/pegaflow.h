@@ -580,7 +580,8 @@ typedef enum pf_dtype {
 
 /* K or V of one layer's cache, seen as [num_blocks, block_size, heads,
  * head_dim] with the last axis contiguous. Strides are in elements and may be
- * of any order, so KV-first, blocks-first and token-major buffers all fit.
+ * of any order (none negative), so KV-first, blocks-first and token-major
+ * buffers all fit.
  * An 8-bit cache has one fp32 scale for each token and head (value = code *
  * scale); a scale stride of 0 shares it (one for each block, or one in all). */
 typedef struct pf_kv_side {
@@ -652,7 +653,7 @@ int pf_kv_read(int32_t device_id, const pf_kv_cache* cache,
  * A query that sees nothing gets zeros and lse = -inf; tokens on a bad block
  * are not seen. Query heads are a multiple of the cache's: head h reads KV head
  * h / (q_heads / heads). Query rows outside the sequences are left as they
- * are. Types: queries and outputs bf16 or fp16, the cache the same type, E4M3
+ * are; `out` is memory of its own. Types: queries and outputs bf16 or fp16, the cache the same type, E4M3
  * or INT8; head_dim a multiple of 16 up to 128; rows 16-byte aligned. */
 typedef struct pf_kv_attention {
   pf_kv_rows query;       /* [n_tokens, q_heads, head_dim] */

@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <climits>
+#include <cmath>
 #include <mutex>
 #include <string>
 
@@ -17,6 +18,10 @@ void check_side(const pf_kv_cache& c, const pf_kv_side& s, const char* name) {
   const std::string n = name;
   if (!s.data) refuse(n + " cache has no address");
   if (s.data % kv_dtype_bytes(c.dtype)) refuse(n + " cache address is not aligned to its elements");
+  if (s.block_stride < 0 || s.token_stride < 0 || s.head_stride < 0 || s.scale_block_stride < 0 || s.scale_token_stride < 0 ||
+      s.scale_head_stride < 0) {
+    refuse(n + " cache has a negative stride");
+  }
   if (kv_quantised(c.dtype)) {
     if (!s.scale) refuse(n + " cache of 8 bits needs scales");
     if (s.scale % 4) refuse(n + " scale address is not aligned to 4 bytes");
@@ -36,6 +41,13 @@ void check_cache(const pf_kv_cache& c) {
 void check_rows(const pf_kv_rows& r, uint32_t dtype, const char* name) {
   if (!r.data) refuse(std::string(name) + " has no address");
   if (r.data % kv_dtype_bytes(dtype)) refuse(std::string(name) + " address is not aligned to its elements");
+  if (r.token_stride < 0 || r.head_stride < 0) refuse(std::string(name) + " has a negative stride");
+}
+
+// Rows that are written: each in a place of its own.
+void check_results(const pf_kv_rows& r, uint32_t dtype, uint64_t n, uint64_t heads, const char* name) {
+  check_rows(r, dtype, name);
+  if ((n > 1 && !r.token_stride) || (heads > 1 && !r.head_stride)) refuse(std::string(name) + " has rows that share their place");
 }
 
 bool aligned_rows(uint64_t data, int64_t a, int64_t b, int64_t c, uint32_t elt) {
@@ -52,7 +64,8 @@ void check_attention(const pf_kv_cache& c, const pf_kv_attention& a) {
   if (a.q_heads > (1u << 16)) refuse("query heads out of range");
   if (a.n_tokens > INT32_MAX / 2 || a.n_tokens * a.q_heads > INT32_MAX) refuse("too many query tokens");
   if (uint64_t(a.n_seqs) * c.heads > INT32_MAX / 2 || a.max_blocks > INT32_MAX) refuse("too many sequences or blocks");
-  if (uint64_t(a.max_blocks) * c.block_size > INT32_MAX) refuse("block table names more tokens than an int32 can count");
+  if (uint64_t(a.max_blocks) * c.block_size > kKvMaxTokens) refuse("block table names more tokens than an int32 can count");
+  if (!std::isfinite(a.scale)) refuse("scale must be finite");
   const uint32_t elt = kv_dtype_bytes(c.dtype);
   if (!aligned_rows(c.key.data, c.key.block_stride, c.key.token_stride, c.key.head_stride, elt) ||
       !aligned_rows(c.value.data, c.value.block_stride, c.value.token_stride, c.value.head_stride, elt)) {
@@ -103,6 +116,12 @@ int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, uint64_t key, int64
     const pf_kv_rows k{key, key_token_stride, key_head_stride}, v{value, value_token_stride, value_head_stride};
     check_rows(k, dtype, "key");
     check_rows(v, dtype, "value");
+    for (const pf_kv_side* s : {&cache->key, &cache->value}) {
+      if ((cache->num_blocks > 1 && !s->block_stride) || (cache->block_size > 1 && !s->token_stride) ||
+          (cache->heads > 1 && !s->head_stride)) {
+        refuse("a cache whose rows share their place cannot be written");
+      }
+    }
     if (!slots) refuse("no slots");
     DeviceGuard g(device_id);
     const KvWriteArgs args{*cache, k, v, slots, n, status, dtype, given_scales ? 1u : 0u, uint32_t(num_sms(device_id))};
@@ -122,10 +141,10 @@ int pf_kv_read(int32_t device_id, const pf_kv_cache* cache, const int32_t* block
     if (n_rows > INT32_MAX || n_rows * cache->heads > UINT32_MAX) refuse("too many rows");
     if (n_seqs > INT32_MAX / 2) refuse("too many sequences");
     if (!n_rows || !n_seqs) return;
-    if (uint64_t(max_blocks) * cache->block_size > INT32_MAX) refuse("block table names more tokens than an int32 can count");
+    if (uint64_t(max_blocks) * cache->block_size > kKvMaxTokens) refuse("block table names more tokens than an int32 can count");
     const pf_kv_rows k{key, key_token_stride, key_head_stride}, v{value, value_token_stride, value_head_stride};
-    check_rows(k, dtype, "key");
-    check_rows(v, dtype, "value");
+    check_results(k, dtype, n_rows, cache->heads, "key");
+    check_results(v, dtype, n_rows, cache->heads, "value");
     if ((!block_table && max_blocks) || !starts) refuse("no block table or starts");
     DeviceGuard g(device_id);
     const KvReadArgs args{*cache, k, v, block_table, starts, status, table_stride, n_rows, max_blocks, n_seqs, dtype, uint32_t(num_sms(device_id))};
@@ -151,7 +170,7 @@ int pf_kv_attention_run(int32_t device_id, const pf_kv_cache* cache, const pf_kv
     const pf_kv_attention& a = *args;
     if (!a.n_tokens || !a.n_seqs) return;
     check_rows(a.query, a.dtype, "query");
-    check_rows(a.out, a.dtype, "out");
+    check_results(a.out, a.dtype, a.n_tokens, a.q_heads, "out");
     const uint32_t elt = kv_dtype_bytes(a.dtype);
     if (!aligned_rows(a.query.data, a.query.token_stride, a.query.head_stride, 0, elt) ||
         !aligned_rows(a.out.data, a.out.token_stride, a.out.head_stride, 0, elt)) {
@@ -164,6 +183,7 @@ int pf_kv_attention_run(int32_t device_id, const pf_kv_cache* cache, const pf_kv
         (a.workspace_bytes && !a.workspace)) {
       refuse("attention workspace is too small or not aligned to 16 bytes");
     }
+    if (a.out.data == a.query.data) refuse("out cannot be the query: rows are read again after others are written");
     DeviceGuard g(device_id);
     cuda_check(launch_kv_attention(k, sms, static_cast<cudaStream_t>(stream)), "kv_attention launch");
   });

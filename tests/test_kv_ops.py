@@ -201,6 +201,59 @@ def test_library_refuses_attention(native, make, change, words):
     assert rc == N.PF_ERR_INVALID_ARGUMENT and words in message(N), message(N)
 
 
+@pytest.mark.parametrize("axis", ["block_stride", "token_stride", "head_stride", "scale_block_stride",
+                                  "scale_token_stride", "scale_head_stride"])
+def test_library_refuses_negative_strides(native, axis):
+    from ctypes import byref
+
+    N = native
+    c = c_cache(N, N.PF_DTYPE_INT8)
+    setattr(c.value, axis, -getattr(c.value, axis))
+    r = (4096, 128, 64)
+    assert N.lib.pf_kv_write(0, byref(c), *r, *r, N.PF_DTYPE_BF16, 4096, 3, 0, 0, 0) == N.PF_ERR_INVALID_ARGUMENT
+    assert "negative stride" in message(N)
+    c = c_cache(N, N.PF_DTYPE_BF16)
+    a = attention(N, c)
+    a.query.head_stride = -64
+    assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_ERR_INVALID_ARGUMENT
+    assert "query has a negative stride" in message(N)
+
+
+def test_library_refuses_results_that_share_their_place(native):
+    from ctypes import byref
+
+    N = native
+    c = c_cache(N, N.PF_DTYPE_BF16)
+    r, flat = (4096, 128, 64), (4096, 128, 0)
+    rc = N.lib.pf_kv_read(0, byref(c), 4096, 4, 4, 1, 4096, *r, *flat, N.PF_DTYPE_BF16, 5, 0, 0)
+    assert rc == N.PF_ERR_INVALID_ARGUMENT and "value has rows that share" in message(N)
+    a = attention(N, c)
+    a.out.token_stride = 0
+    assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_ERR_INVALID_ARGUMENT
+    assert "out has rows that share" in message(N)
+    c.key.block_stride = 0
+    rc = N.lib.pf_kv_write(0, byref(c), *r, *r, N.PF_DTYPE_BF16, 4096, 3, 0, 0, 0)
+    assert rc == N.PF_ERR_INVALID_ARGUMENT and "cannot be written" in message(N)
+
+
+@pytest.mark.parametrize("change, words", [
+    ({"scale": float("nan")}, "scale must be finite"),
+    ({"scale": float("inf")}, "scale must be finite"),
+    ({"max_blocks": (1 << 31) // 16 - 4095}, "block table names more tokens"),
+])
+def test_library_refuses_scales_and_lengths(native, change, words):
+    """A length that a tile's end would carry past an int32 is refused; the longest below it is not, for its sake."""
+    from ctypes import byref
+
+    N = native
+    c = c_cache(N, N.PF_DTYPE_BF16)
+    a = attention(N, c, **change)
+    assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_ERR_INVALID_ARGUMENT
+    assert words in message(N), message(N)
+    a = attention(N, c, max_blocks=(1 << 31) // 16 - 4096, n_tokens=0)
+    assert N.lib.pf_kv_attention_run(0, byref(c), byref(a), 0) == N.PF_OK
+
+
 def test_library_refuses_unaligned_queries(native):
     from ctypes import byref
 
