@@ -83,16 +83,18 @@ __device__ __forceinline__ float4 kv_load4(const pf_kv_side& side, int64_t block
                      kv_to_float<STORE>(v.v[3]) * s);
 }
 
-// One row of the formula over the tokens [lo, hi), by one warp, a token at a
+// One row of the formula over the tokens [lo, hi), by one warp, four tokens at a
 // time, masked tokens never touched: lane l gets the values 4 l .. 4 l + 3 of
 // sum_j 2^(s_j - m) v_j, and m (in powers of two) and the sum of the weights.
+// `alive` (null: none) counts up every 1,024 tokens, for those who wait meanwhile.
 //
 // Matrix products multiply masked values by a weight of zero, which an infinity
 // or a NaN turns into NaN; the kernels send the rows that this may have hit
 // through here. It is for such rows alone: it reads the keys once for each row.
 template <uint32_t Q, uint32_t STORE>
 __device__ __noinline__ void attend_row_exactly(const KvAttendArgs& k, uint32_t seq, int64_t token, uint32_t qh,
-                                                uint32_t head, int32_t lo, int32_t hi, float& m, float& l, float4& o) {
+                                                uint32_t head, int32_t lo, int32_t hi, float& m, float& l, float4& o,
+                                                int* alive) {
   using T = typename KvElem<Q>::type;
   const pf_kv_cache& c = k.cache;
   const uint32_t d = (threadIdx.x & 31) * 4;
@@ -106,25 +108,42 @@ __device__ __noinline__ void attend_row_exactly(const KvAttendArgs& k, uint32_t 
   m = -INFINITY;
   l = 0.0f;
   o = make_float4(0, 0, 0, 0);
-  for (int32_t j = lo; j < hi; ++j) {
-    const int32_t block = kv_block(k, seq, uint32_t(j) / c.block_size);
-    if (block < 0) continue;
-    const uint32_t offset = uint32_t(j) % c.block_size;
-    float s = 0.0f;
-    float4 v = make_float4(0, 0, 0, 0);
-    if (mine) {
-      const float4 x = kv_load4<STORE>(c.key, block, offset, head, d);
-      v = kv_load4<STORE>(c.value, block, offset, head, d);
-      s = q.x * x.x + q.y * x.y + q.z * x.z + q.w * x.w;
+  constexpr int kAtOnce = 4;
+  for (int32_t j0 = lo, n = 0; j0 < hi; j0 += kAtOnce, ++n) {
+    float s[kAtOnce];
+    float4 v[kAtOnce];
+    bool on[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int32_t j = j0 + u, block = j < hi ? kv_block(k, seq, uint32_t(j) / c.block_size) : -1;
+      on[u] = block >= 0;
+      s[u] = 0.0f;
+      v[u] = make_float4(0, 0, 0, 0);
+      if (on[u] && mine) {
+        const uint32_t offset = uint32_t(j) % c.block_size;
+        const float4 x = kv_load4<STORE>(c.key, block, offset, head, d);
+        v[u] = kv_load4<STORE>(c.value, block, offset, head, d);
+        s[u] = q.x * x.x + q.y * x.y + q.z * x.z + q.w * x.w;
+      }
     }
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= k.a.scale * kLog2e;
-    const float top = fmaxf(m, s);
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float keep = exp2f(m - base), p = exp2f(s - base);
-    l = l * keep + p;
-    o = make_float4(o.x * keep + p * v.x, o.y * keep + p * v.y, o.z * keep + p * v.z, o.w * keep + p * v.w);
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      for (int w = 16; w; w >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+      s[u] = on[u] ? s[u] * (k.a.scale * kLog2e) : -INFINITY;
+      top = fmaxf(top, s[u]);
+    }
+    const float base = top == -INFINITY ? 0.0f : top, keep = exp2f(m - base);
+    l *= keep;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float p = exp2f(s[u] - base);
+      l += p;
+      if (on[u]) o = make_float4(o.x + p * v[u].x, o.y + p * v[u].y, o.z + p * v[u].z, o.w + p * v[u].w);
+    }
     m = top;
+    if (alive && (n & 255) == 255 && (threadIdx.x & 31) == 0) atomicAdd(alive, 1);
   }
 }
 

@@ -22,9 +22,11 @@
 // permutation. P^T is S^T transposed: one movmatrix.
 //
 // 8-bit codes become fp16, which holds all of e4m3 and int8 exactly; the scales
-// stay in fp32: K's multiplies the score, V's the weight. Weights are rounded to
-// 16 bits for the second product, divided by a power of two that follows the
-// largest V scale, so that fp16 has its full precision at any scale. A bf16
+// stay in fp32: K's multiplies the score, V's the weight. Weights times V's scales
+// are rounded to fp16 for the second product. So the running maximum is that of the
+// score plus the V scale's exponent (2^-63 to 2^63): a row's largest weight times
+// scale is near 1 whatever the scales are, and what the row does not see has no part
+// in it. A bf16
 // query is brought into fp16's range by a power of two for each row: values down
 // to 2^-28 of the row's largest stay exact, smaller ones are off by at most 2^-39
 // of it.
@@ -133,6 +135,11 @@ struct Stream {
     unsigned char key[kStep][kRowBytes];
     unsigned char value[kStep][kRowBytes];
   };
+  // The power of two (of a V scale) that the running maximum counts.
+  static __device__ __forceinline__ float exponent(float scale) {
+    if constexpr (!kQuant) return 0.0f;
+    return float(min(max(int(__float_as_uint(scale) >> 23 & 255) - 127, -63), 63));
+  }
   static __device__ __forceinline__ int key_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row & 1) << 2 : piece; }
   static __device__ __forceinline__ int value_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row >> 1 & 3) << 1 : piece ^ (row >> 1 & 3); }
   struct Shared {
@@ -324,7 +331,6 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.0f;
     }
-    uint32_t v_exp = 1;  // exponent field of the power of two that the weights are divided by
 
 #pragma unroll 1
     for (int32_t i = 0; i < 2 * mine; ++i) {
@@ -341,24 +347,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       const typename S::Step& now = ring[i % kRing];
       const Staged s0 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g], s1 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g + 8];
 
-      float v_inv = 1.0f;
-      if constexpr (S::kQuant) {
-        const uint32_t largest = __float_as_uint(fmaxf(fabsf(s0.value_scale), fabsf(s1.value_scale)));
-        const uint32_t e = min(__reduce_max_sync(0xffffffffu, largest) >> 23, 253u);
-        if (e > v_exp) {
-          const float keep = e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int x = 0; x < S::kTiles; ++x) {
-#pragma unroll
-              for (int y = 0; y < 4; ++y) o[n][x][y] *= keep;
-            }
-          }
-          v_exp = e;
-        }
-        v_inv = __uint_as_float((254 - v_exp) << 23);
-      }
+      const float e0 = S::exponent(s0.value_scale), e1 = S::exponent(s1.value_scale);
       // S^T: c0, c1 are token g's scores for the rows 2 t and 2 t + 1, c2, c3 token g + 8's.
       float x[NT][4];
 #pragma unroll
@@ -409,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        raise = raise || fmaxf(x[n][0], x[n][2]) > m[n][0] + kRaise || fmaxf(x[n][1], x[n][3]) > m[n][1] + kRaise;
+        raise = raise || fmaxf(x[n][0] + e0, x[n][2] + e1) > m[n][0] + kRaise || fmaxf(x[n][1] + e0, x[n][3] + e1) > m[n][1] + kRaise;
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -417,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
           float keep[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[n][e], x[n][e + 2]);
+            float top = fmaxf(x[n][e] + e0, x[n][e + 2] + e1);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -441,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
           const float base = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
           w[e] = fast_exp2(x[n][e] - base);
           l[n][e & 1] += w[e];
-          if constexpr (S::kQuant) w[e] *= (e < 2 ? s0.value_scale : s1.value_scale) * v_inv;
+          if constexpr (S::kQuant) w[e] *= e < 2 ? s0.value_scale : s1.value_scale;
         }
         const uint32_t first = pack2<S::kBf16>(w[0], w[1]), second = pack2<S::kBf16>(w[2], w[3]);
         p[n][0] = transpose_8x8(first);
@@ -495,7 +484,6 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     __syncwarp();  // the ring is free for the sums
 
     // The warps' shares, then the part's: [row][value] in shared memory.
-    const float v_unit = S::kQuant ? __uint_as_float(v_exp << 23) : 1.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -513,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       for (int i = 0; i < S::kTiles; ++i) {
         const int d = S::kQuant ? g * (DP / 8) + 2 * i : (i / 4 * 8 + g) * 8 + i % 4 * 2;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh.o[warp][(n * 8 + 2 * t + (e & 1)) * DP + d + (e >> 1)] = o[n][i][e] * v_unit;
+        for (int e = 0; e < 4; ++e) sh.o[warp][(n * 8 + 2 * t + (e & 1)) * DP + d + (e >> 1)] = o[n][i][e];
       }
     }
     if (threadIdx.x < S::kRows) sh.bad[threadIdx.x] = 0;
@@ -567,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         float top, sum;
         float4 v;
         attend_row_exactly<Q, STORE>(k, seq, int64_t(s.first) + i, head * group + uint32_t(r - i * group), head,
-                                     max(lo, kv_row_begin(k, s, i)), min(hi, kv_row_end(k, s, i)), top, sum, v);
+                                     max(lo, kv_row_begin(k, s, i)), min(hi, kv_row_end(k, s, i)), top, sum, v, nullptr);
         if (lane * 4 < DP) {
           finish(r, lane * 4, top, sum, v.x);
           finish(r, lane * 4 + 1, top, sum, v.y);
@@ -593,16 +581,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_join_stream_kernel(const _
   const uint64_t id = blockIdx.x;
   const uint32_t token = uint32_t(id / k.a.q_heads), qh = uint32_t(id % k.a.q_heads);
   const uint32_t seq = kv_find_seq(reinterpret_cast<const int32_t*>(k.a.q_start), k.a.n_seqs, token);
-  if (seq == k.a.n_seqs) return;
-  const KvSeq s = kv_sequence(k, seq);
+  KvSeq s{0, 0, 0, 0};
+  if (seq < k.a.n_seqs) s = kv_sequence(k, seq);
   const int32_t group = int32_t(k.a.q_heads / k.cache.heads), rows = s.n * group;
   const int32_t r = (int32_t(token) - s.first) * group + int32_t(qh) % group;
-  if (r >= rows) return;
   const int32_t tile_rows = 8 * int32_t(plan.row_tiles);
   const int32_t row0 = r / tile_rows * tile_rows, row_last = min(rows, row0 + tile_rows) - 1;
   const int32_t used = stream_parts(plan, kv_row_end(k, s, row_last / group) - kv_row_begin(k, s, row0 / group));
-  if (used == 1) return;
+  // Every block waits, those without work too: this kernel's end is what the next in the stream goes by.
   wait_for_previous_kernel();
+  if (seq == k.a.n_seqs || r >= rows || used == 1) return;
   const float* ws = reinterpret_cast<const float*>(k.a.workspace) + id * plan.parts * (DP + 4);
   // The warp's own running maximum, then the block's.
   float top = -INFINITY, sum = 0.0f;

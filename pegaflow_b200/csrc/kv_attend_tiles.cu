@@ -53,7 +53,13 @@ struct alignas(16) KeyInfo {
   uint32_t seen[kTileKeys / 32];
   uint32_t v_exp;             // that power's exponent field; it never falls within an item
   uint32_t boxed;             // came by TMA
-  uint32_t pad[2];
+  float top_scale;            // the largest of value_scale
+  float low_scale;            // and the smallest, of tokens that are there
+};
+
+struct Watch {
+  int failed;  // a wait gave up
+  int alive;   // counts up while rows are made again
 };
 
 struct KvBoxMaps {
@@ -81,14 +87,15 @@ struct Tiles {
     KeyInfo info[kInfos];
     float q_unit[2][kTileRows];  // by the item's parity
     int64_t q_at[kTileRows];
-    uint32_t warp_max[2][kTileKeys / 32];  // by the tile's parity
+    uint32_t warp_max[2][kTileKeys / 32];  // of V's scales, by the tile's parity
+    uint32_t warp_min[2][kTileKeys / 32];
     uint64_t q_full, q_empty;
     uint64_t kv_full[kStages], kv_empty[kStages];
     uint64_t info_full[kInfos], info_empty[kInfos];
     uint64_t s_full[2], p_full[2], o_full[2], o_free[2], done;
     uint32_t tmem;
-    int failed;  // a wait gave up
-    int stuck[2];  // those for copies and products in flight did as well
+    Watch watch;
+    Watch stuck[2];  // waits for copies and products in flight that gave up as well
   };
   // TMEM columns (all 512 are allocated, so they begin at 0).
   static constexpr uint32_t kS = 0, kO = 256;
@@ -112,27 +119,40 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
   return done;
 }
 // Whether the phase of `parity` completed, within kWaitClocks and before another
-// wait of this CTA gave up.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* failed) {
-  if (bar_try(bar, parity)) return true;
-  if (*reinterpret_cast<volatile int*>(failed)) return false;
-  const long long t0 = clock64();
+// wait of this CTA gave up. Rows made again token by token take their time: as
+// long as they get on, the clock starts anew. Out of line: the kernel waits in
+// some twenty places, and with this in each it is slower (391 us against 358 for
+// 2,048 tokens after 8,192: the code that runs all the time no longer fits).
+__device__ __noinline__ bool bar_wait_longer(uint64_t* bar, uint32_t parity, Watch* w) {
+  volatile int* failed = &w->failed;
+  volatile int* alive = &w->alive;
+  if (*failed) return false;
+  long long t0 = clock64();
+  int last = *alive;
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i) {
       if (bar_try(bar, parity)) return true;
     }
-    if (*reinterpret_cast<volatile int*>(failed)) return false;
-    if (clock64() - t0 > kWaitClocks) {
-      *reinterpret_cast<volatile int*>(failed) = 1;
+    if (*failed) return false;
+    const int now = *alive;
+    if (now != last) {
+      last = now;
+      t0 = clock64();
+    } else if (clock64() - t0 > kWaitClocks) {
+      *failed = 1;
       return false;
     }
   }
 }
 
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Watch* watch) {
+  return bar_try(bar, parity) || bar_wait_longer(bar, parity, watch);
+}
+
 // The same for a warp, as one.
-__device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, int* failed) {
-  return __all_sync(0xffffffffu, bar_wait(bar, parity, failed));
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, Watch* watch) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, watch));
 }
 // Meets the other loading threads; whether all of them say yes.
 template <int THREADS>
@@ -444,6 +464,24 @@ __device__ __forceinline__ uint32_t seen_bits(const KeyInfo& info, int piece, in
   return info.seen[piece] & below_to & ~below_from;
 }
 
+// The largest V scale among the tokens that the row sees, or, if all of the tile
+// are within 2^4, the smallest there is.
+__device__ __noinline__ float largest_seen(const KeyInfo& info, int32_t lo, int32_t hi) {
+  if (info.low_scale >= info.top_scale * (1.0f / 16)) {
+    uint32_t any = 0;
+    for (int piece = 0; piece < 4; ++piece) any |= seen_bits(info, piece, lo, hi);
+    return any ? info.low_scale : 0.0f;
+  }
+  float top = 0.0f;
+#pragma unroll 1
+  for (int piece = 0; piece < 4; ++piece) {
+    const uint32_t seen = seen_bits(info, piece, lo, hi);
+#pragma unroll
+    for (int x = 0; x < 32; ++x) top = fmaxf(top, seen >> x & 1 ? fabsf(info.value_scale[piece * 32 + x]) : 0.0f);
+  }
+  return top;
+}
+
 // Multiplies a row's fp32 values, or pairs of 16-bit ones, in TMEM: rarely done,
 // so out of the way.
 __device__ __noinline__ void rescale_sums(uint32_t at, int columns, float by) {
@@ -574,7 +612,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       *reinterpret_cast<typename S::Shared*>(raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const pf_kv_cache& c = k.cache;
-  int* failed = &sh.failed;
+  Watch* watch = &sh.watch;
 
   if (threadIdx.x == 0) {
     bar_init(&sh.q_full, kLoadThreads);
@@ -586,7 +624,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       bar_init(&sh.o_full[i], 1), bar_init(&sh.o_free[i], 128);
     }
     bar_init(&sh.done, 1);
-    sh.failed = sh.stuck[0] = sh.stuck[1] = 0;
+    sh.watch = sh.stuck[0] = sh.stuck[1] = Watch{0, 0};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -597,7 +635,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = 0;
-  if (sh.tmem != 0) sh.failed = 1;  // cannot be: the waits would end the call
+  if (sh.tmem != 0) sh.watch.failed = 1;  // cannot be: the waits would end the call
   wait_for_previous_kernel();  // the costs
   let_next_kernel_start();
 
@@ -614,7 +652,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
     // orders them before its instructions' reads).
     auto copy_rows = [&](const int64_t* at, uint64_t data) -> bool {
       constexpr int kPieces = DP / 8;
-      if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, failed)) return false;
+      if (!bar_wait(&sh.kv_empty[stage_no % S::kStages], (stage_no / S::kStages & 1) ^ 1, watch)) return false;
       const int piece = tid % kPieces;
       const bool there = piece * 8 < int(c.head_dim);
       const uint32_t base = smem_u32(sh.kv[stage_no % S::kStages]) + (piece >> 3) * 16384;
@@ -647,7 +685,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
     constexpr int kCodeRows = kLoadThreads / kCodePieces;
     constexpr int kCodeLoads = (kTileKeys + kCodeRows - 1) / kCodeRows;
     auto copy_codes = [&](uint32_t stage, const int64_t* at, uint64_t data) -> bool {
-      const bool free = bar_wait(&sh.kv_empty[stage % S::kStages], (stage / S::kStages & 1) ^ 1, failed);
+      const bool free = bar_wait(&sh.kv_empty[stage % S::kStages], (stage / S::kStages & 1) ^ 1, watch);
       if (free) {
         const int piece = tid % kCodePieces;
         const bool there = piece * 16 < int(c.head_dim);
@@ -737,7 +775,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       if constexpr (S::kQuant) load_scales(it.unit0);
 
       // Q: the rows' places first, a thread for each; then 16-byte pieces, neighbouring threads on one row.
-      ok = loaders_agree<kLoadThreads>(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, failed));
+      ok = loaders_agree<kLoadThreads>(bar_wait(&sh.q_empty, (item_no & 1) ^ 1, watch));
       if (!ok) break;
       for (int r = tid; r < kTileRows; r += kLoadThreads) {
         const int32_t row = it.row0 + r, i = row / it.group;
@@ -828,13 +866,14 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           if constexpr (S::kQuant) {
             info.key_scale[x] = ks[u];
             const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs[u]) & 0x7fffffffu);
-            if (lane == 0) sh.warp_max[tile_no & 1][x >> 5] = top;
+            const uint32_t low = __reduce_min_sync(0xffffffffu, b < 0 ? 0x7f800000u : __float_as_uint(vs[u]) & 0x7fffffffu);
+            if (lane == 0) sh.warp_max[tile_no & 1][x >> 5] = top, sh.warp_min[tile_no & 1][x >> 5] = low;
           }
         }
       };
       auto prepare = [&](int32_t unit) -> bool {
         KeyInfo& info = sh.info[tile_no % kInfos];
-        ok = ok && bar_wait(&sh.info_empty[tile_no % kInfos], (tile_no / kInfos & 1) ^ 1, failed);
+        ok = ok && bar_wait(&sh.info_empty[tile_no % kInfos], (tile_no / kInfos & 1) ^ 1, watch);
         const uint32_t seen = __ballot_sync(0xffffffffu, block[0] >= 0);
         if (lane == 0 && tid < kTileKeys) info.seen[tid >> 5] = seen;
         if (tid < kTileKeys - kLoadThreads) {
@@ -854,7 +893,12 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           for (int u = 0; u < 2; ++u) {
             if (tid + u * kLoadThreads < kTileKeys) info.value_scale[tid + u * kLoadThreads] = vs[u] * v_inv;
           }
-          if (tid == 0) info.v_exp = v_exp;
+          if (tid == 0) {
+            info.v_exp = v_exp;
+            const uint32_t* low = sh.warp_min[tile_no & 1];
+            info.top_scale = __uint_as_float(max(max(w[0], w[1]), max(w[2], w[3]))) * v_inv;
+            info.low_scale = __uint_as_float(min(min(low[0], low[1]), min(low[2], low[3]))) * v_inv;
+          }
         }
         bar_arrive(&sh.info_full[tile_no % kInfos]);
         return true;
@@ -862,7 +906,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       // A whole tile of one side by TMA: the thread that has a box's first token issues it.
       auto load_boxes = [&](int32_t unit, const CUtensorMap& map) -> bool {
         const uint32_t stage = stage_no++ % S::kStages;
-        if (!bar_wait(&sh.kv_empty[stage], ((stage_no - 1) / S::kStages & 1) ^ 1, failed)) return false;
+        if (!bar_wait(&sh.kv_empty[stage], ((stage_no - 1) / S::kStages & 1) ^ 1, watch)) return false;
         uint32_t mine = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -941,7 +985,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       ++item_no;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (*reinterpret_cast<volatile int*>(failed)) {  // boxes that nobody waits for any more
+    if (*reinterpret_cast<volatile int*>(&watch->failed)) {  // boxes that nobody waits for any more
       for (uint32_t n = stage_no > S::kStages ? stage_no - S::kStages : 0; n < stage_no; ++n) {
         bar_wait(&sh.kv_full[n % S::kStages], n / S::kStages & 1, &sh.stuck[1]);
       }
@@ -954,7 +998,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
     // A stage is there. What copies wrote (no box, no store with a fence of its own) is ordered before what the
     // products read.
     auto filled = [&](uint32_t stage, uint32_t info) {
-      const bool ok = bar_wait_warp(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, failed);
+      const bool ok = bar_wait_warp(&sh.kv_full[stage % S::kStages], stage / S::kStages & 1, watch);
       if constexpr (!S::kQuant) {
         if (!sh.info[info % kInfos].boxed) fence_async_shared();
       }
@@ -1013,8 +1057,8 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       if (!(ok = filled(v, info_no))) return;
       auto half = [&](auto which) -> bool {
         constexpr int h = decltype(which)::value;
-        if (!bar_wait_warp(&sh.p_full[h], tile_no[h]++ & 1, failed)) return false;
-        if (j == 0 && !bar_wait_warp(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, failed)) return false;
+        if (!bar_wait_warp(&sh.p_full[h], tile_no[h]++ & 1, watch)) return false;
+        if (j == 0 && !bar_wait_warp(&sh.o_free[h], (o_no[h]++ & 1) ^ 1, watch)) return false;
         tmem_after_sync();
         sums(which, Value{}, j > 0);
         if (j + 1 < units) {
@@ -1036,7 +1080,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
     while (ok && walk.next(it)) {
       halves = it.rows > 128 ? 2 : 1;
       units = it.unit1 - it.unit0;
-      if (!(ok = bar_wait_warp(&sh.q_full, item_no & 1, failed))) break;
+      if (!(ok = bar_wait_warp(&sh.q_full, item_no & 1, watch))) break;
       if constexpr (!S::kQuant) fence_async_shared();
       for (int32_t j = 0; j < units && ok; ++j) {
         if (stage_no & 2) {
@@ -1066,15 +1110,16 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       RowState sm{-INFINITY, 0.0f};
       float f = factor;
       uint32_t v_exp = 1;
+      float seen_scale = 0.0f;  // the largest V scale that the row sees, in units of 2^(v_exp - 127)
       for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
         KeyInfo& info = sh.info[tile_no % kInfos];
-        if (!(ok = bar_wait_warp(&sh.info_full[tile_no % kInfos], tile_no / kInfos & 1, failed))) break;
+        if (!(ok = bar_wait_warp(&sh.info_full[tile_no % kInfos], tile_no / kInfos & 1, watch))) break;
         if (!active) {
           bar_arrive(&sh.info_empty[tile_no % kInfos]);
           continue;
         }
         if (unit == it.unit0) f = fmaxf(factor * sh.q_unit[item_no & 1][r], 1.2e-38f);
-        if (!(ok = bar_wait_warp(&sh.s_full[h], s_no & 1, failed))) break;
+        if (!(ok = bar_wait_warp(&sh.s_full[h], s_no & 1, watch))) break;
         ++s_no;
         tmem_after_sync();
         const int32_t j0 = it.begin + unit * kTileKeys;
@@ -1084,9 +1129,12 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
         if constexpr (S::kQuant) {
           const uint32_t e = info.v_exp;
           if (e > v_exp) {
-            rescale_sums(o_at, o_columns, e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23));
+            const float by = e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
+            rescale_sums(o_at, o_columns, by);
+            seen_scale *= by;
             v_exp = e;
           }
+          seen_scale = fmaxf(seen_scale, masked ? largest_seen(info, row_lo - j0, row_hi - j0) : info.top_scale);
         }
         if (masked) {
           row_weights<S::kQuant, S::kQuant && !S::kScaledValues, S::kBf16, true>(sm, info, s_at, o_at, o_columns, row_lo - j0, row_hi - j0, f);
@@ -1101,7 +1149,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       ++item_no;
       if (!ok) break;
       if (!active) continue;
-      if (!(ok = bar_wait_warp(&sh.o_full[h], o_no & 1, failed))) break;
+      if (!(ok = bar_wait_warp(&sh.o_full[h], o_no & 1, watch))) break;
       ++o_no;
       tmem_after_sync();
       const float m = sm.m, l = sm.l;
@@ -1114,7 +1162,8 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
                     int64_t(max(it.slot, 0)) * kTileRows * (DP + 2) + r;
       const float times = it.slot >= 0 ? v_unit : l == 0.0f ? 0.0f : v_unit / l;
-      bool bad = false;
+      // And rows whose V scales are far below one that they do not see: it has set the power of two.
+      bool bad = S::kQuant && v_exp > 9 && seen_scale > 0.0f && seen_scale < 1.0f / 4096;
 #pragma unroll 1
       for (int piece = 0; piece < DP / 32; ++piece) {
         uint32_t s[32];
@@ -1164,7 +1213,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
         float4 v;
         attend_row_exactly<Q, STORE>(k, it.seq, token_r, uint32_t(qh_r), uint32_t(it.head),
                                      max(it.begin + it.unit0 * kTileKeys, kv_row_begin(k, it.s, i_r)),
-                                     min(it.begin + it.unit1 * kTileKeys, kv_row_end(k, it.s, i_r)), m_r, l_r, v);
+                                     min(it.begin + it.unit1 * kTileKeys, kv_row_end(k, it.s, i_r)), m_r, l_r, v, &sh.watch.alive);
         if (it.slot >= 0) {
           float* to = reinterpret_cast<float*>(reinterpret_cast<char*>(k.a.workspace) + plan.parts_at) +
                       int64_t(it.slot) * kTileRows * (DP + 2) + (r & ~31) + src;
@@ -1191,7 +1240,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
   }
   __syncthreads();
   if (warp == kMmaWarp) {
-    if (sh.failed) kv_flag(reinterpret_cast<int32_t*>(k.a.status), PF_KV_TIMED_OUT);
+    if (sh.watch.failed) kv_flag(reinterpret_cast<int32_t*>(k.a.status), PF_KV_TIMED_OUT);
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem));
   }
 }

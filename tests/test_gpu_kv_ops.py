@@ -502,6 +502,88 @@ def test_attention_ignores_what_is_masked(cuda, pattern, bad, store):
         at += n
 
 
+@pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8"), ("fp16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("pattern", ["verify", "chunk", "prefill", "mixed"])
+@pytest.mark.parametrize("window", [0, 70])
+def test_attention_ignores_masked_scales(cuda, pattern, q_type, store, window):
+    """A V scale 2^60 times the others', at the chunk's last token and (with a window) in front of it: rows that do not
+    see it are as exact as without."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+    page, kw = 16, dict(seed=23, window=window)
+
+    def edit(k, v, ks, vs, table, q):
+        for s, (n, length) in enumerate(zip(counts, lens)):
+            at = {length - 1} | ({max(0, length - n - 69)} if window and n > 1 else set())
+            for j in at:
+                vs[int(table[s, j // page]), j % page] *= 2.0 ** 60
+
+    clean = run_attention(torch, q_type, store, 128, 2, 4, page, counts, lens, **kw)
+    o, lse = run_attention(torch, q_type, store, 128, 2, 4, page, counts, lens, edit=edit, **kw)[:2]
+    tol, tol_l = attend_bound(torch, o.dtype, True, clean[2], clean[4], clean[5], max(lens), 128)
+    at = 0
+    for n, length in zip(counts, lens):
+        # With a window the planted token is the first that query 0 sees: it alone, of those in front of the last.
+        rows = slice(at + (1 if window and length - n - 69 >= 0 else 0), at + n - 1)
+        if not window or length - n - 69 >= 0:
+            assert ((o[rows].double() - clean[2][rows]).abs() <= tol[rows]).all()
+            assert ((lse[rows].double() - clean[3][rows]).abs() <= tol_l[rows] + clean[3][rows].abs() * 2.0 ** -23).all()
+        at += n
+
+
+@pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8")])
+@pytest.mark.parametrize("pattern", ["decode", "decode_long", "verify"])
+def test_attention_scales_of_any_size(cuda, pattern, q_type, store):
+    """V scales over a hundred powers of two: what is far below a row's largest is off by half of fp16's smallest step
+    of that, 2^-25, for each code."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+
+    def edit(k, v, ks, vs, table, q):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        vs *= torch.exp2(torch.randint(-60, 41, vs.shape, generator=g, device="cuda").float())
+
+    o, lse, want, wl, mag, dot, (cache, q, table, q_start, kv_len) = run_attention(
+        torch, q_type, store, 128, 2, 4, 16, counts, lens, seed=29, edit=edit)
+    tol, tol_l = attend_bound(torch, o.dtype, True, want, mag, dot, max(lens), 128)
+    # The largest weight times scale is at most 2^9 of the unit that the steps are of, and at least 1; a row's largest
+    # magnitude has a code of 448 or 127 (a cache row's largest) next to it.
+    tol = tol + max(lens) * 2.0 ** -25 * mag.amax(2, keepdim=True) * 4
+    if o.dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half of its smallest step
+    big = torch.finfo(o.dtype).max
+    on = want.abs() < big
+    assert ((o.double() - want).abs()[on] <= tol[on]).all()
+    assert ((lse.double() - wl).abs() <= tol_l + wl.abs() * 2.0 ** -23).all()
+
+
+def test_attention_waits_for_rows_made_again(cuda):
+    """A NaN that only the last query sees, after a long context: the rows beside it are made again token by token,
+    which takes longer than a wait's limit, and the call neither gives up nor changes them."""
+    torch = cuda
+    from pegaflow_b200 import KVCache, chunk_attention
+
+    heads, group, dim, page, n, length = 8, 4, 128, 16, 2048, 34816
+    g = torch.Generator(device="cuda").manual_seed(31)
+    buf = torch.randn((2, length // page, page, heads, dim), generator=g, device="cuda").half()
+    cache = KVCache(buf[0], buf[1])
+    table = torch.randperm(length // page, generator=g, device="cuda").int()[None]
+    q = torch.randn((n, heads * group, dim), generator=g, device="cuda").half()
+    args = (q, cache, table, torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+            torch.tensor([length], dtype=torch.int32, device="cuda"))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    clean = chunk_attention(*args, status=status)
+    buf[1, table[0, -1].long(), -1] = math.nan
+    dirty = chunk_attention(*args, status=status)
+    assert status.item() == 0
+    assert torch.isnan(dirty[-1]).all()
+    # Both are within the bound of the formula: u |o| and, for weights in fp16, u times the mean magnitude, at most the
+    # largest value there is.
+    u = 2.0 ** -11
+    off = (dirty[:-1].double() - clean[:-1].double()).abs()
+    assert (off <= 2 * (u * clean[:-1].double().abs() + u * 6.5 + 2.0 ** -12)).all()
+
+
 def test_attention_nan_query(cuda):
     """A NaN in one query reaches its own row alone."""
     torch = cuda
