@@ -12,9 +12,9 @@
 // units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
 // 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
 //
-// Warps 0-3 and 4-7: the softmax of the two halves. Three, or seven over an 8-bit
-// cache: load Q, K and V. The last: issues the products. mbarriers order them; every wait is bounded, and one that
-// runs out ends the call with a status bit and no hang.
+// Warps 0-3 and 4-7: the softmax of the two halves. Three, or five over an 8-bit
+// cache: load Q, K and V. The last: issues the products. mbarriers order them; every
+// wait is bounded, and one that runs out ends the call with a status bit and no hang.
 //
 // A tile of 128 16-bit keys comes by TMA, a box of each block, where all 128 are
 // seen and the block size allows it (8 to 128 tokens, or whole tiles); else a row
@@ -75,8 +75,9 @@ struct Tiles {
   // is too fine for the rounding that this costs, and takes them with the weights.
   static constexpr bool kScaledValues = kQuant && Q == PF_DTYPE_BF16;
   static constexpr int kStages = 4;  // two tiles' K and V
-  // 16 bits: 12 warps of 168 registers. 8 bits: expanding codes keeps seven warps busy, so 16 of 128 registers.
-  static constexpr int kLoadWarps = kQuant ? 7 : 3;
+  // 16 bits: 12 warps of 168 registers. 8 bits: expanding codes takes more, 14 warps of 128 (2,048 tokens after 32,768:
+  // 1.49 ms with four, 1.39 with five, 1.45 with six or seven, which take issue slots from the softmax).
+  static constexpr int kLoadWarps = kQuant ? 5 : 3;
   static constexpr int kLoadThreads = kLoadWarps * 32;
   static constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
