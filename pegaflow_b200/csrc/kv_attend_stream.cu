@@ -715,7 +715,7 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   // Parts of equal length: the CTAs run in rounds of as many as fit, each round as long as a part and its start and
   // end (queries, addresses, joining: about 384 tokens' time). Few sequences: one round, whose parts are as short as
   // that leaves them. Many: sequences are rarely equally long, so among splits that are within a tenth of the best
-  // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 315 us in one round, 228 in seven).
+  // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 286 us in one round, 221 in seven).
   const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * p.tiles * k.cache.heads);
   const uint64_t slots = uint64_t(num_sms) * ctas_per_sm(k, p);
   const uint64_t units = (longest + kStreamMinPart - 1) / kStreamMinPart;  // shortest parts

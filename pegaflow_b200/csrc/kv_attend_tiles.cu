@@ -12,9 +12,9 @@
 // units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
 // 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
 //
-// Warps 0-3 and 4-7: the softmax of the two halves. Three, or five over an 8-bit
-// cache: load Q, K and V. The last: issues the products. mbarriers order them; every
-// wait is bounded, and one that runs out ends the call with a status bit and no hang.
+// Warps 0-3 and 4-7: the softmax of the two halves. Three or five: load Q, K and
+// V. The last: issues the products. mbarriers order them; every wait is bounded, and
+// one that runs out ends the call with a status bit and no hang.
 //
 // A tile of 128 16-bit keys comes by TMA, a box of each block, where all 128 are
 // seen and the block size allows it (8 to 128 tokens, or whole tiles); else a row
@@ -26,7 +26,7 @@
 // scores. V's, divided by a power of two that follows the largest, multiply V there
 // where the result is bf16 (two roundings of 2^-11 beside its own of 2^-8), and the
 // fp32 weights where it is fp16 (2.9e-4 off in all, 4.0e-4 the other way, 2.1e-4
-// being its own rounding; 1.80 ms instead of 1.47 for 2,048 tokens after 32,768).
+// being its own rounding; 1.51 ms instead of 1.39 for 2,048 tokens after 32,768).
 // As in the streaming kernel a bf16 query is brought into fp16's range by a power
 // of two for each row.
 #include <cuda.h>
@@ -75,9 +75,11 @@ struct Tiles {
   // is too fine for the rounding that this costs, and takes them with the weights.
   static constexpr bool kScaledValues = kQuant && Q == PF_DTYPE_BF16;
   static constexpr int kStages = 4;  // two tiles' K and V
-  // 16 bits: 12 warps of 168 registers. 8 bits: expanding codes takes more, 14 warps of 128 (2,048 tokens after 32,768:
-  // 1.49 ms with four, 1.39 with five, 1.45 with six or seven, which take issue slots from the softmax).
-  static constexpr int kLoadWarps = kQuant ? 5 : 3;
+  // 12 warps may have 168 registers, 13 to 16 have 128. 16 bits: 12 warps, copying takes few. 8 bits: expanding codes
+  // takes more, and 14 warps are best (2,048 tokens after 32,768: 1.49 ms with four loading, 1.39 with five, 1.45 with
+  // six or seven, which take issue slots from the softmax), but where the softmax has 128 scaled weights in hand:
+  // 128 registers spill there (1.89 ms; with 168 1.51).
+  static constexpr int kLoadWarps = kQuant && (kScaledValues || DP == 64) ? 5 : 3;
   static constexpr int kLoadThreads = kLoadWarps * 32;
   static constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
@@ -123,7 +125,7 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
 // wait of this CTA gave up. Rows made again token by token take their time: as
 // long as they get on, the clock starts anew. Out of line: the kernel waits in
 // some twenty places, and with this in each it is slower (391 us against 358 for
-// 2,048 tokens after 8,192: the code that runs all the time no longer fits).
+// 2,048 tokens after 10,240: the code that runs all the time no longer fits).
 __device__ __noinline__ bool bar_wait_longer(uint64_t* bar, uint32_t parity, Watch* w) {
   volatile int* failed = &w->failed;
   volatile int* alive = &w->alive;
