@@ -5,7 +5,7 @@
 // group) are at most 8 or 16. A CTA takes a part of the tokens for them; its four
 // warps take batches of 32 tokens in turn, each warp on its own: its running
 // maximum, its sums, its accumulators, joined at the end of the part. Parts of a
-// sequence are joined by a second kernel.
+// sequence are joined by their cluster, where they are one, or by a second kernel.
 //
 // Each warp copies its rows (16-byte cp.async, from wherever the block table says)
 // into a ring of its own in shared memory, two steps of 16 tokens ahead: with 8 to
@@ -74,6 +74,20 @@ __device__ __forceinline__ void copy16(void* to, const char* from, const char* v
 
 __device__ __forceinline__ void copy16(void* to, const char* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+
+// A value in the shared memory of another CTA of the cluster.
+__device__ __forceinline__ float load_of(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
+               : "=f"(v)
+               : "r"(uint32_t(__cvta_generic_to_shared(p))), "r"(rank)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_meets() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -150,12 +164,14 @@ struct Stream {
     Staged staged[kWarps][2][kBatch];
     float m[kWarps][kRows];
     float l[kWarps][kRows];
+    float part_m[kRows];  // the CTA's own, for the others of its cluster
+    float part_l[kRows];
     int bad[kRows];
   };
   static_assert(sizeof(Step) * kRing >= kRows * DP * 4, "a warp's sums fit into its ring");
 };
 
-template <uint32_t Q, uint32_t STORE, int DP, int NT>
+template <uint32_t Q, uint32_t STORE, int DP, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     kv_attend_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
   using S = Stream<Q, STORE, DP, NT>;
@@ -183,7 +199,9 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     const int32_t per = stream_part_tokens(plan, end - begin);
     const int32_t lo = begin + int32_t(part) * per;
     const int32_t hi = min(end, lo + per);
-    if (part && lo >= end) continue;
+    if constexpr (!CLUSTER) {
+      if (part && lo >= end) continue;
+    }
 
     const char* key_base = reinterpret_cast<const char*>(c.key.data);
     const char* value_base = reinterpret_cast<const char*>(c.value.data);
@@ -513,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     auto finish = [&](int32_t r, uint32_t d, float top, float sum, float value) {
       const int32_t i = r / group, qh = int32_t(head) * group + r - i * group;
       const int64_t token = int64_t(s.first) + i, id = token * k.a.q_heads + qh;
-      if (used == 1) {
+      if (CLUSTER || used == 1) {
         const float y = sum == 0.0f ? 0.0f : value / sum;
         if (d < c.head_dim) {
           reinterpret_cast<T*>(k.a.out.data)[token * k.a.out.token_stride + int64_t(qh) * k.a.out.head_stride + d] = kv_from_float<Q>(y);
@@ -525,6 +543,15 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         float* ws = reinterpret_cast<float*>(k.a.workspace) + (id * plan.parts + part) * (DP + 4);
         ws[4 + d] = value;
         if (d == 0) ws[0] = top, ws[1] = sum;
+      }
+    };
+    // What the CTA has of a row: for its cluster into the place of the first warp's share, or done with.
+    auto leave = [&](int32_t row, uint32_t d, float top, float sum, float value) {
+      if constexpr (CLUSTER) {
+        sh.o[0][row * DP + int32_t(d)] = value;
+        if (d == 0) sh.part_m[row] = top, sh.part_l[row] = sum;
+      } else {
+        finish(row0 + row, d, top, sum, value);
       }
     };
     for (int32_t e = threadIdx.x; e < S::kRows * DP; e += kThreads) {
@@ -544,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       if (uneven && sum == sum && !isfinite(value)) {
         sh.bad[row] = 1;
       } else {
-        finish(row0 + row, d, top, sum, value);
+        leave(row, d, top, sum, value);
       }
     }
     if (uneven) {
@@ -557,12 +584,39 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         attend_row_exactly<Q, STORE>(k, seq, int64_t(s.first) + i, head * group + uint32_t(r - i * group), head,
                                      max(lo, kv_row_begin(k, s, i)), min(hi, kv_row_end(k, s, i)), top, sum, v, nullptr);
         if (lane * 4 < DP) {
-          finish(r, lane * 4, top, sum, v.x);
-          finish(r, lane * 4 + 1, top, sum, v.y);
-          finish(r, lane * 4 + 2, top, sum, v.z);
-          finish(r, lane * 4 + 3, top, sum, v.w);
+          leave(row, lane * 4, top, sum, v.x);
+          leave(row, lane * 4 + 1, top, sum, v.y);
+          leave(row, lane * 4 + 2, top, sum, v.z);
+          leave(row, lane * 4 + 3, top, sum, v.w);
         }
       }
+    }
+    if constexpr (CLUSTER) {
+      // Joins the cluster's parts: weights 2^(m_part - max) over their sums, a share of the rows' values for each CTA.
+      cluster_meets();
+      for (int32_t e = int32_t(part) * kThreads + int32_t(threadIdx.x); e < S::kRows * DP; e += int32_t(plan.parts) * kThreads) {
+        const int32_t row = e / DP;
+        if (row0 + row >= rows) break;
+        float m_of[kStreamMaxCluster], l_of[kStreamMaxCluster], o_of[kStreamMaxCluster], top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < int(kStreamMaxCluster); ++p) {
+          m_of[p] = p < used ? load_of(&sh.part_m[row], p) : -INFINITY;
+          l_of[p] = p < used ? load_of(&sh.part_l[row], p) : 0.0f;
+          o_of[p] = p < used ? load_of(&sh.o[0][e], p) : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < int(kStreamMaxCluster); ++p) top = fmaxf(top, m_of[p]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int p = 0; p < int(kStreamMaxCluster); ++p) {
+          const float by = exp2f(m_of[p] - base);
+          sum += l_of[p] * by;
+          value += o_of[p] * by;
+        }
+        finish(row0 + row, uint32_t(e % DP), top, sum, value);
+      }
+      cluster_meets();  // shared memory is read by the others until here
     }
     __syncthreads();  // shared memory is used again by the next tile
   }
@@ -658,14 +712,27 @@ uint32_t ctas_per_sm(const KvAttendArgs& k, const KvStreamPlan& p) {
   return row == 256 ? 2 : p.row_tiles == 1 ? 4 : 2;
 }
 
-template <uint32_t Q, uint32_t STORE, int DP, int NT>
+template <uint32_t Q, uint32_t STORE, int DP, int NT, bool CLUSTER>
 cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
   using S = Stream<Q, STORE, DP, NT>;
-  const auto kernel = kv_attend_stream_kernel<Q, STORE, DP, NT>;
+  const auto kernel = kv_attend_stream_kernel<Q, STORE, DP, NT, CLUSTER>;
   const int shm = int(sizeof(typename S::Shared));
   if (shm > 48 * 1024) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shm);
     if (err != cudaSuccess) return err;
+  }
+  if constexpr (CLUSTER) {
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = 1, cluster.val.clusterDim.y = p.parts, cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(k.a.n_seqs * p.tiles * k.cache.heads, p.parts);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = shm;
+    cfg.stream = stream;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, k, p);
   }
   kernel<<<dim3(k.a.n_seqs * p.tiles * k.cache.heads, p.parts), kThreads, shm, stream>>>(k, p);
   if (p.parts == 1) return cudaGetLastError();
@@ -685,10 +752,13 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t
 
 template <uint32_t Q, uint32_t STORE>
 cudaError_t launch_dims(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t stream) {
+  const bool c = p.clusters;
   if (k.cache.head_dim <= 64) {
-    return p.row_tiles == 1 ? launch_as<Q, STORE, 64, 1>(k, p, stream) : launch_as<Q, STORE, 64, 2>(k, p, stream);
+    if (p.row_tiles == 1) return c ? launch_as<Q, STORE, 64, 1, true>(k, p, stream) : launch_as<Q, STORE, 64, 1, false>(k, p, stream);
+    return c ? launch_as<Q, STORE, 64, 2, true>(k, p, stream) : launch_as<Q, STORE, 64, 2, false>(k, p, stream);
   }
-  return p.row_tiles == 1 ? launch_as<Q, STORE, 128, 1>(k, p, stream) : launch_as<Q, STORE, 128, 2>(k, p, stream);
+  if (p.row_tiles == 1) return c ? launch_as<Q, STORE, 128, 1, true>(k, p, stream) : launch_as<Q, STORE, 128, 1, false>(k, p, stream);
+  return c ? launch_as<Q, STORE, 128, 2, true>(k, p, stream) : launch_as<Q, STORE, 128, 2, false>(k, p, stream);
 }
 
 template <uint32_t Q>
@@ -731,11 +801,15 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   per = std::min(per, units);
   p.part_tokens = static_cast<int32_t>(std::min<uint64_t>(per * kStreamMinPart, 1u << 30));
   p.parts = static_cast<uint32_t>((longest + p.part_tokens - 1) / p.part_tokens);
+  // Up to eight parts that all run at once are a cluster and joined by it, without a second launch (one sequence of
+  // 1,000 tokens: 7.1 us instead of 7.7, eight of 4,000: 21.8 instead of 22.9). In several rounds a cluster waits for
+  // room for all of its parts (16 sequences of 100 to 8,000 tokens: 70 us instead of 50).
+  p.clusters = p.parts > 1 && p.parts <= kStreamMaxCluster && items * p.parts <= slots;
   return p;
 }
 
 uint64_t stream_workspace(const KvAttendArgs& k, const KvStreamPlan& p) {
-  if (p.parts == 1) return 0;
+  if (p.parts == 1 || p.clusters) return 0;
   const uint64_t dp = k.cache.head_dim <= 64 ? 64 : 128;
   return k.a.n_tokens * k.a.q_heads * p.parts * (dp + 4) * sizeof(float);
 }

@@ -11,6 +11,7 @@ namespace pf {
 
 constexpr uint32_t kStreamMaxRows = 16;  // queries times heads of a group that one CTA takes
 constexpr uint32_t kStreamMaxParts = 32768;  // a grid's y axis ends at 65,535
+constexpr uint32_t kStreamMaxCluster = 8;  // parts that a cluster's CTAs join among themselves
 constexpr uint32_t kStreamMinPart = 128;  // tokens: a batch for each warp
 
 struct KvStreamPlan {
@@ -19,6 +20,7 @@ struct KvStreamPlan {
   uint32_t parts;       // CTAs along the tokens
   int32_t part_tokens;  // tokens of a part, a multiple of kStreamMinPart
   int32_t page_shift;   // log2 of the block size, -1 if it is no power of two
+  uint32_t clusters;    // a sequence's parts are a cluster, which joins them
 };
 
 // Tokens of each part when `range` tokens are to be covered, and how many parts
