@@ -6,6 +6,8 @@
 // warps take batches of 32 tokens in turn, each warp on its own: its running
 // maximum, its sums, its accumulators, joined at the end of the part. Parts of a
 // sequence are joined by their cluster, where they are one, or by a second kernel.
+// Measured: 64 sequences of 1K to 16K tokens, 32 heads on 8 of 128 over e4m3, 1.2 GB,
+// 221 us (5.4 TB/s); one of 1,000 in bf16 7.0 us, which are latency.
 //
 // Each warp copies its rows (16-byte cp.async, from wherever the block table says)
 // into a ring of its own in shared memory, two steps of 16 tokens ahead: with 8 to
