@@ -159,10 +159,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Watch* 
 __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, Watch* watch) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, watch));
 }
-// Meets the other loading threads; whether all of them say yes.
+// Meets the other loading threads; whether all of them say yes. A warp arrives as
+// one (.aligned), and its lanes may come from waits that they left at different
+// times.
 template <int THREADS>
 __device__ __forceinline__ bool loaders_agree(bool ok) {
   uint32_t all;
+  __syncwarp();
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
       : "=r"(all)
