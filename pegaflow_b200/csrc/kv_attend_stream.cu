@@ -198,9 +198,8 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     const int32_t row_last = min(rows, row0 + S::kRows) - 1;
     const int32_t begin = kv_row_begin(k, s, row0 / group);
     const int32_t end = kv_row_end(k, s, row_last / group);
-    const int32_t per = stream_part_tokens(plan, end - begin);
-    const int32_t lo = begin + int32_t(part) * per;
-    const int32_t hi = min(end, lo + per);
+    const KvPart span = stream_part(plan, begin, end, part);
+    const int32_t lo = span.lo, hi = span.hi;
     if constexpr (!CLUSTER) {
       if (part && lo >= end) continue;
     }
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         }
       }
     };
-    const int32_t batches = (max(0, hi - lo) + kBatch - 1) / kBatch;
+    const int32_t batches = (hi - lo + kBatch - 1) / kBatch;
     // This warp's batches: warp, warp + 4, ...; step i is half of its batch i / 2.
     const int32_t mine = warp < batches ? (batches - warp + kWarps - 1) / kWarps : 0;
     typename S::Step* ring = sh.ring[warp];

@@ -30,8 +30,19 @@ __host__ __device__ inline int32_t stream_part_tokens(const KvStreamPlan& p, int
   return p.part_tokens > least ? p.part_tokens : least;
 }
 __host__ __device__ inline int32_t stream_parts(const KvStreamPlan& p, int32_t range) {
-  const int32_t per = stream_part_tokens(p, range);
-  return range <= per ? 1 : (range + per - 1) / per;
+  const int64_t per = stream_part_tokens(p, range);
+  return range <= per ? 1 : int32_t((range + per - 1) / per);
+}
+
+// The tokens [lo, hi) of a part; empty ones end where the range does. In 64 bits:
+// a part may be millions of tokens long and the range end close to 2^31.
+struct KvPart {
+  int32_t lo;
+  int32_t hi;
+};
+__host__ __device__ inline KvPart stream_part(const KvStreamPlan& p, int32_t begin, int32_t end, uint32_t part) {
+  const int64_t per = stream_part_tokens(p, end - begin), lo = begin + int64_t(part) * per, hi = lo + per;
+  return KvPart{int32_t(lo < end ? lo : end), int32_t(hi < end ? hi : end)};
 }
 
 KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms);
