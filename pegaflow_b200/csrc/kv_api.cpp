@@ -62,7 +62,7 @@ void check_attention(const pf_kv_cache& c, const pf_kv_attention& a) {
   if (c.head_dim % 16 || c.head_dim > kKvMaxAttentionDim) refuse("attention head_dim must be a multiple of 16 up to 128");
   if (!a.q_heads || a.q_heads % c.heads) refuse("query heads must be a multiple of the cache's heads");
   if (a.q_heads > (1u << 16)) refuse("query heads out of range");
-  if (a.n_tokens > INT32_MAX / 2 || a.n_tokens * a.q_heads > INT32_MAX) refuse("too many query tokens");
+  if (a.n_tokens > INT32_MAX / 2 || a.n_tokens * a.q_heads > kKvMaxRows) refuse("too many query tokens");
   if (uint64_t(a.n_seqs) * c.heads > INT32_MAX / 2 || a.max_blocks > INT32_MAX) refuse("too many sequences or blocks");
   if (uint64_t(a.max_blocks) * c.block_size > kKvMaxTokens) refuse("block table names more tokens than an int32 can count");
   if (!std::isfinite(a.scale)) refuse("scale must be finite");

@@ -14,6 +14,8 @@ constexpr uint32_t kKvMaxHeadDim = 256;
 constexpr uint32_t kKvMaxAttentionDim = 128;
 // Tokens that a block table's row may name: positions rounded up to tiles still fit an int32.
 constexpr uint64_t kKvMaxTokens = (1ull << 31) - (1ull << 16);
+// Query rows (tokens times heads) of a call: rounded up to tiles they still fit one as well.
+constexpr uint64_t kKvMaxRows = (1ull << 31) - (1ull << 16);
 // Smallest scale a quantised row gets: the smallest normal fp32, so that 1 /
 // scale is finite and a row of zeros stores zeros.
 constexpr float kKvSmallestScale = 1.17549435e-38f;
