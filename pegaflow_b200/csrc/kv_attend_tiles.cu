@@ -491,7 +491,8 @@ __device__ __noinline__ float largest_seen(const KeyInfo& info, int32_t lo, int3
 }
 
 // Multiplies a row's fp32 values, or pairs of 16-bit ones, in TMEM: rarely done,
-// so out of the way.
+// so out of the way. Loads and stores of TMEM keep no order among themselves: the
+// caller has waited for its own of both (tmem_wait_load, tmem_wait_store).
 __device__ __noinline__ void rescale_sums(uint32_t at, int columns, float by) {
 #pragma unroll 1
   for (int x = 0; x < columns; x += 32) {
@@ -587,6 +588,10 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
     const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
     const bool raise = top > (row.m == -INFINITY ? -INFINITY : kRaise);  // a NaN raises nothing: it reaches the sum
     if (__any_sync(0xffffffffu, raise)) {
+      // What is read back below was stored asynchronously (weights of pieces before, O by a rescaling), and the next
+      // scores are still on their way into registers that a call may save: both are waited for first.
+      tmem_wait_load(s);
+      tmem_wait_store();
       float keep = 1.0f;
       if (raise) {
         const float m = base + top;
