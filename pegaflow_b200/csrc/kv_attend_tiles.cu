@@ -472,6 +472,12 @@ __device__ __forceinline__ uint32_t seen_bits(const KeyInfo& info, int piece, in
   return info.seen[piece] & below_to & ~below_from;
 }
 
+// A scale in other units, y, that keeps a trace (and its sign) where it becomes too
+// small for them: what a row sees of V scales is nothing only if all of them are zero.
+__device__ __forceinline__ float still_there(float x, float y) {
+  return x != 0.0f && fabsf(y) < kKvSmallestScale ? copysignf(kKvSmallestScale, x) : y;
+}
+
 // The largest V scale among the tokens that the row sees, or, if all of the tile
 // are within 2^4, the smallest there is.
 __device__ __noinline__ float largest_seen(const KeyInfo& info, int32_t lo, int32_t hi) {
@@ -904,13 +910,15 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           const float v_inv = __uint_as_float((254 - v_exp) << 23);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            if (tid + u * kLoadThreads < kTileKeys) info.value_scale[tid + u * kLoadThreads] = vs[u] * v_inv;
+            if (tid + u * kLoadThreads < kTileKeys) info.value_scale[tid + u * kLoadThreads] = still_there(vs[u], vs[u] * v_inv);
           }
           if (tid == 0) {
             info.v_exp = v_exp;
             const uint32_t* low = sh.warp_min[tile_no & 1];
-            info.top_scale = __uint_as_float(max(max(w[0], w[1]), max(w[2], w[3]))) * v_inv;
-            info.low_scale = __uint_as_float(min(min(low[0], low[1]), min(low[2], low[3]))) * v_inv;
+            const float top_scale = __uint_as_float(max(max(w[0], w[1]), max(w[2], w[3])));
+            const float low_scale = __uint_as_float(min(min(low[0], low[1]), min(low[2], low[3])));
+            info.top_scale = still_there(top_scale, top_scale * v_inv);
+            info.low_scale = still_there(low_scale, low_scale * v_inv);
           }
         }
         bar_arrive(&sh.info_full[tile_no % kInfos]);
@@ -1144,7 +1152,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           if (e > v_exp) {
             const float by = e - v_exp > 126 ? 0.0f : __uint_as_float((127 - (e - v_exp)) << 23);
             rescale_sums(o_at, o_columns, by);
-            seen_scale *= by;
+            seen_scale = still_there(seen_scale, seen_scale * by);
             v_exp = e;
           }
           seen_scale = fmaxf(seen_scale, masked ? largest_seen(info, row_lo - j0, row_hi - j0) : info.top_scale);

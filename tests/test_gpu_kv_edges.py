@@ -66,3 +66,41 @@ def test_attention_rises_within_tiles(cuda, pattern, dim, step, q_type, store):
 
     got = run_attention(torch, q_type, store, dim, 2, 4, page, counts, lens, seed=43, edit=edit)
     check_attention(torch, got, dim, max(lens), store in QMAX)
+
+
+# ------------------------------------------------------- V scales of any size
+
+@pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8"), ("fp16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("pattern", ["verify", "chunk", "prefill", "mixed"])
+@pytest.mark.parametrize("small", [2.0 ** -6, 2.0 ** -26])
+def test_attention_ignores_masked_scales_of_any_size(cuda, pattern, q_type, store, small):
+    """A V scale of 2^119 at the chunk's last token, 2^132 (2^152) times the others': more than an exponent's range away,
+    in the same tile of keys as some rows' ends and in a later one than others'. Rows that do not see it are as exact
+    as without."""
+    torch = cuda
+    if q_type == "fp16" and small < 2.0 ** -10:
+        small *= 2.0 ** 12  # fp16 holds no smaller results
+    counts, lens = PATTERNS[pattern]
+    page, kw = 16, dict(seed=45)
+
+    def shrink(k, v, ks, vs, table, q):
+        vs.mul_(small)
+
+    def edit(k, v, ks, vs, table, q):
+        shrink(k, v, ks, vs, table, q)
+        for s, length in enumerate(lens):
+            if length:
+                vs[int(table[s, (length - 1) // page]), (length - 1) % page] = 2.0 ** 119
+
+    clean = run_attention(torch, q_type, store, 128, 2, 4, page, counts, lens, edit=shrink, **kw)
+    o, lse = run_attention(torch, q_type, store, 128, 2, 4, page, counts, lens, edit=edit, **kw)[:2]
+    tol, tol_l = attend_bound(torch, o.dtype, True, clean[2], clean[4], clean[5], max(lens), 128)
+    if o.dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half of its smallest step
+    at = 0
+    for n in counts:
+        rows = slice(at, at + max(0, n - 1))
+        assert ((o[rows].double() - clean[2][rows]).abs() <= tol[rows]).all()
+        far = torch.where(torch.isinf(clean[3][rows]), 0.0, (lse[rows].double() - clean[3][rows]).abs())
+        assert (far <= tol_l[rows] + clean[3][rows].abs().nan_to_num(posinf=0) * 2.0 ** -23).all()
+        at += n
