@@ -57,7 +57,15 @@ struct alignas(16) KeyInfo {
   uint32_t boxed;             // came by TMA
   float top_scale;            // the largest of value_scale
   float low_scale;            // and the smallest, of tokens that are there
+  uint32_t far;               // one of them is below kFarScale, and of more than zeros
 };
+
+// A V scale, or a weight times it, below this share of the unit is no normal fp16 number:
+// it is off by up to 2^-25, and so a value of 448 codes by 2^-16.2.
+constexpr float kFarScale = 1.0f / 16384;
+// Rows that have such and whose largest value is below this (for each unit of their weights, or for each token where
+// the weights are scaled) are made again: what is left is off by 2^-11 of that value at most.
+constexpr float kSmallRow = 1.0f / 32;
 
 struct Watch {
   int failed;  // a wait gave up
@@ -899,7 +907,10 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           const uint32_t last = __ballot_sync(0xffffffffu, block[1] >= 0);
           if (lane == 0) info.seen[kLoadThreads / 32] = last;
         }
-        if constexpr (S::kQuant) offsets(unit, info);
+        if constexpr (S::kQuant) {
+          offsets(unit, info);
+          if (tid == 0) info.far = 0;
+        }
         // Meeting here also keeps the slots apart: who writes a slot again (kInfos tiles on; warp_max: two) has
         // met those who read it last.
         ok = loaders_agree<kLoadThreads>(ok);
@@ -910,7 +921,12 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
           const float v_inv = __uint_as_float((254 - v_exp) << 23);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            if (tid + u * kLoadThreads < kTileKeys) info.value_scale[tid + u * kLoadThreads] = still_there(vs[u], vs[u] * v_inv);
+            if (tid + u * kLoadThreads < kTileKeys) {
+              const float in_units = still_there(vs[u], vs[u] * v_inv);
+              info.value_scale[tid + u * kLoadThreads] = in_units;
+              // The smallest scale that a row is written with is that of zeros.
+              if (fabsf(in_units) < kFarScale && fabsf(vs[u]) > kKvSmallestScale) info.far = 1;
+            }
           }
           if (tid == 0) {
             info.v_exp = v_exp;
@@ -1132,6 +1148,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       float f = factor;
       uint32_t v_exp = 1;
       float seen_scale = 0.0f;  // the largest V scale that the row sees, in units of 2^(v_exp - 127)
+      bool far = false;         // a tile held scales far below the unit of its time
       for (int32_t unit = it.unit0; unit < it.unit1; ++unit, ++tile_no) {
         KeyInfo& info = sh.info[tile_no % kInfos];
         if (!(ok = bar_wait_warp(&sh.info_full[tile_no % kInfos], tile_no / kInfos & 1, watch))) break;
@@ -1156,6 +1173,7 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
             v_exp = e;
           }
           seen_scale = fmaxf(seen_scale, masked ? largest_seen(info, row_lo - j0, row_hi - j0) : info.top_scale);
+          far = far || info.far;
         }
         if (masked) {
           row_weights<S::kQuant, S::kQuant && !S::kScaledValues, S::kBf16, true>(sm, info, s_at, o_at, o_columns, row_lo - j0, row_hi - j0, f);
@@ -1185,11 +1203,16 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       const float times = it.slot >= 0 ? v_unit : l == 0.0f ? 0.0f : v_unit / l;
       // And rows whose V scales are far below one that they do not see: it has set the power of two.
       bool bad = S::kQuant && v_exp > 9 && seen_scale > 0.0f && seen_scale < 1.0f / 4096;
+      float largest = 0.0f;  // of O, where that has to be known
 #pragma unroll 1
       for (int piece = 0; piece < DP / 32; ++piece) {
         uint32_t s[32];
         tmem_load32(s, o_at + piece * 32);
         tmem_wait_load(s);
+        if (S::kQuant && far) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) largest = fmaxf(largest, fabsf(__uint_as_float(s[x])));
+        }
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
           bad = bad || !isfinite(__uint_as_float(s[x]));
@@ -1216,6 +1239,10 @@ __global__ void __launch_bounds__((Tiles<Q, STORE, DP>::kThreads), 1)
       }
       tmem_before_sync();
       bar_arrive(&sh.o_free[h]);
+      // And rows whose result is so small that the rounding of what is far below the unit shows in it.
+      if (S::kQuant && far) {
+        bad = bad || largest < kSmallRow * (S::kScaledValues ? l : float((it.unit1 - it.unit0) * kTileKeys));
+      }
       if (mine) {
         if (it.slot >= 0) {
           part[0] = m, part[kTileRows] = l;

@@ -104,3 +104,62 @@ def test_attention_ignores_masked_scales_of_any_size(cuda, pattern, q_type, stor
         far = torch.where(torch.isinf(clean[3][rows]), 0.0, (lse[rows].double() - clean[3][rows]).abs())
         assert (far <= tol_l[rows] + clean[3][rows].abs().nan_to_num(posinf=0) * 2.0 ** -23).all()
         at += n
+
+
+def scales_bound(torch, o, want, mag, dot, longest):
+    """attend_bound, and what V scales that differ by more than 2^14 cost on top: 2^-11 of the row's largest magnitude."""
+    tol, tol_l = attend_bound(torch, o.dtype, True, want, mag, dot, longest, 128)
+    tol = tol + 2.0 ** -11 * mag.amax(2, keepdim=True)
+    if o.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    return tol, tol_l
+
+
+@pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8"), ("fp16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("pattern", ["chunk", "prefill", "mixed", "short"])
+@pytest.mark.parametrize("window", [0, 90])
+def test_attention_scales_of_any_size_in_chunks(cuda, pattern, q_type, store, window):
+    """V scales over a hundred powers of two, all of them seen."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+
+    def edit(k, v, ks, vs, table, q):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        vs *= torch.exp2(torch.randint(-60, 41, vs.shape, generator=g, device="cuda").float())
+
+    o, lse, want, wl, mag, dot, _ = run_attention(torch, q_type, store, 128, 2, 4, 16, counts, lens, seed=29, edit=edit,
+                                                  window=window)
+    tol, tol_l = scales_bound(torch, o, want, mag, dot, max(lens))
+    # A value that may be off by tol may be anything from want - tol to want + tol: past the type's largest, infinity.
+    on = want.abs() + tol < torch.finfo(o.dtype).max
+    off = (o.double() - want).abs()
+    assert (off[on] <= tol[on]).all(), f"worst {(off / tol)[on].max().item():.2f} of the bound"
+
+
+@pytest.mark.parametrize("ratio", [14, 20, 24, 40, 90])
+@pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8")])
+@pytest.mark.parametrize("pattern", ["chunk", "mixed"])
+def test_attention_far_scale_of_small_weight(cuda, pattern, q_type, store, ratio):
+    """Each sequence's first token, which all of it see, has a V scale 2^ratio times the mean of all (with those planted
+    before it, so they grow from sequence to sequence) and a weight of about e^-90: as long as that is the smaller, the
+    others' values are the result, whatever kernel takes the call."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+
+    def edit(k, v, ks, vs, table, q):
+        q.copy_(q.abs())
+        k.copy_(k.float().abs().to(k.dtype))
+        for s, length in enumerate(lens):
+            b = int(table[s, 0])
+            k[b, 0] = torch.full_like(k[b, 0].float(), -96.0).to(k.dtype)
+            ks[b, 0] = 10.0 / 96.0
+            vs[b, 0] = vs.mean() * 2.0 ** ratio
+
+    for hints in (True, False):
+        o, lse, want, wl, mag, dot, _ = run_attention(torch, q_type, store, 128, 2, 4, 16, counts, lens, seed=30, edit=edit,
+                                                      hints=hints)
+        tol, tol_l = scales_bound(torch, o, want, mag, dot, max(lens))
+        # Rows that see the first token alone have it whole, and fp16 does not hold it then.
+        on = want.abs() + tol < torch.finfo(o.dtype).max
+        off = (o.double() - want).abs()
+        assert (off[on] <= tol[on]).all(), f"worst {(off / tol)[on].max().item():.2f} of the bound"
