@@ -25,10 +25,11 @@
 //
 // 8-bit codes become fp16, which holds all of e4m3 and int8 exactly; the scales
 // stay in fp32: K's multiplies the score, V's the weight. Weights times V's scales
-// are rounded to fp16 for the second product. So the running maximum is that of the
-// score plus the V scale's exponent (2^-63 to 2^63): a row's largest weight times
-// scale is near 1 whatever the scales are, and what the row does not see has no part
-// in it. A bf16
+// are rounded to fp16 for the second product, so they have a running maximum of their
+// own, of the score plus the V scale's exponent, and an exponential of their own: a
+// row's largest weight times scale is near 1 whatever the scales are, what the row
+// does not see has no part in it, and the sum of the weights goes by the scores
+// alone. A bf16
 // query is brought into fp16's range by a power of two for each row: values down
 // to 2^-28 of the row's largest stay exact, smaller ones are off by at most 2^-39
 // of it.
@@ -109,6 +110,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// y times 2^by, in two steps: the power alone may lie outside fp32.
+__device__ __forceinline__ float in_units(float y, float by) {
+  const float half = exp2f(0.5f * by);
+  return y * half * half;
+}
+
 // Two codes in the low (HIGH: high) 16 bits of x as two fp16 values.
 template <uint32_t STORE, bool HIGH>
 __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
@@ -151,10 +158,16 @@ struct Stream {
     unsigned char key[kStep][kRowBytes];
     unsigned char value[kStep][kRowBytes];
   };
-  // The power of two (of a V scale) that the running maximum counts.
-  static __device__ __forceinline__ float exponent(float scale) {
-    if constexpr (!kQuant) return 0.0f;
-    return float(min(max(int(__float_as_uint(scale) >> 23 & 255) - 127, -63), 63));
+  // A V scale as a power of two, which the values' maximum counts, and what is left of it: 1 to 2 (up to 4 from 2^127 on),
+  // less below 2^-126, 0, an infinity or NaN.
+  struct Scale {
+    float exponent;
+    float rest;
+  };
+  static __device__ __forceinline__ Scale split(float scale) {
+    if constexpr (!kQuant) return Scale{0.0f, 1.0f};
+    const int e = min(max(int(__float_as_uint(scale) >> 23 & 255) - 127, -126), 126);
+    return Scale{float(e), scale * __uint_as_float(uint32_t(127 - e) << 23)};
   }
   static __device__ __forceinline__ int key_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row & 1) << 2 : piece; }
   static __device__ __forceinline__ int value_piece(int row, int piece) { return kPieces >= 8 ? piece ^ (row >> 1 & 3) << 1 : piece ^ (row >> 1 & 3); }
@@ -166,8 +179,10 @@ struct Stream {
     Staged staged[kWarps][2][kBatch];
     float m[kWarps][kRows];
     float l[kWarps][kRows];
+    float mv[kWarps][kRows];
     float part_m[kRows];  // the CTA's own, for the others of its cluster
     float part_l[kRows];
+    float part_mv[kRows];
     int bad[kRows];
   };
   static_assert(sizeof(Step) * kRing >= kRows * DP * 4, "a warp's sums fit into its ring");
@@ -343,11 +358,12 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
 
     float o[NT][S::kTiles][4];
     float m[NT][2], l[NT][2];
+    float mv[NT][2];  // what the values go by: the largest score with its V scale's exponent (16 bits: m itself)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < S::kTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = mv[n][0] = mv[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.0f;
     }
 
@@ -366,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       const typename S::Step& now = ring[i % kRing];
       const Staged s0 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g], s1 = sh.staged[warp][i >> 1 & 1][(i & 1) * kStep + g + 8];
 
-      const float e0 = S::exponent(s0.value_scale), e1 = S::exponent(s1.value_scale);
+      const typename S::Scale v0 = S::split(s0.value_scale), v1 = S::split(s1.value_scale);
       // S^T: c0, c1 are token g's scores for the rows 2 t and 2 t + 1, c2, c3 token g + 8's.
       float x[NT][4];
 #pragma unroll
@@ -417,22 +433,31 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        raise = raise || fmaxf(x[n][0] + e0, x[n][2] + e1) > m[n][0] + kRaise || fmaxf(x[n][1] + e0, x[n][3] + e1) > m[n][1] + kRaise;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          raise = raise || fmaxf(x[n][e], x[n][e + 2]) > m[n][e] + kRaise;
+          if constexpr (S::kQuant) raise = raise || fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent) > mv[n][e] + kRaise;
+        }
       }
       if (__any_sync(0xffffffffu, raise)) {
+        // The old maximum's share of the new one's units, which becomes the old one.
+        auto raised = [](float& old, float top) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, old);
+          const float keep = top == -INFINITY ? 0.0f : fast_exp2(old - top);
+          old = top;
+          return keep;
+        };
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float keep[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[n][e] + e0, x[n][e + 2] + e1);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[n][e]);
-            keep[e] = top == -INFINITY ? 0.0f : fast_exp2(m[n][e] - top);
-            m[n][e] = top;
+            keep[e] = raised(m[n][e], fmaxf(x[n][e], x[n][e + 2]));
             l[n][e] *= keep[e];
+            if constexpr (S::kQuant) keep[e] = raised(mv[n][e], fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent));
           }
 #pragma unroll
           for (int y = 0; y < S::kTiles; ++y) {
@@ -449,7 +474,11 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
           const float base = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
           w[e] = fast_exp2(x[n][e] - base);
           l[n][e & 1] += w[e];
-          if constexpr (S::kQuant) w[e] *= e < 2 ? s0.value_scale : s1.value_scale;
+          if constexpr (S::kQuant) {
+            const typename S::Scale& v = e < 2 ? v0 : v1;
+            const float by = mv[n][e & 1] == -INFINITY ? 0.0f : mv[n][e & 1];
+            w[e] = fast_exp2(x[n][e] + v.exponent - by) * v.rest;
+          }
         }
         const uint32_t first = pack2<S::kBf16>(w[0], w[1]), second = pack2<S::kBf16>(w[2], w[3]);
         p[n][0] = transpose_8x8(first);
@@ -513,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         if (g == 0) {
           sh.m[warp][n * 8 + 2 * t + e] = m[n][e];
+          sh.mv[warp][n * 8 + 2 * t + e] = S::kQuant ? mv[n][e] : m[n][e];
           sh.l[warp][n * 8 + 2 * t + e] = sum;
         }
       }
@@ -529,11 +559,12 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
     const int32_t used = stream_parts(plan, end - begin);
     // Rows of one tile see different tokens: an infinity behind one row's end may have met its weight of zero.
     const bool uneven = max(lo, all_lo) > lo || min(hi, all_hi) < hi;
-    auto finish = [&](int32_t r, uint32_t d, float top, float sum, float value) {
+    // Sums of weights are in units of 2^top, of weights times values in units of 2^top_v.
+    auto finish = [&](int32_t r, uint32_t d, float top, float sum, float top_v, float value) {
       const int32_t i = r / group, qh = int32_t(head) * group + r - i * group;
       const int64_t token = int64_t(s.first) + i, id = token * k.a.q_heads + qh;
       if (CLUSTER || used == 1) {
-        const float y = sum == 0.0f ? 0.0f : value / sum;
+        const float y = sum == 0.0f ? 0.0f : S::kQuant ? in_units(value / sum, top_v - top) : value / sum;
         if (d < c.head_dim) {
           reinterpret_cast<T*>(k.a.out.data)[token * k.a.out.token_stride + int64_t(qh) * k.a.out.head_stride + d] = kv_from_float<Q>(y);
         }
@@ -543,36 +574,37 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       } else {
         float* ws = reinterpret_cast<float*>(k.a.workspace) + (id * plan.parts + part) * (DP + 4);
         ws[4 + d] = value;
-        if (d == 0) ws[0] = top, ws[1] = sum;
+        if (d == 0) ws[0] = top, ws[1] = sum, ws[2] = top_v;
       }
     };
     // What the CTA has of a row: for its cluster into the place of the first warp's share, or done with.
-    auto leave = [&](int32_t row, uint32_t d, float top, float sum, float value) {
+    auto leave = [&](int32_t row, uint32_t d, float top, float sum, float top_v, float value) {
       if constexpr (CLUSTER) {
         sh.o[0][row * DP + int32_t(d)] = value;
-        if (d == 0) sh.part_m[row] = top, sh.part_l[row] = sum;
+        if (d == 0) sh.part_m[row] = top, sh.part_l[row] = sum, sh.part_mv[row] = top_v;
       } else {
-        finish(row0 + row, d, top, sum, value);
+        finish(row0 + row, d, top, sum, top_v, value);
       }
     };
     for (int32_t e = threadIdx.x; e < S::kRows * DP; e += kThreads) {
       const int32_t row = e / DP;
       const uint32_t d = uint32_t(e % DP);
       if (row0 + row >= rows) break;
-      float top = sh.m[0][row];
+      float top = sh.m[0][row], top_v = sh.mv[0][row];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.m[w][row]);
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.m[w][row]), top_v = fmaxf(top_v, sh.mv[w][row]);
       float sum = 0.0f, value = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float keep = top == -INFINITY ? 1.0f : exp2f(sh.m[w][row] - top);
+        const float keep_v = !S::kQuant ? keep : top_v == -INFINITY ? 1.0f : exp2f(sh.mv[w][row] - top_v);
         sum += sh.l[w][row] * keep;
-        value += sh.o[w][row * DP + int32_t(d)] * keep;
+        value += sh.o[w][row * DP + int32_t(d)] * keep_v;
       }
       if (uneven && sum == sum && !isfinite(value)) {
         sh.bad[row] = 1;
       } else {
-        leave(row, d, top, sum, value);
+        leave(row, d, top, sum, top_v, value);
       }
     }
     if (uneven) {
@@ -585,10 +617,10 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         attend_row_exactly<Q, STORE>(k, seq, int64_t(s.first) + i, head * group + uint32_t(r - i * group), head,
                                      max(lo, kv_row_begin(k, s, i)), min(hi, kv_row_end(k, s, i)), top, sum, v, nullptr);
         if (lane * 4 < DP) {
-          leave(row, lane * 4, top, sum, v.x);
-          leave(row, lane * 4 + 1, top, sum, v.y);
-          leave(row, lane * 4 + 2, top, sum, v.z);
-          leave(row, lane * 4 + 3, top, sum, v.w);
+          leave(row, lane * 4, top, sum, top, v.x);
+          leave(row, lane * 4 + 1, top, sum, top, v.y);
+          leave(row, lane * 4 + 2, top, sum, top, v.z);
+          leave(row, lane * 4 + 3, top, sum, top, v.w);
         }
       }
     }
@@ -598,24 +630,26 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       for (int32_t e = int32_t(part) * kThreads + int32_t(threadIdx.x); e < S::kRows * DP; e += int32_t(plan.parts) * kThreads) {
         const int32_t row = e / DP;
         if (row0 + row >= rows) break;
-        float m_of[kStreamMaxCluster], l_of[kStreamMaxCluster], o_of[kStreamMaxCluster], top = -INFINITY;
+        float m_of[kStreamMaxCluster], l_of[kStreamMaxCluster], v_of[kStreamMaxCluster], o_of[kStreamMaxCluster];
+        float top = -INFINITY, top_v = -INFINITY;
 #pragma unroll
         for (int p = 0; p < int(kStreamMaxCluster); ++p) {
           m_of[p] = p < used ? load_of(&sh.part_m[row], p) : -INFINITY;
           l_of[p] = p < used ? load_of(&sh.part_l[row], p) : 0.0f;
+          v_of[p] = S::kQuant && p < used ? load_of(&sh.part_mv[row], p) : -INFINITY;
           o_of[p] = p < used ? load_of(&sh.o[0][e], p) : 0.0f;
         }
 #pragma unroll
-        for (int p = 0; p < int(kStreamMaxCluster); ++p) top = fmaxf(top, m_of[p]);
-        const float base = top == -INFINITY ? 0.0f : top;
+        for (int p = 0; p < int(kStreamMaxCluster); ++p) top = fmaxf(top, m_of[p]), top_v = fmaxf(top_v, v_of[p]);
+        const float base = top == -INFINITY ? 0.0f : top, base_v = top_v == -INFINITY ? 0.0f : top_v;
         float sum = 0.0f, value = 0.0f;
 #pragma unroll
         for (int p = 0; p < int(kStreamMaxCluster); ++p) {
           const float by = exp2f(m_of[p] - base);
           sum += l_of[p] * by;
-          value += o_of[p] * by;
+          value += o_of[p] * (S::kQuant ? exp2f(v_of[p] - base_v) : by);
         }
-        finish(row0 + row, uint32_t(e % DP), top, sum, value);
+        finish(row0 + row, uint32_t(e % DP), top, sum, top_v, value);
       }
       cluster_meets();  // shared memory is read by the others until here
     }
@@ -631,7 +665,7 @@ template <uint32_t Q, int DP>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv_join_stream_kernel(const __grid_constant__ KvAttendArgs k, const KvStreamPlan plan) {
   using T = typename KvElem<Q>::type;
   __shared__ float4 values[kJoinWarps][32];
-  __shared__ float sums[kJoinWarps], tops[kJoinWarps];
+  __shared__ float sums[kJoinWarps], tops[kJoinWarps], tops_v[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t id = blockIdx.x;
   const uint32_t token = uint32_t(id / k.a.q_heads), qh = uint32_t(id % k.a.q_heads);
@@ -647,13 +681,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_join_stream_kernel(const _
   wait_for_previous_kernel();
   if (seq == k.a.n_seqs || r >= rows || used == 1) return;
   const float* ws = reinterpret_cast<const float*>(k.a.workspace) + id * plan.parts * (DP + 4);
-  // The warp's own running maximum, then the block's.
-  float top = -INFINITY, sum = 0.0f;
+  // The warp's own running maxima, then the block's.
+  float top = -INFINITY, top_v = -INFINITY, sum = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
   const bool mine = lane * 4 < DP;
 #pragma unroll 1
   for (int32_t p0 = warp; p0 < used; p0 += 4 * kJoinWarps) {
-    float m[4], l[4];
+    float m[4], l[4], mv[4];
     float4 v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -661,41 +695,44 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_join_stream_kernel(const _
       const float* w = ws + int64_t(p) * (DP + 4);
       m[u] = p < used ? w[0] : -INFINITY;
       l[u] = p < used ? w[1] : 0.0f;
+      mv[u] = p < used ? w[2] : -INFINITY;
       v[u] = p < used && mine ? *reinterpret_cast<const float4*>(w + 4 + lane * 4) : make_float4(0, 0, 0, 0);
     }
     const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
-    const float base = now == -INFINITY ? 0.0f : now;
-    const float keep = exp2f(top - base);
-    sum *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
-    top = now;
+    const float now_v = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])), top_v);
+    const float base = now == -INFINITY ? 0.0f : now, base_v = now_v == -INFINITY ? 0.0f : now_v;
+    const float keep = exp2f(top_v - base_v);
+    sum *= exp2f(top - base);
+    o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+    top = now, top_v = now_v;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float by = exp2f(m[u] - base);
-      sum += l[u] * by;
+      const float by = exp2f(mv[u] - base_v);
+      sum += l[u] * exp2f(m[u] - base);
       o.x += v[u].x * by, o.y += v[u].y * by, o.z += v[u].z * by, o.w += v[u].w * by;
     }
   }
   values[warp][lane] = o;
-  if (lane == 0) sums[warp] = sum, tops[warp] = top;
+  if (lane == 0) sums[warp] = sum, tops[warp] = top, tops_v[warp] = top_v;
   __syncthreads();
   if (warp) return;
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
-  const float base = top == -INFINITY ? 0.0f : top;
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]), top_v = fmaxf(top_v, tops_v[w]);
+  const float base = top == -INFINITY ? 0.0f : top, base_v = top_v == -INFINITY ? 0.0f : top_v;
   sum = 0.0f, o = make_float4(0, 0, 0, 0);
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
-    const float by = exp2f(tops[w] - base);
+    const float by = exp2f(tops_v[w] - base_v);
     const float4 v = values[w][lane];
-    sum += sums[w] * by;
+    sum += sums[w] * exp2f(tops[w] - base);
     o.x += v.x * by, o.y += v.y * by, o.z += v.z * by, o.w += v.w * by;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (lane * 4 < int(k.cache.head_dim)) {
     KvPack<T, 4> y;
-    y.v[0] = kv_from_float<Q>(o.x * inv);
-    y.v[1] = kv_from_float<Q>(o.y * inv);
-    y.v[2] = kv_from_float<Q>(o.z * inv);
-    y.v[3] = kv_from_float<Q>(o.w * inv);
+    y.v[0] = kv_from_float<Q>(in_units(o.x * inv, base_v - base));
+    y.v[1] = kv_from_float<Q>(in_units(o.y * inv, base_v - base));
+    y.v[2] = kv_from_float<Q>(in_units(o.z * inv, base_v - base));
+    y.v[3] = kv_from_float<Q>(in_units(o.w * inv, base_v - base));
     *reinterpret_cast<KvPack<T, 4>*>(reinterpret_cast<T*>(k.a.out.data) + int64_t(token) * k.a.out.token_stride +
                                      int64_t(qh) * k.a.out.head_stride + lane * 4) = y;
   }

@@ -138,7 +138,7 @@ def test_attention_scales_of_any_size_in_chunks(cuda, pattern, q_type, store, wi
 
 @pytest.mark.parametrize("ratio", [14, 20, 24, 40, 90])
 @pytest.mark.parametrize("q_type, store", [("bf16", "e4m3"), ("fp16", "int8")])
-@pytest.mark.parametrize("pattern", ["chunk", "mixed"])
+@pytest.mark.parametrize("pattern", ["decode", "verify", "chunk", "mixed"])
 def test_attention_far_scale_of_small_weight(cuda, pattern, q_type, store, ratio):
     """Each sequence's first token, which all of it see, has a V scale 2^ratio times the mean of all (with those planted
     before it, so they grow from sequence to sequence) and a weight of about e^-90: as long as that is the smaller, the
@@ -156,10 +156,42 @@ def test_attention_far_scale_of_small_weight(cuda, pattern, q_type, store, ratio
             vs[b, 0] = vs.mean() * 2.0 ** ratio
 
     for hints in (True, False):
-        o, lse, want, wl, mag, dot, _ = run_attention(torch, q_type, store, 128, 2, 4, 16, counts, lens, seed=30, edit=edit,
-                                                      hints=hints)
+        o, _, _, _, _, _, (cache, q, table, _, _) = run_attention(torch, q_type, store, 128, 2, 4, 16, counts, lens, seed=30,
+                                                                  edit=edit, hints=hints)
+        # A value is code * scale in fp32: the last sequence's first token of four (ratio 40) has 448 * 4.4e36 = 2e39, an
+        # infinity there, and so have its rows.
+        values = dense(torch, cache.value, cache.value_scale).float().double()
+        want, wl, mag, dot = attend_plain(torch, q, dense(torch, cache.key, cache.key_scale), values, lens, counts, table,
+                                          16, 1 / math.sqrt(128))
         tol, tol_l = scales_bound(torch, o, want, mag, dot, max(lens))
         # Rows that see the first token alone have it whole, and fp16 does not hold it then.
         on = want.abs() + tol < torch.finfo(o.dtype).max
         off = (o.double() - want).abs()
         assert (off[on] <= tol[on]).all(), f"worst {(off / tol)[on].max().item():.2f} of the bound"
+
+
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("pattern", ["decode", "decode_long", "verify", "chunk", "mixed"])
+@pytest.mark.parametrize("power", [97, -85, "any"])
+def test_attention_scales_near_the_ends(cuda, pattern, store, power):
+    """V scales of 2^90 and of 2^-92, which bf16 results hold as well as others, and of every size between 2^-117 and
+    2^108: both kernels, with and without the hints that choose between them."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+
+    def edit(k, v, ks, vs, table, q):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        vs *= 2.0 ** power if power != "any" else torch.exp2(torch.randint(-110, 115, vs.shape, generator=g,
+                                                                           device="cuda").float())
+
+    for hints in (True, False):
+        o, lse, want, wl, mag, dot, _ = run_attention(torch, "bf16", store, 128, 2, 4, 16, counts, lens, seed=31, edit=edit,
+                                                      hints=hints)
+        tol, tol_l = scales_bound(torch, o, want, mag, dot, max(lens))
+        if power == "any":
+            # Decoding: half of fp16's smallest step, 2^-25 of the row's largest weight times scale, for each code.
+            tol = tol + max(lens) * 2.0 ** -25 * mag.amax(2, keepdim=True) * 4
+        off = (o.double() - want).abs()
+        assert (off <= tol).all(), f"worst {(off / tol).max().item():.2f} of the bound"
+        seen = ~torch.isinf(wl)
+        assert ((lse.double() - wl).abs()[seen] <= (tol_l + wl.abs() * 2.0 ** -23)[seen]).all()
