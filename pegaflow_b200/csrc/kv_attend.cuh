@@ -12,6 +12,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 // powers of two): the exponentials stay below 2^8, which fp16, bf16 and the
 // fp32 sums hold as well as 1, and the accumulators are rescaled rarely.
 constexpr float kRaise = 8.0f;
+// Where weights become fp16 they are taken this many powers of two up: with kRaise and V scales (below 4) they still end
+// at 2^15, and small ones keep fp16's 11 bits down to 2^-21 (2^-19 with V scales) of the row's largest instead of 2^-14.
+// A row whose strong tokens hold nothing is what many small weights add up to.
+constexpr float kLift = 7.0f;
+constexpr float kLiftScaled = 5.0f;
 
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;

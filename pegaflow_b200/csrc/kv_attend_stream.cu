@@ -139,6 +139,9 @@ struct Stream {
   // An fp16 result over codes: its own rounding is no larger than the weights', so theirs is made good by a second
   // product with what it left (3.2e-4 off in all without, 2.1e-4 with; HBM bounds the kernel, not the products).
   static constexpr bool kExact = kQuant && Q == PF_DTYPE_FP16;
+  // Powers of two that weights (times V scales) are taken up when they become fp16, and that their sum goes with them.
+  static constexpr float kUp = kBf16 ? 0.0f : kQuant ? kLiftScaled : kLift;
+  static constexpr float kSumUp = kQuant ? 0.0f : kUp;
   static constexpr int kElt = kQuant ? 1 : 2;
   static constexpr int kRows = 8 * NT;
   static constexpr int kChunk = 16 / kElt;           // values of 16 bytes
@@ -435,17 +438,17 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          raise = raise || fmaxf(x[n][e], x[n][e + 2]) > m[n][e] + kRaise;
-          if constexpr (S::kQuant) raise = raise || fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent) > mv[n][e] + kRaise;
+          raise = raise || fmaxf(x[n][e], x[n][e + 2]) > m[n][e] + (kRaise + S::kSumUp);
+          if constexpr (S::kQuant) raise = raise || fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent) > mv[n][e] + (kRaise + S::kUp);
         }
       }
       if (__any_sync(0xffffffffu, raise)) {
-        // The old maximum's share of the new one's units, which becomes the old one.
-        auto raised = [](float& old, float top) {
+        // What weights go by becomes the maximum less the lift; returns what that makes of earlier ones.
+        auto raised = [](float& old, float top, float up) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          top = fmaxf(top, old);
+          top = fmaxf(top - up, old);
           const float keep = top == -INFINITY ? 0.0f : fast_exp2(old - top);
           old = top;
           return keep;
@@ -455,9 +458,9 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
           float keep[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            keep[e] = raised(m[n][e], fmaxf(x[n][e], x[n][e + 2]));
+            keep[e] = raised(m[n][e], fmaxf(x[n][e], x[n][e + 2]), S::kSumUp);
             l[n][e] *= keep[e];
-            if constexpr (S::kQuant) keep[e] = raised(mv[n][e], fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent));
+            if constexpr (S::kQuant) keep[e] = raised(mv[n][e], fmaxf(x[n][e] + v0.exponent, x[n][e + 2] + v1.exponent), S::kUp);
           }
 #pragma unroll
           for (int y = 0; y < S::kTiles; ++y) {

@@ -554,17 +554,18 @@ __device__ __forceinline__ float2 weights32(uint32_t (&p)[16], const float2 (&y)
 
 // What a row's softmax carries from tile to tile.
 struct RowState {
-  float m;  // the maximum that the weights go by
+  float m;  // what the weights go by: 2^(score - m). The maximum less the lift
   float l;  // their sum
 };
 
 // One tile's scores of a row into weights 2^(score f - m), 16-bit pairs over the
 // scores in TMEM, 32 scores at a time. m stays as long as no score passes it by
-// kRaise. Where one does (or the row had none yet), m becomes the largest score so
-// far, and the sum, O (o_columns of it) and the weights already made follow.
+// kRaise more than the lift. Where one does (or the row had none yet), m becomes the
+// largest score so far less the lift, and the sum, O (o_columns of it) and the weights already made follow.
 template <bool QUANT, bool SCALED, bool BF16, bool MASKED>
 __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, uint32_t s_at, uint32_t o_at, int o_columns,
                                             int32_t lo, int32_t hi, float f) {
+  constexpr float kUp = BF16 ? 0.0f : SCALED ? kLiftScaled : kLift;
   float2 all = make_float2(row.l, 0.0f);
   const float2 ff = make_float2(f, f);
   uint32_t s[32];
@@ -600,7 +601,7 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
 #pragma unroll
     for (int x = 0; x < 16; ++x) tops[x & 3] = max3_nan(tops[x & 3], y[x].x, y[x].y);
     const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-    const bool raise = top > (row.m == -INFINITY ? -INFINITY : kRaise);  // a NaN raises nothing: it reaches the sum
+    const bool raise = top > (row.m == -INFINITY ? -INFINITY : kRaise + kUp);  // a NaN raises nothing: it reaches the sum
     if (__any_sync(0xffffffffu, raise)) {
       // What is read back below was stored asynchronously (weights of pieces before, O by a rescaling), and the next
       // scores are still on their way into registers that a call may save: both are waited for first.
@@ -608,9 +609,9 @@ __device__ __forceinline__ void row_weights(RowState& row, const KeyInfo& info, 
       tmem_wait_store();
       float keep = 1.0f;
       if (raise) {
-        const float m = base + top;
+        const float by = top - kUp, m = base + by;
         keep = fast_exp2(row.m - m);  // 0 at first
-        const float2 shift = make_float2(-top, -top);
+        const float2 shift = make_float2(-by, -by);
 #pragma unroll
         for (int x = 0; x < 16; ++x) y[x] = add2(y[x], shift);
         row.m = m;

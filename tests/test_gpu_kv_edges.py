@@ -195,3 +195,40 @@ def test_attention_scales_near_the_ends(cuda, pattern, store, power):
         assert (off <= tol).all(), f"worst {(off / tol).max().item():.2f} of the bound"
         seen = ~torch.isinf(wl)
         assert ((lse.double() - wl).abs()[seen] <= (tol_l + wl.abs() * 2.0 ** -23)[seen]).all()
+
+
+# ----------------------------------------------------- small weights, many
+
+@pytest.mark.parametrize("q_type, store", [("fp16", "fp16"), ("fp16", "int8"), ("bf16", "e4m3"), ("fp16", "e4m3"),
+                                           ("bf16", "bf16")])
+@pytest.mark.parametrize("pattern", ["decode", "decode_long", "verify", "chunk", "mixed"])
+def test_attention_small_weights_beside_a_strong_one(cuda, pattern, q_type, store):
+    """Every 32nd token takes almost all the weight and has a V of zero: the result is what the others add up to, each
+    with a weight of 20.5 * 2^-24 (about) of it. In fp16 units of the largest that would be 20 or 21 of the smallest
+    steps; with the weights taken 2^5 up, 656."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+    dim, weight = 128, 20.5 * 2.0 ** -24
+
+    def edit(k, v, ks, vs, table, q):
+        q.fill_(1.0)
+        strong = -math.log(weight) / math.sqrt(dim)
+        if ks is None:
+            k.zero_(), v.fill_(1.0)
+        else:
+            k.zero_(), v.copy_(torch.full_like(v.float(), 96.0).to(v.dtype))
+            ks.fill_(strong / 96.0), vs.fill_(1.0 / 96.0)
+        for s, length in enumerate(lens):
+            for j in range(0, length, 32):
+                at = int(table[s, j // 16]), j % 16
+                k[at] = torch.full_like(k[at].float(), strong if ks is None else 96.0).to(k.dtype)
+                v[at] = torch.zeros_like(v[at].float()).to(v.dtype)
+
+    o, lse, want, wl, mag, dot, _ = run_attention(torch, q_type, store, dim, 2, 4, 16, counts, lens, seed=33, edit=edit)
+    tol, _ = attend_bound(torch, o.dtype, store in QMAX, want, mag, dot, max(lens), dim)
+    # Half of fp16's smallest step beside weights of 656 of them; the strong key's rounding moves these by 0.4 % at most.
+    tol = tol + mag / (2 * 650)
+    if o.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    off = (o.double() - want).abs()
+    assert (off <= tol).all(), f"worst {(off / tol).max().item():.2f} of the bound"
