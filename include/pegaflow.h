@@ -621,7 +621,8 @@ typedef struct pf_kv_rows {
  *   scale = max(max|x| / q, 2^-126),  code = round(clamp(x * (1 / scale), -q, q))
  * in fp32, with q = 448 (E4M3) or 127 (INT8), ties to even. A row that holds a
  * NaN or an infinity reads back as NaN. With given_scales != 0 the scales are
- * read, not written, and values beyond them saturate. */
+ * read, not written, and values beyond them saturate; 1 / scale is then at most
+ * fp32's largest, so that zeros under a scale of 0 (none set yet) are zeros. */
 int pf_kv_write(int32_t device_id, const pf_kv_cache* cache, uint64_t key,
                 int64_t key_token_stride, int64_t key_head_stride,
                 uint64_t value, int64_t value_token_stride,

@@ -32,6 +32,13 @@ __device__ __forceinline__ float row_scale(float top) {
   return s < kKvSmallestScale ? kKvSmallestScale : s == INFINITY ? NAN : s;
 }
 
+// 1 / a given scale. Of none (0), or one so small that it would be infinite, the largest there is: values saturate,
+// and zeros stay zeros, which an infinity would make NaN.
+__device__ __forceinline__ float inverse(float s) {
+  const float inv = 1.0f / s;
+  return fabsf(inv) == INFINITY ? copysignf(3.402823466e38f, inv) : inv;
+}
+
 // Values of a row that a thread moves when reading: 16 bytes of a 16-bit result, so
 // that a warp's stores fill whole sectors (with 16 codes and two stores 32 bytes
 // apart, 10,240 tokens of 8 x 128 took 15.1 us instead of 12.1).
@@ -96,18 +103,17 @@ __device__ __forceinline__ void write_elements(const pf_kv_rows& rows, const pf_
   if constexpr (STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8) {
     float* sp = reinterpret_cast<float*>(side.scale) + block * side.scale_block_stride + offset * side.scale_token_stride +
                 int64_t(head) * side.scale_head_stride;
-    float s;
     if (given) {
-      s = on ? *sp : 1.0f;
+      inv = inverse(on ? *sp : 1.0f);
     } else {
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
       for (uint32_t w = (1u << log_l) >> 1; w; w >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, w));
-      s = row_scale<STORE>(__uint_as_float(top));
+      const float s = row_scale<STORE>(__uint_as_float(top));
       if (on && lane == 0) *sp = s;
+      inv = 1.0f / s;
     }
-    inv = 1.0f / s;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -321,12 +327,11 @@ __global__ void __launch_bounds__(kThreads, kWriteBlocks<IN>) kv_write_rows_kern
     S* vp = address<S>(a.cache.value.data, plan.strides.value, block, offset, head) + d;
     if constexpr (kQuant) {
       // Even lanes make K's scale, odd ones V's (a group of one lane both, one after the other).
-      float ks, vs, ki, vi;
+      float ki, vi;
       float* ksp = address<float>(a.cache.key.scale, plan.strides.key_scale, block, offset, head);
       float* vsp = address<float>(a.cache.value.scale, plan.strides.value_scale, block, offset, head);
       if (a.given_scales) {
-        ks = on ? *ksp : 1.0f, vs = on ? *vsp : 1.0f;
-        ki = 1.0f / ks, vi = 1.0f / vs;
+        ki = inverse(on ? *ksp : 1.0f), vi = inverse(on ? *vsp : 1.0f);
       } else {
         Tops<IN> tops(k, v);
         tops.over_group(plan.log_l);
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, kWriteBlocks<IN>) kv_write_rows_kern
           ki = odd ? other : inv, vi = odd ? inv : other;
           if (on && lane < 2) *(odd ? vsp : ksp) = s;
         } else {
-          ks = row_scale<STORE>(tops.of(false)), vs = row_scale<STORE>(tops.of(true));
+          const float ks = row_scale<STORE>(tops.of(false)), vs = row_scale<STORE>(tops.of(true));
           ki = 1.0f / ks, vi = 1.0f / vs;
           if (on) *ksp = ks, *vsp = vs;
         }

@@ -232,3 +232,56 @@ def test_attention_small_weights_beside_a_strong_one(cuda, pattern, q_type, stor
         tol = tol + 2.0 ** -25
     off = (o.double() - want).abs()
     assert (off <= tol).all(), f"worst {(off / tol).max().item():.2f} of the bound"
+
+
+# ------------------------------------------------------------- given scales
+
+@pytest.mark.parametrize("dim", [64, 20])
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+def test_write_given_scales_of_both_sides(cuda, store, dim):
+    """K and V by scales of their own, one for each block: rounded by them, saturated beyond, NaN kept (int8: 0); rows
+    of 16-byte pieces and odd ones."""
+    torch = cuda
+    from pegaflow_b200 import KVCache, kv_write
+
+    t = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}[store]
+    k, v = (torch.zeros((4, 16, 2, dim), dtype=t, device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(7)
+    scales = [torch.exp2(torch.randint(-5, 3, (4, 1, 1), generator=g, device="cuda").float()) * 1.3 for _ in range(2)]
+    cache = KVCache(k, v, *scales)
+    x = torch.randn((2, 9, 2, dim), generator=g, device="cuda") * 60
+    x[:, 3, 1, 5] = math.nan
+    x[:, 4, 0, 7], x[:, 4, 0, 8] = math.inf, -math.inf
+    slots = torch.randperm(64, generator=g, device="cuda")[:9]
+    kv_write(cache, x[0], x[1], slots, given_scales=True)
+    q = QMAX[store]
+    for codes, s, y in ((k, scales[0], x[0]), (v, scales[1], x[1])):
+        want = (y * (1.0 / s[slots // 16])).clamp(-q, q)  # both fp32 operations are correctly rounded; a NaN stays
+        got = codes[slots // 16, slots % 16].float()
+        if store == "int8":
+            want = want.round().nan_to_num(0.0)
+        else:
+            want = want.to(t).float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("dim", [64, 20])
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 2.0 ** -140])
+def test_write_given_scales_without_an_inverse(cuda, store, dim, scale):
+    """A scale that is not set yet (zero), or so small that 1 / scale is infinite: zeros stay zeros, which a product with
+    an infinity would make NaN, and other values saturate."""
+    torch = cuda
+    from pegaflow_b200 import KVCache, kv_write
+
+    t = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}[store]
+    k, v = (torch.zeros((2, 16, 2, dim), dtype=t, device="cuda") for _ in range(2))
+    cache = KVCache(k, v, *[torch.full((2, 1, 1), scale, device="cuda") for _ in range(2)])
+    x = torch.zeros((3, 2, dim), device="cuda")
+    x[1, 0, 3], x[1, 1, 4], x[2, 0, 0] = 5.0, -7.0, 0.25
+    kv_write(cache, x, -x, torch.tensor([1, 17, 30], device="cuda"), given_scales=True)
+    q = QMAX[store] * math.copysign(1.0, scale)
+    for codes, y in ((k, x), (v, -x)):
+        got = torch.stack([codes[0, 1], codes[1, 1], codes[1, 14]]).float()
+        assert torch.equal(got, y.sign() * q)
