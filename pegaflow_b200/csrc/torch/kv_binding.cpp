@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -83,6 +84,13 @@ Cache cache(PyObject* address, PyObject* index) {
   return Cache{reinterpret_cast<const pf_kv_cache*>(static_cast<uintptr_t>(integer(address))), int(integer(index))};
 }
 
+// The operators have no backward pass: a result or a cache without it would stop the gradient and say nothing.
+void need_no_gradient(const at::Tensor& t, const char* what) {
+  if (t.requires_grad() && c10::GradMode::is_enabled()) {
+    refuse(std::string(what) + " requires a gradient, which these operators do not compute: call them under torch.no_grad(), or detach it");
+  }
+}
+
 pf_kv_rows rows(const Cache& c, const at::Tensor& t, int64_t n, int64_t heads, const char* what) {
   const int64_t dim = c.c->head_dim;
   if (t.dim() != 3 || t.size(0) != n || t.size(1) != heads || t.size(2) != dim || t.get_device() != c.index ||
@@ -92,6 +100,7 @@ pf_kv_rows rows(const Cache& c, const at::Tensor& t, int64_t n, int64_t heads, c
       << shown(t.sizes()) << " with strides " << shown(t.strides()) << " on " << t.device();
     refuse(s.str());
   }
+  need_no_gradient(t, what);
   return pf_kv_rows{reinterpret_cast<uint64_t>(t.data_ptr()), t.stride(0), t.stride(1)};
 }
 

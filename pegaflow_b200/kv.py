@@ -14,7 +14,9 @@ Sizes, types and strides are checked before anything is queued (ValueError, or
 PegaError from the library); what only the device knows (slots, block ids,
 lengths) is skipped where it is out of range, and reported through ``status``,
 an int32 tensor that gets the bits BAD_BLOCK, BAD_LENGTH and TIMED_OUT (a wait
-within a kernel ran out: the outputs are not valid) ORed into it.
+within a kernel ran out: the outputs are not valid) ORed into it. They are for
+inference and have no backward pass: outside of ``torch.no_grad()`` tensors that
+require a gradient are refused.
 
 A cache that a transfer loads, or that ``kv_write`` fills, is read by the others
 as soon as their stream is behind it; the same tensors are registered with
@@ -85,6 +87,8 @@ class KVCache:
             _need(key_scale is None and value_scale is None, f"a cache of {key.dtype} has no scales")
         tensors = [t for t in (key, value, *scales) if t is not None]
         _need(all(t.device == key.device for t in tensors), "the cache's tensors must be on one device")
+        _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), "a cache cannot require a gradient, "
+              "which these operators do not compute: make it under torch.no_grad(), or detach it")
         self.key, self.value, self.key_scale, self.value_scale = key, value, *scales
         self.device, self.dtype = key.device, key.dtype
         # get_device(): -1 on the CPU, which every operator refuses.

@@ -285,3 +285,24 @@ def test_write_given_scales_without_an_inverse(cuda, store, dim, scale):
     for codes, y in ((k, x), (v, -x)):
         got = torch.stack([codes[0, 1], codes[1, 1], codes[1, 14]]).float()
         assert torch.equal(got, y.sign() * q)
+
+
+# ----------------------------------------------------------------- gradients
+
+def test_results_that_require_a_gradient(cuda):
+    """Outputs that autograd follows are refused, and are written under no_grad()."""
+    torch = cuda
+    from pegaflow_b200 import chunk_attention, kv_read
+
+    cache, k, v, ks, vs = make_cache(torch, "bf16", 2, 16, 2, 64, fill=5)
+    table, starts = torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([20], dtype=torch.int32, device="cuda")
+    x = torch.ones((3, 2, 64), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros_like(x).requires_grad_()
+    for call in (lambda: kv_read(cache, table, starts, out=(x, y)), lambda: chunk_attention(x, cache, table, starts, lens, out=y),
+                 lambda: chunk_attention(y, cache, table, starts, lens)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+    with torch.no_grad():
+        kv_read(cache, table, starts, out=(x, y))
+        assert torch.equal(y, v[1, :3])

@@ -35,3 +35,35 @@ def test_library_refuses_rows_that_a_tile_carries_past_an_int32(native):
 
     assert answer(2 ** 30 - 1) and answer(2 ** 30 - 2 ** 15 + 1)
     assert not answer(2 ** 30 - 2 ** 15)
+
+
+def test_operators_refuse_gradients():
+    """There is no backward pass: outside of no_grad() what requires a gradient is refused, not silently detached."""
+    import pytest
+    import torch
+
+    from pegaflow_b200 import KVCache, chunk_attention, kv_read, kv_write
+
+    def kv(grad=False):
+        return torch.zeros((2, 4, 16, 2, 64), dtype=torch.bfloat16, requires_grad=grad)
+
+    cache, x = KVCache.from_tensor(kv()), torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    y = x.clone().requires_grad_()
+    slots, table = torch.zeros(3, dtype=torch.int64), torch.zeros((1, 4), dtype=torch.int32)
+    q_start, kv_len = torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    calls = [lambda: chunk_attention(y, cache, table, q_start, kv_len), lambda: kv_write(cache, y, x, slots),
+             lambda: kv_write(cache, x, y, slots), lambda: kv_read(cache, table, q_start, out=(x, y)),
+             lambda: chunk_attention(x, cache, table, q_start, kv_len, out=y)]
+    for i, call in enumerate(calls):
+        # Results are looked at behind the device, which a cache of the CPU does not have.
+        words = "requires a gradient" if i < 3 else "requires a gradient|CUDA device"
+        with pytest.raises(ValueError, match=words):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+            call()
+        with torch.inference_mode(), pytest.raises(ValueError, match="CUDA device"):
+            call()
+    with pytest.raises(ValueError, match="cannot require a gradient"):
+        KVCache.from_tensor(kv(True))
+    with torch.no_grad():
+        KVCache.from_tensor(kv(True))
