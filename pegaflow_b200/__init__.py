@@ -12,6 +12,7 @@ broken library raises ImportError at that first use; there is no fallback.
 """
 
 import importlib
+import importlib.util
 
 _EXPORTS = {
     "PegaEngine": ".engine",
@@ -36,7 +37,8 @@ _EXPORTS = {
     "chunk_attention": ".kv",
 }
 
-__all__ = sorted(_EXPORTS)
+# `import *` takes the operators where torch is installed; by name they fail without it, with the reason.
+__all__ = sorted(n for n, m in _EXPORTS.items() if m != ".kv" or importlib.util.find_spec("torch"))
 
 
 def __getattr__(name):

@@ -3,7 +3,8 @@
 Every translation unit is compiled by nvcc for sm_100a only; the shared
 library lands next to this file so it travels with the source tree.
 The binding of the paged-cache operators for torch tensors (_kv_torch.so) is
-compiled with the host compiler against the installed torch and this library.
+compiled with the host compiler against the installed torch and this library;
+where torch is not installed it is left out.
 Run: python -m pegaflow_b200.build [--force]
 """
 
@@ -23,6 +24,7 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libpegaflow_b200.so"
 TORCH_BINDING = PKG / "_kv_torch.so"
+TORCH_STAMP = BUILD / "kv_torch.stamp"  # what the binding was built against
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = [
@@ -58,11 +60,27 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def _torch_command(src: Path, target: Path) -> list[str]:
-    import sysconfig
+def _torch_home() -> Path | None:
+    """Where torch is installed: found, not imported, as the build needs its headers alone."""
     from importlib.util import find_spec
 
-    torch = Path(find_spec("torch").origin).parent  # found, not imported: the build needs its headers alone
+    spec = find_spec("torch")
+    return Path(spec.origin).parent if spec and spec.origin else None
+
+
+def _torch_stamp(home: Path) -> str:
+    from importlib.metadata import PackageNotFoundError, version
+
+    try:
+        installed = version("torch")
+    except PackageNotFoundError:  # a source tree on the path
+        installed = "of no package"
+    return f"{home}\ntorch {installed}\npython {sys.version}\n"
+
+
+def _torch_command(src: Path, target: Path, torch: Path) -> list[str]:
+    import sysconfig
+
     cuda = Path(nvcc()).resolve().parent.parent
     includes = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
                 cuda / "include", ROOT / "include"]
@@ -72,8 +90,8 @@ def _torch_command(src: Path, target: Path) -> list[str]:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile and link the library and the torch binding if any source or
-    header changed."""
+    """Compile and link the library if any source or header changed, and the
+    torch binding if that or the installed torch did."""
     BUILD.mkdir(exist_ok=True)
     cc = nvcc()
     headers = _headers()
@@ -103,10 +121,18 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         run(cmd)
         os.replace(tmp, LIB)
     binding = CSRC / "torch" / "kv_binding.cpp"
-    if force or _stale(TORCH_BINDING, [binding, ROOT / "include" / "pegaflow.h", Path(__file__)]):
+    home = _torch_home()
+    if home is None:
+        if verbose:
+            print("torch is not installed: the binding of the paged-cache operators is left out", flush=True)
+        return LIB
+    stamp = _torch_stamp(home)
+    built_against = TORCH_STAMP.read_text() if TORCH_STAMP.exists() else None
+    if force or built_against != stamp or _stale(TORCH_BINDING, [binding, ROOT / "include" / "pegaflow.h", Path(__file__)]):
         tmp = TORCH_BINDING.with_suffix(".so.tmp")
-        run(_torch_command(binding, tmp))
+        run(_torch_command(binding, tmp, home))
         os.replace(tmp, TORCH_BINDING)
+        TORCH_STAMP.write_text(stamp)
     return LIB
 
 

@@ -67,3 +67,50 @@ def test_operators_refuse_gradients():
         KVCache.from_tensor(kv(True))
     with torch.no_grad():
         KVCache.from_tensor(kv(True))
+
+
+NO_TORCH = "import sys; sys.path.insert(0, '.'); sys.modules['torch'] = None\n"  # an import of it fails, and no spec is found
+
+
+def run_python(code, *args):
+    import sys
+
+    return subprocess.run([sys.executable, "-c", code, *args], cwd=ROOT, capture_output=True, text=True, timeout=600)
+
+
+def test_build_without_torch(native, tmp_path):
+    """The library is for C and Rust callers too: without torch it is built as before, and the binding is left out."""
+    out = run_python(NO_TORCH + "from pathlib import Path; from pegaflow_b200 import build as b\n"
+                     "b.TORCH_BINDING = Path(sys.argv[1]) / 'x.so'; b.TORCH_STAMP = Path(sys.argv[1]) / 'x.stamp'\n"
+                     "print(b.build()); print(list(Path(sys.argv[1]).iterdir()))", str(tmp_path))
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.split() == [str(native.LIB_PATH), "[]"]
+
+
+def test_import_without_torch(native):
+    out = run_python(NO_TORCH + "from pegaflow_b200 import *\nprint(Layout.__name__, PegaEngine.__name__, 'kv_write' in globals())\n"
+                     "import pegaflow_b200\ntry:\n    pegaflow_b200.kv_write\nexcept ImportError as e:\n    print('ImportError')")
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.split() == ["Layout", "PegaEngine", "False", "ImportError"]
+    import pegaflow_b200
+
+    assert {"kv_write", "kv_read", "chunk_attention", "KVCache"} <= set(pegaflow_b200.__all__)
+
+
+def test_binding_follows_the_installed_torch(native, tmp_path, monkeypatch):
+    """A binding that another torch (or Python) was there for is built again, without being asked to."""
+    import importlib.metadata
+
+    from pegaflow_b200 import build as b
+
+    built = tmp_path / "built"
+    monkeypatch.setattr(b, "TORCH_BINDING", tmp_path / "x.so")
+    monkeypatch.setattr(b, "TORCH_STAMP", tmp_path / "x.stamp", raising=False)
+    monkeypatch.setattr(b, "_torch_command", lambda src, target, *_: ["sh", "-c", f"echo x >> {built}; touch {target}"])
+    b.build()
+    b.build()
+    assert built.read_text() == "x\n"
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "9.9.9")
+    b.build()
+    b.build()
+    assert built.read_text() == "x\nx\n"
