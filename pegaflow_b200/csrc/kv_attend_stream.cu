@@ -203,16 +203,15 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
   const int g = lane >> 2, t = lane & 3;
   // Along x, the axis that has room for any number: the heads of a sequence side by side, because in most layouts
   // their rows of a token are, and run at the same time they meet in HBM's open pages.
-  const uint32_t part = blockIdx.y, item = blockIdx.x / c.heads, head = blockIdx.x - item * c.heads;
-  const uint32_t seq = item / plan.tiles;
+  const uint32_t part = blockIdx.y, seq = blockIdx.x / c.heads, head = blockIdx.x - seq * c.heads;
   const int32_t group = int32_t(k.a.q_heads / c.heads);
   let_next_kernel_start();
   auto page_of = [&](int32_t j) { return plan.page_shift >= 0 ? uint32_t(j) >> plan.page_shift : uint32_t(j) / c.block_size; };
 
   const KvSeq s = kv_sequence(k, seq);
   const int32_t rows = s.n * group;
-  // Tiles beyond the bound that the grid was made for are taken by its CTAs in turn.
-  for (int32_t row0 = int32_t(item % plan.tiles) * S::kRows; row0 < rows; row0 += int32_t(plan.tiles) * S::kRows) {
+  // One tile, unless a sequence has more queries than the bound that chose this kernel.
+  for (int32_t row0 = 0; row0 < rows; row0 += S::kRows) {
     const int32_t row_last = min(rows, row0 + S::kRows) - 1;
     const int32_t begin = kv_row_begin(k, s, row0 / group);
     const int32_t end = kv_row_end(k, s, row_last / group);
@@ -767,7 +766,7 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = 1, cluster.val.clusterDim.y = p.parts, cluster.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(k.a.n_seqs * p.tiles * k.cache.heads, p.parts);
+    cfg.gridDim = dim3(k.a.n_seqs * k.cache.heads, p.parts);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = shm;
     cfg.stream = stream;
@@ -775,7 +774,7 @@ cudaError_t launch_as(const KvAttendArgs& k, const KvStreamPlan& p, cudaStream_t
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, k, p);
   }
-  kernel<<<dim3(k.a.n_seqs * p.tiles * k.cache.heads, p.parts), kThreads, shm, stream>>>(k, p);
+  kernel<<<dim3(k.a.n_seqs * k.cache.heads, p.parts), kThreads, shm, stream>>>(k, p);
   if (p.parts == 1) return cudaGetLastError();
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
@@ -818,7 +817,6 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   p.page_shift = page_shift(k.cache);
   const uint32_t rows = most_queries(k) * (k.a.q_heads / k.cache.heads);
   p.row_tiles = rows <= 8 ? 1 : 2;
-  p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   uint64_t longest = uint64_t(k.a.max_blocks) * k.cache.block_size;
   if (k.a.max_kv) longest = std::min<uint64_t>(longest, k.a.max_kv);
   if (k.a.window) longest = std::min<uint64_t>(longest, uint64_t(k.a.window) + most_queries(k));
@@ -827,7 +825,7 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   // end (queries, addresses, joining: about 384 tokens' time). Few sequences: one round, whose parts are as short as
   // that leaves them. Many: sequences are rarely equally long, so among splits that are within a tenth of the best
   // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 286 us in one round, 221 in seven).
-  const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * p.tiles * k.cache.heads);
+  const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * k.cache.heads);
   const uint64_t slots = uint64_t(num_sms) * ctas_per_sm(k, p);
   const uint64_t units = (longest + kStreamMinPart - 1) / kStreamMinPart;  // shortest parts
   auto cost = [&](uint64_t per) {

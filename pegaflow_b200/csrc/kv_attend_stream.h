@@ -16,7 +16,6 @@ constexpr uint32_t kStreamMinPart = 128;  // tokens: a batch for each warp
 
 struct KvStreamPlan {
   uint32_t row_tiles;   // 8-row tiles of a CTA: 1 or 2
-  uint32_t tiles;       // CTAs side by side for a sequence's rows
   uint32_t parts;       // CTAs along the tokens
   int32_t part_tokens;  // tokens of a part, a multiple of kStreamMinPart
   int32_t page_shift;   // log2 of the block size, -1 if it is no power of two
