@@ -110,6 +110,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
 // y times 2^by, in two steps: the power alone may lie outside fp32.
 __device__ __forceinline__ float in_units(float y, float by) {
   const float half = exp2f(0.5f * by);
@@ -136,9 +142,11 @@ template <uint32_t Q, uint32_t STORE, int DP, int NT>
 struct Stream {
   static constexpr bool kQuant = STORE == PF_DTYPE_E4M3 || STORE == PF_DTYPE_INT8;
   static constexpr bool kBf16 = !kQuant && Q == PF_DTYPE_BF16;  // type of the products
-  // An fp16 result over codes: its own rounding is no larger than the weights', so theirs is made good by a second
-  // product with what it left (3.2e-4 off in all without, 2.1e-4 with; HBM bounds the kernel, not the products).
-  static constexpr bool kExact = kQuant && Q == PF_DTYPE_FP16;
+  // The rounding of the weights is made good by a second product with what it left: HBM bounds the kernel, not the
+  // products, and it takes no time (one sequence of 1,000 in bf16 8.2 us with and without, four of 32K 22.5; off by
+  // 1.6e-3 in all, the result's own rounding, without by 2.1e-3). Not where a bf16 result over codes has weights in fp16:
+  // they are eight times as fine as the result.
+  static constexpr bool kExact = !kQuant || Q == PF_DTYPE_FP16;
   // Powers of two that weights (times V scales) are taken up when they become fp16, and that their sum goes with them.
   static constexpr float kUp = kBf16 ? 0.0f : kQuant ? kLiftScaled : kLift;
   static constexpr float kSumUp = kQuant ? 0.0f : kUp;
@@ -486,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
         p[n][0] = transpose_8x8(first);
         p[n][1] = transpose_8x8(second);
         if constexpr (S::kExact) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&first)), b = __half22float2(*reinterpret_cast<const __half2*>(&second));
-          rest[n][0] = transpose_8x8(pack2<false>(w[0] - a.x, w[1] - a.y));
-          rest[n][1] = transpose_8x8(pack2<false>(w[2] - b.x, w[3] - b.y));
+          const float2 a = unpack2<S::kBf16>(first), b = unpack2<S::kBf16>(second);
+          rest[n][0] = transpose_8x8(pack2<S::kBf16>(w[0] - a.x, w[1] - a.y));
+          rest[n][1] = transpose_8x8(pack2<S::kBf16>(w[2] - b.x, w[3] - b.y));
         }
       }
       // V^T: the tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of this lane's values.
@@ -525,7 +533,10 @@ __global__ void __launch_bounds__(kThreads, (Stream<Q, STORE, DP, NT>::kCtas))
             const uint32_t a0 = __byte_perm(w[0][u], w[1][u], 0x5410), a1 = __byte_perm(w[0][u], w[1][u], 0x7632);
             const uint32_t a2 = __byte_perm(w[2][u], w[3][u], 0x5410), a3 = __byte_perm(w[2][u], w[3][u], 0x7632);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma<S::kBf16>(o[n][4 * j + u], a0, a1, a2, a3, p[n][0], p[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              mma<S::kBf16>(o[n][4 * j + u], a0, a1, a2, a3, p[n][0], p[n][1]);
+              if constexpr (S::kExact) mma<S::kBf16>(o[n][4 * j + u], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+            }
           }
         }
       }

@@ -306,3 +306,25 @@ def test_results_that_require_a_gradient(cuda):
     with torch.no_grad():
         kv_read(cache, table, starts, out=(x, y))
         assert torch.equal(y, v[1, :3])
+
+
+# ------------------------------------------------------- weights in 16 bits
+
+@pytest.mark.parametrize("q_type, store", [("bf16", "bf16"), ("fp16", "fp16"), ("fp16", "e4m3"), ("fp16", "int8")])
+@pytest.mark.parametrize("dim, heads, group", [(128, 2, 4), (64, 3, 1), (80, 1, 4)])
+@pytest.mark.parametrize("pattern", ["one", "decode", "decode_long", "verify"])
+def test_attention_decoding_keeps_the_weights(cuda, pattern, dim, heads, group, q_type, store):
+    """When decoding, what the rounding of a weight to 16 bits leaves has a product of its own: the result is off by its
+    own rounding, and by 2^-8 of 2^-8 (fp16: 2^-11 of 2^-11) of the weighted magnitudes."""
+    torch = cuda
+    counts, lens = PATTERNS[pattern]
+    o, lse, want, wl, mag, dot, _ = run_attention(torch, q_type, store, dim, heads, group, 16, counts, lens, seed=51)
+    u, quantised = torch.finfo(o.dtype).eps / 2, store in QMAX
+    tol, _ = attend_bound(torch, o.dtype, quantised, want, mag, dot, max(lens), dim)
+    tol = tol - (u - u * u) * mag * 1.01
+    if o.dtype == torch.float16:
+        # The rest of a small weight is rounded to half of fp16's smallest step, 2^-25, beside a largest weight (times V
+        # scale, of 1 to 2) of 2^5 at least, and values of 448 codes; results to half of the smallest step.
+        tol = tol + 2.0 ** -25 + max(lens) * 2.0 ** -30 * 2 * mag.amax(2, keepdim=True)
+    off = (o.double() - want).abs()
+    assert (off <= tol).all(), f"worst {(off / tol).max().item():.2f} of the bound"
