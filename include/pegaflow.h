@@ -654,8 +654,15 @@ int pf_kv_read(int32_t device_id, const pf_kv_cache* cache,
  * A query that sees nothing gets zeros and lse = -inf; tokens on a bad block
  * are not seen. Query heads are a multiple of the cache's: head h reads KV head
  * h / (q_heads / heads). Query rows outside the sequences are left as they
- * are; `out` is memory of its own. Types: queries and outputs bf16 or fp16, the cache the same type, E4M3
- * or INT8; head_dim a multiple of 16 up to 128; rows 16-byte aligned. */
+ * are; `out` is memory of its own. Types: queries and outputs bf16 or fp16, the
+ * cache the same type, E4M3 or INT8; head_dim a multiple of 16 up to 128; rows
+ * 16-byte aligned.
+ * Scores, maxima and sums are fp32. Weights are rounded to 16 bits in front of the
+ * second product: to bf16 over a bf16 cache, else to fp16, 11 bits down to 2^-19 of
+ * the row's largest (with V scales multiplied in: of its largest weight times
+ * scale), fewer below. With up to 16 rows for a KV head what that leaves is added
+ * (not for a bf16 result over 8 bits). With more rows over an 8-bit cache V scales
+ * that a row sees may cost 2^-11 of the row's largest value. */
 typedef struct pf_kv_attention {
   pf_kv_rows query;       /* [n_tokens, q_heads, head_dim] */
   pf_kv_rows out;
@@ -673,7 +680,8 @@ typedef struct pf_kv_attention {
   uint32_t q_heads;
   uint32_t dtype;         /* of query and out */
   /* Upper bounds of a sequence's queries and cached tokens, for the choice of
-   * kernel and split; results do not depend on them. 0 = not known. */
+   * kernel and split; results depend on them by no more than rounding. 0 = not
+   * known. */
   uint32_t max_q;
   uint32_t max_kv;
   float scale;

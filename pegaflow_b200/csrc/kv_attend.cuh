@@ -9,8 +9,8 @@ namespace pf {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // A part's running maximum is raised only when a score passes it by this (in
-// powers of two): the exponentials stay below 2^8, which fp16, bf16 and the
-// fp32 sums hold as well as 1, and the accumulators are rescaled rarely.
+// powers of two): the exponentials stay below 2^8 times the lift, which fp16, bf16
+// and the fp32 sums hold as well as 1, and the accumulators are rescaled rarely.
 constexpr float kRaise = 8.0f;
 // Where weights become fp16 they are taken this many powers of two up: with kRaise and V scales (below 4) they still end
 // at 2^15, and small ones keep fp16's 11 bits down to 2^-21 (2^-19 with V scales) of the row's largest instead of 2^-14.

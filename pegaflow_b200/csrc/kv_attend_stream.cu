@@ -7,7 +7,8 @@
 // maximum, its sums, its accumulators, joined at the end of the part. Parts of a
 // sequence are joined by their cluster, where they are one, or by a second kernel.
 // Measured: 64 sequences of 1K to 16K tokens, 32 heads on 8 of 128 over e4m3, 1.2 GB,
-// 221 us (5.4 TB/s); one of 1,000 in bf16 7.0 us, which are latency.
+// 252 us in calls without a pause (4.7 TB/s; 1,777 MHz under the power limit), 234 in
+// twenty (1,965 MHz); one of 1,000 in bf16 8.2 us, which are latency.
 //
 // Each warp copies its rows (16-byte cp.async, from wherever the block table says)
 // into a ring of its own in shared memory, two steps of 16 tokens ahead: with 8 to
@@ -835,7 +836,8 @@ KvStreamPlan stream_plan(const KvAttendArgs& k, int num_sms) {
   // Parts of equal length: the CTAs run in rounds of as many as fit, each round as long as a part and its start and
   // end (queries, addresses, joining: about 384 tokens' time). Few sequences: one round, whose parts are as short as
   // that leaves them. Many: sequences are rarely equally long, so among splits that are within a tenth of the best
-  // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens: 286 us in one round, 221 in seven).
+  // the finest is taken, which evens them out (64 sequences of 1K to 16K tokens, at 1,965 MHz: 286 us in one round, 221
+  // in seven).
   const uint64_t items = std::max<uint64_t>(1, uint64_t(k.a.n_seqs) * k.cache.heads);
   const uint64_t slots = uint64_t(num_sms) * ctas_per_sm(k, p);
   const uint64_t units = (longest + kStreamMinPart - 1) / kStreamMinPart;  // shortest parts

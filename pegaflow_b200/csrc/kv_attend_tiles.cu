@@ -11,8 +11,15 @@
 // 256 x 128 keys take 2,048; their 32,768 exponentials take the special-function
 // units (16 a clock) 2,048 too. m follows the row's maximum only when it rises by
 // 2^8 (kRaise): then, rarely, O is rescaled in TMEM by the threads of that tile.
-// Measured for 2,048 tokens, 32 heads on 8 of 128: after 10,240 in bf16 360 us (1,050
-// TFLOP/s), after 32,768 over e4m3 1.39 ms (816).
+// Measured for 2,048 tokens, 32 heads on 8 of 128, in calls without a pause, whose
+// clocks the power limit sets: after 10,240 in bf16 405 us (933 TFLOP/s at 1,750 MHz),
+// after 32,768 over e4m3 1.46 ms (775 at 1,890 MHz). Twenty calls, at 1,965 MHz: 361 us
+// and 1.41 ms. Times of variants below are of such short runs.
+//
+// P has the type of V: over bf16 its rounding to 8 bits is seen in the result (off by
+// 2.3e-3, 1.7e-3 being the result's own rounding; a second product for what it leaves,
+// as the streaming kernel has, would be half as much again of the tensor cores' work).
+// In fp16 it is taken 2^7 up (kLift), so that small weights keep their bits longer.
 //
 // Warps 0-3 and 4-7: the softmax of the two halves. Three or five: load Q, K and
 // V. The last: issues the products. mbarriers order them; every wait is bounded, and
@@ -28,7 +35,8 @@
 // scores. V's, divided by a power of two that follows the largest, multiply V there
 // where the result is bf16 (two roundings of 2^-11 beside its own of 2^-8), and the
 // fp32 weights where it is fp16 (2.9e-4 off in all, 4.0e-4 the other way, 2.1e-4
-// being its own rounding; 1.51 ms instead of 1.39 for 2,048 tokens after 32,768).
+// being its own rounding; 1.51 ms instead of 1.39 for 2,048 tokens after 32,768). Rows
+// that see V scales 2^14 apart are made again where it shows.
 // As in the streaming kernel a bf16 query is brought into fp16's range by a power
 // of two for each row.
 #include <cuda.h>

@@ -7,8 +7,10 @@
 // travel through one chain of shuffles, indexes are divided by multiplying, and a
 // thread has K and V in flight together. Rows that are not aligned for 16-byte
 // pieces go element by element in kernels of their own. Measured for 8 heads of 128
-// between bf16 and e4m3: 8,192 tokens written in 14.2 us (3.6 TB/s, instructions
-// bound it), 10,240 read in 11.8 us (5.4 TB/s).
+// between bf16 and e4m3, calls over changing inputs: 8,192 tokens written in 16.4 us
+// (3.1 TB/s: issue slots 68 % busy, the rest is latency, with one row read ahead),
+// 10,240 read in 13.2 to 16.4 us (4.8 to 3.9 TB/s). Over the same inputs again and
+// again, which L2 then holds, 14.3 and 12.3.
 #include <algorithm>
 
 #include "kv_device.cuh"

@@ -196,11 +196,12 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, block_table: torch.Tens
     (int32 ``[n_seqs + 1]``) and ``kv_len[s]`` (int32) tokens in the cache on the
     blocks ``block_table[s]`` (int32 ``[n_seqs, max_blocks]``), the chunk the last
     of them. A query at position p sees the tokens up to p (all of them without
-    ``causal``), with ``window`` the last ``window`` of those only. ``q_heads`` is
+    ``causal``), with ``window`` none at p - window or in front of it. ``q_heads`` is
     a multiple of the cache's heads; ``scale`` is 1 / sqrt(head_dim) by default.
 
     ``max_q`` and ``max_kv`` bound a sequence's new and cached tokens: they choose
-    the kernel and how far it splits long sequences, never the result.
+    the kernel and how far it splits long sequences, and change the result by no
+    more than rounding.
 
     Returns the output (``out``, or a new tensor like ``query``), and with
     ``return_lse`` the log of each row's sum of exponentials too, fp32
