@@ -37,8 +37,16 @@ _EXPORTS = {
     "chunk_attention": ".kv",
 }
 
+
+def _torch_found() -> bool:
+    try:
+        return importlib.util.find_spec("torch") is not None
+    except ValueError:  # a module of that name that was not imported from anywhere: a stand-in
+        return False
+
+
 # `import *` takes the operators where torch is installed; by name they fail without it, with the reason.
-__all__ = sorted(n for n, m in _EXPORTS.items() if m != ".kv" or importlib.util.find_spec("torch"))
+__all__ = sorted(n for n, m in _EXPORTS.items() if m != ".kv" or _torch_found())
 
 
 def __getattr__(name):

@@ -64,7 +64,10 @@ def _torch_home() -> Path | None:
     """Where torch is installed: found, not imported, as the build needs its headers alone."""
     from importlib.util import find_spec
 
-    spec = find_spec("torch")
+    try:
+        spec = find_spec("torch")
+    except ValueError:  # a stand-in of that name that was not imported from anywhere
+        spec = None
     return Path(spec.origin).parent if spec and spec.origin else None
 
 

@@ -97,6 +97,14 @@ def test_import_without_torch(native):
     assert {"kv_write", "kv_read", "chunk_attention", "KVCache"} <= set(pegaflow_b200.__all__)
 
 
+def test_import_beside_a_stand_in_for_torch(native):
+    """A module named torch that somebody put together (to run without it) has no spec, and looking for one raises."""
+    out = run_python("import sys, types; sys.path.insert(0, '.'); sys.modules['torch'] = types.ModuleType('torch')\n"
+                     "from pegaflow_b200 import *\nfrom pegaflow_b200 import build as b\nprint(Layout.__name__, b._torch_home())")
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.split() == ["Layout", "None"]
+
+
 def test_binding_follows_the_installed_torch(native, tmp_path, monkeypatch):
     """A binding that another torch (or Python) was there for is built again, without being asked to."""
     import importlib.metadata
